@@ -168,6 +168,43 @@ int sfl_attn_bwd(const SflAttnTensor* q, const SflAttnTensor* k, const SflAttnTe
 int sfl_rope_bwd(void* x_bf16, long ld, const float* cos, const float* sin, long rows, int cols,
                  int T, int head_dim, void* stream);
 
+/* ---------------------------------------------------------------- rotary -- */
+/* Heads of one tensor [B, heads, T, D], D contiguous; strides in elements.  weight (fp32 [D],
+ * NULL: no norm) scales the per-head RMS norm that precedes the rotation.  y may be x itself.
+ * Backward: dy is the gradient of the result, y receives the gradient of x. */
+typedef struct SflRotaryTensor {
+  const void* x;
+  void* y;
+  const void* dy;
+  const float* weight;
+  long x_b, x_h, x_t, y_b, y_h, y_t, dy_b, dy_h, dy_t;
+  int heads;
+} SflRotaryTensor;
+
+/* cos / sin fp32 [rows, rotated / 2]; positions int64 with strides pos_b, pos_t (NULL: token t
+ * is at position t).  Rotated lanes of a token whose position is not in [0, rows) become NaN. */
+typedef struct SflRotaryTable {
+  const float* cos;
+  const float* sin;
+  const int64_t* positions;
+  long pos_b, pos_t;
+  int rows;
+  int rotated;
+} SflRotaryTable;
+
+/* Rotates the first `rotated` lanes of every head of one or two tensors (queries and keys), after
+ * the norm where they have weights.  half_layout 0: pairs (2i, 2i+1), 1: pairs (i, i + rotated/2).
+ * inverse 1 turns by the opposite angle (the gradient of a rotation without norm).  dtype 0 bf16,
+ * 1 fp16, 2 fp32; D <= 256. */
+int sfl_rotary(const SflRotaryTensor* tensors, int count, const SflRotaryTable* table, int B, int T,
+               int D, float eps, int half_layout, int inverse, int dtype, void* stream);
+/* Gradients of the norm and rotation together: dx into y, weight gradients (fp32 [D], summed in a
+ * fixed order) into dw0 / dw1.  partial: sfl_rotary_bwd_partial_bytes of scratch. */
+long sfl_rotary_bwd_partial_bytes(int heads0, int heads1, int B, int T, int D);
+int sfl_rotary_bwd(const SflRotaryTensor* tensors, int count, const SflRotaryTable* table, int B,
+                   int T, int D, float eps, int half_layout, int dtype, float* partial,
+                   long partial_bytes, float* dw0, float* dw1, void* stream);
+
 /* ---------------------------------------------------------------- decode -- */
 /* Single-token attention: q [B,Hq,D], k/v [B,Hkv,N,D] (contiguous, 16-bit),
  * lengths int32 [B] (clamped to [0,N]), out [B,Hq,D].  Hq/Hkv in {1,2,4,8},

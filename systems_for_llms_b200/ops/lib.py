@@ -103,7 +103,8 @@ def register_signature(name: str, argtypes: list) -> None:
 
 
 # Kernels launched per call of each entry point (default 1, 0 for host-only calls).
-_KERNELS_PER_CALL = {"sfl_attn_bwd": 2, "sfl_embedding_bwd": 2, "sfl_block_forward": 7, "sfl_block_backward": 11,
+_KERNELS_PER_CALL = {"sfl_attn_bwd": 2, "sfl_rotary_bwd": 2, "sfl_rotary_bwd_partial_bytes": 0,
+                     "sfl_embedding_bwd": 2, "sfl_block_forward": 7, "sfl_block_backward": 11,
                      "sfl_block_saved_bytes": 0, "sfl_block_scratch_bytes": 0, "sfl_rmsnorm_bwd_blocks": 0, "sfl_sqnorm_blocks": 0,
                      "sfl_ipc_alloc": 0, "sfl_ipc_free": 0, "sfl_ipc_get_handle": 0,
                      "sfl_ipc_open_handle": 0, "sfl_ipc_close_handle": 0,
@@ -185,6 +186,23 @@ def stream_ptr() -> int:
     same lookup without the object.
     """
     return _raw_stream(_current_device())
+
+
+class on_device:
+    """Makes ``device`` current for a launch.  Cheaper than ``torch.cuda.device`` in the usual
+    case that it already is."""
+
+    def __init__(self, device: torch.device):
+        self._index = device.index
+
+    def __enter__(self) -> None:
+        self._previous = _current_device()
+        if self._index is not None and self._index != self._previous:
+            torch.cuda.set_device(self._index)
+
+    def __exit__(self, *exc) -> None:
+        if self._index is not None and self._index != self._previous:
+            torch.cuda.set_device(self._previous)
 
 
 def ptr(tensor: torch.Tensor | None) -> int | None:
