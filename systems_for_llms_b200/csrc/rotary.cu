@@ -14,8 +14,12 @@
 // accesses in flight: a lane owns eight consecutive elements of a head, a group of 4 to 32
 // lanes owns a head (so the norm is a few shuffles and the statistics never leave registers),
 // and a warp issues the loads of several head groups of one token before it uses the first.
-// The table row of the token is read once for all of them.  The backward pass recomputes the
-// statistics from x, which it has to read anyway, instead of storing them.
+// The table row of the token is read once for all of them and multiplied by the weights, so that
+// a head costs two products per element; partners of the half layout travel between lanes as the
+// 16-bit pairs they were loaded as.  (A first form with a product per weight, fp32 exchanges,
+// IEEE division and 64-bit index arithmetic issued 255 instructions per head group and was bound
+// by them: 1.4 ms where this takes a fifth.)  The backward pass recomputes the statistics from x,
+// which it has to read anyway, instead of storing them.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -47,7 +51,6 @@ struct Side {
   const float* weight;
   long x_b, x_h, x_t, y_b, y_h, y_t, dy_b, dy_h, dy_t;
   int heads;
-  int vec;            // every row of x, y (and dy) starts on a 16-byte boundary
 };
 
 struct RotaryParams {
@@ -61,6 +64,9 @@ struct RotaryParams {
   int B, T, D;
   int group;          // lanes per head (power of two)
   float eps, sign;    // sign -1 turns by the opposite angle
+  float inv_dim;
+  int chunks0, chunks1;  // warp items per token on each side
+  int tokens;
   float* partial;     // backward with norm: [blocks, D]
 };
 
@@ -79,14 +85,14 @@ template <> __device__ __forceinline__ __half from_f32(float v) { return __float
 // loads in flight hold 16 bytes (32 for fp32) of registers per lane.
 template <typename T> struct Raw { T v[kVec]; };
 
-template <typename T>
-__device__ __forceinline__ void load_raw(Raw<T>& r, const T* row, int e0, int D, bool vec,
-                                         bool live) {
-  if (live && vec) {
+template <bool VEC, typename T>
+__device__ __forceinline__ void load_raw(Raw<T>& r, const T* row, int e0, int D, bool live) {
+  if constexpr (VEC) {
     const uint4* src = reinterpret_cast<const uint4*>(row + e0);
     uint4* dst = reinterpret_cast<uint4*>(r.v);
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(Raw<T>) / 16); ++i) dst[i] = src[i];
+    for (int i = 0; i < static_cast<int>(sizeof(Raw<T>) / 16); ++i)
+      dst[i] = live ? src[i] : make_uint4(0, 0, 0, 0);
   } else {
 #pragma unroll
     for (int i = 0; i < kVec; ++i)
@@ -94,12 +100,12 @@ __device__ __forceinline__ void load_raw(Raw<T>& r, const T* row, int e0, int D,
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void store_raw(T* row, const float (&f)[kVec], int e0, int D, bool vec) {
+template <bool VEC, typename T>
+__device__ __forceinline__ void store_raw(T* row, const float (&f)[kVec], int e0, int D) {
   Raw<T> r;
 #pragma unroll
   for (int i = 0; i < kVec; ++i) r.v[i] = from_f32<T>(f[i]);
-  if (vec) {
+  if constexpr (VEC) {
     uint4* dst = reinterpret_cast<uint4*>(row + e0);
     const uint4* src = reinterpret_cast<const uint4*>(r.v);
 #pragma unroll
@@ -164,42 +170,61 @@ __device__ __forceinline__ void load_angles(const RotaryParams& p, int b, int t,
   }
 }
 
-// Turns the pairs of u in place.  All lanes of the warp take part.  Lanes beyond the rotated
-// ones keep their value untouched: multiplying by S = 0 would make NaN of an infinity.
-template <int PAIR>
-__device__ __forceinline__ void turn(const RotaryParams& p, float (&u)[kVec], const float (&C)[kVec],
-                                     const float (&S)[kVec], int e0, int lane, float* strip) {
-  if constexpr (PAIR == kInterleaved) {
-#pragma unroll
-    for (int i = 0; i < kVec; i += 2) {
-      if (e0 + i < p.rotated) {
-        const float a = u[i], b = u[i + 1];
-        u[i] = fmaf(a, C[i], b * S[i]);
-        u[i + 1] = fmaf(b, C[i + 1], a * S[i + 1]);
-      }
-    }
-  } else if constexpr (PAIR == kHalfShuffle) {
+// The other element of each pair, as loaded.  All lanes of the warp take part.  Lanes beyond the
+// rotated ones get zeros: S is zero there, and an infinity times zero would be NaN.
+template <typename T, int PAIR>
+__device__ __forceinline__ void partners(const RotaryParams& p, const Raw<T>& mine, Raw<T>& other,
+                                         int e0, int lane, T* strip) {
+  if constexpr (PAIR == kHalfShuffle) {
     const int half = p.rotated >> 1;
-    const int apart = half / kVec;
-    const int src = e0 < half ? lane + apart : (e0 < p.rotated ? lane - apart : lane);
+    const bool turns = e0 < p.rotated;
+    const int src = turns ? (e0 < half ? lane + half / kVec : lane - half / kVec) : lane;
+    constexpr int kWords = static_cast<int>(sizeof(Raw<T>) / 4);
+    const uint32_t* from = reinterpret_cast<const uint32_t*>(mine.v);
+    uint32_t* to = reinterpret_cast<uint32_t*>(other.v);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const float other = __shfl_sync(0xffffffffu, u[i], src);
-      if (e0 < p.rotated) u[i] = fmaf(u[i], C[i], other * S[i]);
+    for (int i = 0; i < kWords; ++i) {
+      const uint32_t got = __shfl_sync(0xffffffffu, from[i], src);
+      to[i] = turns ? got : 0u;
     }
-  } else {
+  } else if constexpr (PAIR == kHalfShared) {
     const int half = p.rotated >> 1;
-    float* mine = strip + (lane - e0 / kVec) * kVec;  // the head's first element
+    const T* head = strip + (lane * kVec - e0);  // the head's first element
     __syncwarp();
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) strip[lane * kVec + i] = u[i];
+    for (int i = 0; i < kVec; ++i) strip[lane * kVec + i] = mine.v[i];
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
       const int e = e0 + i;
-      if (e < p.rotated) u[i] = fmaf(u[i], C[i], mine[e < half ? e + half : e - half] * S[i]);
+      other.v[i] = e < p.rotated ? head[e < half ? e + half : e - half] : from_f32<T>(0.f);
     }
   }
+}
+
+// f_e = own_e C_e + partner_e S_e
+template <typename T, int PAIR>
+__device__ __forceinline__ void combine(const RotaryParams& p, const Raw<T>& mine,
+                                        const Raw<T>& other, const float (&C)[kVec],
+                                        const float (&S)[kVec], int e0, float (&f)[kVec]) {
+#pragma unroll
+  for (int i = 0; i < kVec; ++i) {
+    if constexpr (PAIR == kInterleaved) {
+      f[i] = to_f32(mine.v[i]) * C[i];
+      if (e0 + (i & ~1) < p.rotated) f[i] = fmaf(to_f32(mine.v[i ^ 1]), S[i], f[i]);
+    } else {
+      f[i] = fmaf(to_f32(other.v[i]), S[i], to_f32(mine.v[i]) * C[i]);
+    }
+  }
+}
+
+// The element whose weight multiplies the partner of element e.
+template <int PAIR>
+__device__ __forceinline__ int partner_of(const RotaryParams& p, int e) {
+  if (e >= p.rotated) return e;
+  if constexpr (PAIR == kInterleaved) return e ^ 1;
+  const int half = p.rotated >> 1;
+  return e < half ? e + half : e - half;
 }
 
 __device__ __forceinline__ float group_sum(float v, int group) {
@@ -222,136 +247,142 @@ __device__ __forceinline__ Where where(const RotaryParams& p) {
   return w;
 }
 
-// One warp takes PER head groups of one token.  Measured on B200 (training microbatches,
-// L2-cold): PER = 4 keeps enough bytes in flight; PER = 1 is for calls with few tokens, which
-// are over sooner when every head group has a warp of its own.
-template <typename T, int PAIR, bool NORM, int PER>
-__global__ void __launch_bounds__(32 * kWarps)
+// One warp takes PER head groups of one token.  PER = 4 keeps 2 KB of loads in flight per warp;
+// PER = 1 is for calls with few tokens, which are over sooner when every head group has a warp
+// of its own (16 tokens x 40 heads x 128: 3.0 us against 3.9 us).
+template <typename T, int PAIR, bool VEC, bool NORM, int PER>
+__global__ void __launch_bounds__(32 * kWarps, PER == 4 && VEC && sizeof(T) == 2 ? 4 : 2)
 rotary_kernel(const __grid_constant__ RotaryParams p) {
-  __shared__ float strips[PAIR == kHalfShared ? kWarps * 32 * kVec : 1];
+  __shared__ T strips[PAIR == kHalfShared ? kWarps * 32 * kVec : 1];
   pdl_launch_dependents();
   pdl_wait();
-  const bool first = static_cast<int>(blockIdx.x) < p.blocks0;
+  const unsigned chunks = p.chunks0 + p.chunks1;
+  const unsigned block_token = blockIdx.x / chunks;
+  int chunk = blockIdx.x - block_token * chunks;
+  const bool first = chunk < p.chunks0;
+  if (!first) chunk -= p.chunks0;
   const Side& s = p.side[first ? 0 : 1];
-  const int block = first ? blockIdx.x : blockIdx.x - p.blocks0;
   const int warp = threadIdx.x >> 5;
   const Where w = where(p);
-  float* strip = strips + (PAIR == kHalfShared ? warp * 32 * kVec : 0);
+  T* strip = strips + (PAIR == kHalfShared ? warp * 32 * kVec : 0);
   const int heads_per = 32 / p.group;
-  const int chunks = (s.heads + heads_per * PER - 1) / (heads_per * PER);
-  const long item = static_cast<long>(block) * kWarps + warp;
-  const long token = item / chunks;
-  if (token >= static_cast<long>(p.B) * p.T) return;  // warp-uniform
-  const int h0 = static_cast<int>(item - token * chunks) * heads_per * PER + w.sub;
-  const int b = static_cast<int>(token / p.T), t = static_cast<int>(token - static_cast<long>(b) * p.T);
-  const T* x = static_cast<const T*>(s.x) + b * s.x_b + t * s.x_t;
-  T* y = static_cast<T*>(s.y) + b * s.y_b + t * s.y_t;
+  const unsigned token = block_token * kWarps + warp;
+  if (token >= static_cast<unsigned>(p.tokens)) return;  // warp-uniform
+  const int b = token / static_cast<unsigned>(p.T), t = token - b * p.T;
+  const int h0 = chunk * heads_per * PER + w.sub;
+  const T* x = static_cast<const T*>(s.x) + b * s.x_b + t * s.x_t + h0 * s.x_h;
+  T* y = static_cast<T*>(s.y) + b * s.y_b + t * s.y_t + h0 * s.y_h;
 
   Raw<T> raw[PER];
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    const int h = h0 + j * heads_per;
-    load_raw(raw[j], x + static_cast<long>(h) * s.x_h, w.e0, p.D, s.vec, w.live && h < s.heads);
-  }
-  float C[kVec], S[kVec], weight[kVec];
+  for (int j = 0; j < PER; ++j)
+    load_raw<VEC>(raw[j], x + j * heads_per * s.x_h, w.e0, p.D,
+                  w.live && h0 + j * heads_per < s.heads);
+  float C[kVec], S[kVec];
   load_angles<PAIR>(p, b, t, w.e0, C, S);
   if constexpr (NORM) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) weight[i] = w.e0 + i < p.D ? s.weight[w.e0 + i] : 0.f;
+    for (int i = 0; i < kVec; ++i) {
+      const int e = w.e0 + i;
+      C[i] *= e < p.D ? s.weight[e] : 0.f;
+      S[i] *= e < p.D ? s.weight[partner_of<PAIR>(p, e)] : 0.f;
+    }
   }
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    const int h = h0 + j * heads_per;
-    float u[kVec];
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) u[i] = to_f32(raw[j].v[i]);
+    float rstd = 1.f;
     if constexpr (NORM) {
       float sq = 0.f;
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) sq = fmaf(u[i], u[i], sq);
-      sq = group_sum(sq, p.group);
-      const float rstd = 1.0f / sqrtf(sq / p.D + p.eps);
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) u[i] = u[i] * rstd * weight[i];
+      for (int i = 0; i < kVec; ++i) sq = fmaf(to_f32(raw[j].v[i]), to_f32(raw[j].v[i]), sq);
+      rstd = rsqrtf(fmaf(group_sum(sq, p.group), p.inv_dim, p.eps));
     }
-    turn<PAIR>(p, u, C, S, w.e0, w.lane, strip);
-    if (w.live && h < s.heads) store_raw(y + static_cast<long>(h) * s.y_h, u, w.e0, p.D, s.vec);
+    Raw<T> other;
+    partners<T, PAIR>(p, raw[j], other, w.e0, w.lane, strip);
+    float f[kVec];
+    combine<T, PAIR>(p, raw[j], other, C, S, w.e0, f);
+    if constexpr (NORM) {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) f[i] *= rstd;
+    }
+    if (w.live && h0 + j * heads_per < s.heads)
+      store_raw<VEC>(y + j * heads_per * s.y_h, f, w.e0, p.D);
   }
 }
 
 // Backward with the norm.  A persistent grid: every warp keeps the weight gradient of its
 // eight elements in registers over all its tokens; the block folds its warps in a fixed order
 // and leaves one row of partial sums (deterministic, no atomics).
-template <typename T, int PAIR, int PER>
-__global__ void __launch_bounds__(32 * kWarps)
+constexpr int kBwdBlocksPerSm = 3;
+
+template <typename T, int PAIR, bool VEC, int PER>
+__global__ void __launch_bounds__(32 * kWarps, VEC && sizeof(T) == 2 ? kBwdBlocksPerSm : 2)
 rotary_bwd_kernel(const __grid_constant__ RotaryParams p) {
-  __shared__ float strips[PAIR == kHalfShared ? kWarps * 32 * kVec : 1];
+  __shared__ T strips[PAIR == kHalfShared ? kWarps * 32 * kVec : 1];
   __shared__ float fold[kWarps][kMaxDim];
+  __shared__ __align__(16) float weights[kMaxDim];  // eight registers per lane fewer than held there
   pdl_launch_dependents();
   pdl_wait();
   const bool first = static_cast<int>(blockIdx.x) < p.blocks0;
   const Side& s = p.side[first ? 0 : 1];
-  const int block = first ? blockIdx.x : blockIdx.x - p.blocks0;
-  const int blocks = first ? p.blocks0 : gridDim.x - p.blocks0;
+  const unsigned block = first ? blockIdx.x : blockIdx.x - p.blocks0;
+  const unsigned blocks = first ? p.blocks0 : gridDim.x - p.blocks0;
   const int warp = threadIdx.x >> 5;
   const Where w = where(p);
-  float* strip = strips + (PAIR == kHalfShared ? warp * 32 * kVec : 0);
+  T* strip = strips + (PAIR == kHalfShared ? warp * 32 * kVec : 0);
   const int heads_per = 32 / p.group;
-  const int chunks = (s.heads + heads_per * PER - 1) / (heads_per * PER);
-  const long items = static_cast<long>(p.B) * p.T * chunks;
+  const unsigned chunks = first ? p.chunks0 : p.chunks1;
+  const unsigned items = static_cast<unsigned>(p.tokens) * chunks;  // below 2^31
 
-  float weight[kVec], acc[kVec];
+  for (int e = threadIdx.x; e < kMaxDim; e += blockDim.x) weights[e] = e < p.D ? s.weight[e] : 0.f;
+  __syncthreads();
+  const float4* my_weights = reinterpret_cast<const float4*>(weights + w.e0);
+  float acc[kVec];
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) {
-    weight[i] = w.e0 + i < p.D ? s.weight[w.e0 + i] : 0.f;
-    acc[i] = 0.f;
-  }
-  for (long item = static_cast<long>(block) * kWarps + warp; item < items;
-       item += static_cast<long>(blocks) * kWarps) {
-    const long token = item / chunks;
+  for (int i = 0; i < kVec; ++i) acc[i] = 0.f;
+  for (unsigned item = block * kWarps + warp; item < items; item += blocks * kWarps) {
+    const unsigned token = item / chunks;
     const int h0 = static_cast<int>(item - token * chunks) * heads_per * PER + w.sub;
-    const int b = static_cast<int>(token / p.T), t = static_cast<int>(token - static_cast<long>(b) * p.T);
-    const T* x = static_cast<const T*>(s.x) + b * s.x_b + t * s.x_t;
-    const T* dy = static_cast<const T*>(s.dy) + b * s.dy_b + t * s.dy_t;
-    T* dx = static_cast<T*>(s.y) + b * s.y_b + t * s.y_t;
+    const int b = token / static_cast<unsigned>(p.T), t = token - b * p.T;
+    const T* x = static_cast<const T*>(s.x) + b * s.x_b + t * s.x_t + h0 * s.x_h;
+    const T* dy = static_cast<const T*>(s.dy) + b * s.dy_b + t * s.dy_t + h0 * s.dy_h;
+    T* dx = static_cast<T*>(s.y) + b * s.y_b + t * s.y_t + h0 * s.y_h;
     Raw<T> rx[PER], rg[PER];
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const int h = h0 + j * heads_per;
-      const bool live = w.live && h < s.heads;
-      load_raw(rx[j], x + static_cast<long>(h) * s.x_h, w.e0, p.D, s.vec, live);
-      load_raw(rg[j], dy + static_cast<long>(h) * s.dy_h, w.e0, p.D, s.vec, live);
+      const bool live = w.live && h0 + j * heads_per < s.heads;
+      load_raw<VEC>(rx[j], x + j * heads_per * s.x_h, w.e0, p.D, live);
+      load_raw<VEC>(rg[j], dy + j * heads_per * s.dy_h, w.e0, p.D, live);
     }
     float C[kVec], S[kVec];
     load_angles<PAIR>(p, b, t, w.e0, C, S);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      const int h = h0 + j * heads_per;
-      float v[kVec], u[kVec];
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        v[i] = to_f32(rg[j].v[i]);
-        u[i] = to_f32(rx[j].v[i]);
-      }
-      turn<PAIR>(p, v, C, S, w.e0, w.lane, strip);
+      Raw<T> other;
+      partners<T, PAIR>(p, rg[j], other, w.e0, w.lane, strip);
+      float v[kVec];
+      combine<T, PAIR>(p, rg[j], other, C, S, w.e0, v);
+      const float4 w0 = my_weights[0], w1 = my_weights[1];
+      const float weight[kVec] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
       float sq = 0.f, dot = 0.f;
 #pragma unroll
       for (int i = 0; i < kVec; ++i) {
-        sq = fmaf(u[i], u[i], sq);
-        dot = fmaf(v[i] * weight[i], u[i], dot);
+        const float u = to_f32(rx[j].v[i]);
+        sq = fmaf(u, u, sq);
+        dot = fmaf(v[i] * weight[i], u, dot);
       }
       sq = group_sum(sq, p.group);
       dot = group_sum(dot, p.group);
-      const float rstd = 1.0f / sqrtf(sq / p.D + p.eps);
-      const float mean = dot * rstd / p.D;
-      if (w.live && h < s.heads) {
+      const float rstd = rsqrtf(fmaf(sq, p.inv_dim, p.eps));
+      const float pull = dot * p.inv_dim * rstd * rstd;  // mean(v w xhat) / rms
+      if (w.live && h0 + j * heads_per < s.heads) {
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
-          const float unit = u[i] * rstd;
-          acc[i] = fmaf(v[i], unit, acc[i]);
-          v[i] = rstd * (v[i] * weight[i] - unit * mean);
+          const float u = to_f32(rx[j].v[i]);
+          acc[i] = fmaf(v[i], u * rstd, acc[i]);
+          v[i] = rstd * fmaf(-u, pull, v[i] * weight[i]);
         }
-        store_raw(dx + static_cast<long>(h) * s.y_h, v, w.e0, p.D, s.vec);
+        store_raw<VEC>(dx + j * heads_per * s.y_h, v, w.e0, p.D);
       }
     }
   }
@@ -385,8 +416,10 @@ rotary_dw_kernel(const float* __restrict__ partial, int blocks0, int blocks1, in
   const int rows = second ? blocks1 : blocks0;
   const float* src = partial + (second ? static_cast<long>(blocks0) * D : 0);
   float sum = 0.f;
-  if (e < D)
+  if (e < D) {
+#pragma unroll 8
     for (int r = warp; r < rows; r += 32) sum += src[static_cast<long>(r) * D + e];
+  }
   sums[warp][lane] = sum;
   __syncthreads();
   if (warp == 0 && e < D) {
@@ -412,7 +445,8 @@ int sm_count_here() {
 }
 
 int fill(RotaryParams& p, const SflRotaryTensor* tensors, int count, const SflRotaryTable* table,
-         int B, int T, int D, float eps, int inverse, int dtype, bool backward) {
+         int B, int T, int D, float eps, int inverse, int dtype, bool backward, bool* vec) {
+  *vec = true;
   if (tensors == nullptr || table == nullptr || count < 1 || count > 2 || B < 0 || T < 0 || D < 1 ||
       D > kMaxDim || dtype < 0 || dtype > 2)
     return -2;
@@ -426,10 +460,11 @@ int fill(RotaryParams& p, const SflRotaryTensor* tensors, int count, const SflRo
     if (backward && (q.dy == nullptr || !norm)) return -2;
     Side& s = p.side[i];
     s = Side{q.x, q.y, q.dy, q.weight, q.x_b, q.x_h, q.x_t, q.y_b, q.y_h, q.y_t, q.dy_b, q.dy_h,
-             q.dy_t, q.heads, 0};
-    s.vec = D % kVec == 0 && aligned(q.x, q.x_b, q.x_h, q.x_t, size) &&
-            aligned(q.y, q.y_b, q.y_h, q.y_t, size) &&
-            (!backward || aligned(q.dy, q.dy_b, q.dy_h, q.dy_t, size));
+             q.dy_t, q.heads};
+    // 16-byte accesses need every head row of x, y (and dy) to start on a 16-byte boundary
+    *vec = *vec && D % kVec == 0 && aligned(q.x, q.x_b, q.x_h, q.x_t, size) &&
+           aligned(q.y, q.y_b, q.y_h, q.y_t, size) &&
+           (!backward || aligned(q.dy, q.dy_b, q.dy_h, q.dy_t, size));
   }
   if (count == 1) p.side[1] = p.side[0];
   p.cos = table->cos;
@@ -441,9 +476,12 @@ int fill(RotaryParams& p, const SflRotaryTensor* tensors, int count, const SflRo
   p.rotated = table->rotated;
   p.table_vec = (table->rotated / 2) % 4 == 0 && (reinterpret_cast<uintptr_t>(table->cos) & 15) == 0 &&
                 (reinterpret_cast<uintptr_t>(table->sin) & 15) == 0;
+  if (static_cast<long>(B) * T > 0x7fffffffL) return -2;
   p.B = B;
   p.T = T;
   p.D = D;
+  p.tokens = B * T;
+  p.inv_dim = 1.0f / static_cast<float>(D);
   p.group = 1;
   while (p.group * kVec < D) p.group *= 2;
   p.eps = eps;
@@ -452,69 +490,78 @@ int fill(RotaryParams& p, const SflRotaryTensor* tensors, int count, const SflRo
   return 0;
 }
 
-long blocks_for(const RotaryParams& p, const Side& s, int per) {
+void set_chunks(RotaryParams& p, int count, int per) {
   const int each = 32 / p.group * per;
-  const long items = static_cast<long>(p.B) * p.T * ((s.heads + each - 1) / each);
-  return (items + kWarps - 1) / kWarps;
+  p.chunks0 = (p.side[0].heads + each - 1) / each;
+  p.chunks1 = count == 2 ? (p.side[1].heads + each - 1) / each : 0;
 }
 
-int pairing(int half_layout, int rotated) {
+// Unaligned rows are read element by element; of the half layout's forms only the one through
+// shared memory exists for them.
+int pairing(int half_layout, int rotated, bool vec) {
   if (!half_layout) return kInterleaved;
-  return (rotated / 2) % kVec == 0 ? kHalfShuffle : kHalfShared;
+  return vec && (rotated / 2) % kVec == 0 ? kHalfShuffle : kHalfShared;
 }
 
-template <typename T, int PAIR, bool NORM>
+template <typename T, int PAIR, bool VEC, bool NORM>
 int launch_forward(RotaryParams p, int count, int sms, cudaStream_t stream) {
-  auto go = [&](auto kernel, int per) -> int {
-    const long b0 = blocks_for(p, p.side[0], per);
-    const long b1 = count == 2 ? blocks_for(p, p.side[1], per) : 0;
-    if (b0 + b1 > 0x7fffffffL) return -2;
-    p.blocks0 = static_cast<int>(b0);
-    return launch_pdl(kernel, dim3(static_cast<unsigned>(b0 + b1)), dim3(32 * kWarps), 0, stream, p);
+  const long token_blocks = (p.tokens + kWarps - 1L) / kWarps;
+  auto go = [&](auto kernel) -> int {
+    const long blocks = token_blocks * (p.chunks0 + p.chunks1);
+    if (blocks > 0x7fffffffL) return -2;
+    return launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(32 * kWarps), 0, stream, p);
   };
-  long few = blocks_for(p, p.side[0], 4) + (count == 2 ? blocks_for(p, p.side[1], 4) : 0);
-  if (few >= 2L * sms) return go(rotary_kernel<T, PAIR, NORM, 4>, 4);
-  return go(rotary_kernel<T, PAIR, NORM, 1>, 1);
+  set_chunks(p, count, 4);
+  if (token_blocks * (p.chunks0 + p.chunks1) >= 2L * sms)
+    return go(rotary_kernel<T, PAIR, VEC, NORM, 4>);
+  set_chunks(p, count, 1);
+  return go(rotary_kernel<T, PAIR, VEC, NORM, 1>);
 }
 
-template <typename T>
-int forward_of(const RotaryParams& p, int count, int pair, bool norm, int sms, cudaStream_t stream) {
-  switch (pair * 2 + (norm ? 1 : 0)) {
-    case 0: return launch_forward<T, kInterleaved, false>(p, count, sms, stream);
-    case 1: return launch_forward<T, kInterleaved, true>(p, count, sms, stream);
-    case 2: return launch_forward<T, kHalfShuffle, false>(p, count, sms, stream);
-    case 3: return launch_forward<T, kHalfShuffle, true>(p, count, sms, stream);
-    case 4: return launch_forward<T, kHalfShared, false>(p, count, sms, stream);
-    default: return launch_forward<T, kHalfShared, true>(p, count, sms, stream);
+template <typename T, bool NORM>
+int forward_of(const RotaryParams& p, int count, int pair, bool vec, int sms, cudaStream_t stream) {
+  if (vec) {
+    if (pair == kInterleaved) return launch_forward<T, kInterleaved, true, NORM>(p, count, sms, stream);
+    if (pair == kHalfShuffle) return launch_forward<T, kHalfShuffle, true, NORM>(p, count, sms, stream);
+    return launch_forward<T, kHalfShared, true, NORM>(p, count, sms, stream);
   }
+  if (pair == kInterleaved) return launch_forward<T, kInterleaved, false, NORM>(p, count, sms, stream);
+  return launch_forward<T, kHalfShared, false, NORM>(p, count, sms, stream);
 }
 
 // Warps of the persistent backward grid share the tokens; each side gets blocks in proportion
-// to its heads, and no more than it has work for.
+// to its heads, and no more than it has work for.  Returns false beyond 32-bit item counts.
 constexpr int kBwdPer = 2;
-constexpr int kBwdBlocksPerSm = 3;
 
-void backward_blocks(const RotaryParams& p, int count, int sms, int* b0, int* b1) {
+bool backward_blocks(RotaryParams& p, int count, int sms, int* b0, int* b1) {
+  set_chunks(p, count, kBwdPer);
   const long total = static_cast<long>(sms) * kBwdBlocksPerSm;
   const long heads = p.side[0].heads + (count == 2 ? p.side[1].heads : 0);
-  auto share = [&](const Side& s) {
+  auto share = [&](const Side& s, int chunks) {
     long want = total * s.heads / heads;
-    const long most = blocks_for(p, s, kBwdPer);
+    const long most = (static_cast<long>(p.tokens) * chunks + kWarps - 1) / kWarps;
     if (want > most) want = most;
     return static_cast<int>(want < 1 ? 1 : want);
   };
-  *b0 = share(p.side[0]);
-  *b1 = count == 2 ? share(p.side[1]) : 0;
+  *b0 = share(p.side[0], p.chunks0);
+  *b1 = count == 2 ? share(p.side[1], p.chunks1) : 0;
+  // the grid's stride past the last item must not wrap either
+  const long most = p.chunks0 > p.chunks1 ? p.chunks0 : p.chunks1;
+  return p.tokens * most + total * kWarps <= 0x7fffffffL;
 }
 
 template <typename T>
-int backward_of(const RotaryParams& p, int pair, int grid, cudaStream_t stream) {
+int backward_of(const RotaryParams& p, int pair, bool vec, int grid, cudaStream_t stream) {
   auto go = [&](auto kernel) {
     return launch_pdl(kernel, dim3(grid), dim3(32 * kWarps), 0, stream, p);
   };
-  if (pair == kInterleaved) return go(rotary_bwd_kernel<T, kInterleaved, kBwdPer>);
-  if (pair == kHalfShuffle) return go(rotary_bwd_kernel<T, kHalfShuffle, kBwdPer>);
-  return go(rotary_bwd_kernel<T, kHalfShared, kBwdPer>);
+  if (vec) {
+    if (pair == kInterleaved) return go(rotary_bwd_kernel<T, kInterleaved, true, kBwdPer>);
+    if (pair == kHalfShuffle) return go(rotary_bwd_kernel<T, kHalfShuffle, true, kBwdPer>);
+    return go(rotary_bwd_kernel<T, kHalfShared, true, kBwdPer>);
+  }
+  if (pair == kInterleaved) return go(rotary_bwd_kernel<T, kInterleaved, false, kBwdPer>);
+  return go(rotary_bwd_kernel<T, kHalfShared, false, kBwdPer>);
 }
 
 }  // namespace
@@ -525,17 +572,22 @@ extern "C" int sfl_rotary(const SflRotaryTensor* tensors, int count, const SflRo
                           void* stream) {
   using namespace sfl;
   RotaryParams p{};
-  const int bad = fill(p, tensors, count, table, B, T, D, eps, inverse, dtype, false);
+  bool vec;
+  const int bad = fill(p, tensors, count, table, B, T, D, eps, inverse, dtype, false, &vec);
   if (bad != 0) return bad;
   if (B == 0 || T == 0) return 0;
   const int sms = sm_count_here();
   if (sms == 0) return -1;
-  const int pair = pairing(half_layout, p.rotated);
-  const bool norm = tensors[0].weight != nullptr;
+  const int pair = pairing(half_layout, p.rotated, vec);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == 0) return forward_of<__nv_bfloat16>(p, count, pair, norm, sms, st);
-  if (dtype == 1) return forward_of<__half>(p, count, pair, norm, sms, st);
-  return forward_of<float>(p, count, pair, norm, sms, st);
+  auto of = [&](auto zero) -> int {
+    using T = decltype(zero);
+    return tensors[0].weight != nullptr ? forward_of<T, true>(p, count, pair, vec, sms, st)
+                                        : forward_of<T, false>(p, count, pair, vec, sms, st);
+  };
+  if (dtype == 0) return of(__nv_bfloat16{});
+  if (dtype == 1) return of(__half{});
+  return of(0.f);
 }
 
 extern "C" long sfl_rotary_bwd_partial_bytes(int heads0, int heads1, int B, int T, int D) {
@@ -553,23 +605,24 @@ extern "C" int sfl_rotary_bwd(const SflRotaryTensor* tensors, int count,
                               float* dw0, float* dw1, void* stream) {
   using namespace sfl;
   RotaryParams p{};
-  const int bad = fill(p, tensors, count, table, B, T, D, eps, 1, dtype, true);
+  bool vec;
+  const int bad = fill(p, tensors, count, table, B, T, D, eps, 1, dtype, true, &vec);
   if (bad != 0) return bad;
   if (partial == nullptr || dw0 == nullptr || (count == 2 && dw1 == nullptr)) return -2;
   if (B == 0 || T == 0) return -2;
   const int sms = sm_count_here();
   if (sms == 0) return -1;
   int b0, b1;
-  backward_blocks(p, count, sms, &b0, &b1);
+  if (!backward_blocks(p, count, sms, &b0, &b1)) return -2;
   if (static_cast<long>(b0 + b1) * D * static_cast<long>(sizeof(float)) > partial_bytes) return -2;
   p.blocks0 = b0;
   p.partial = partial;
-  const int pair = pairing(half_layout, p.rotated);
+  const int pair = pairing(half_layout, p.rotated, vec);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int code;
-  if (dtype == 0) code = backward_of<__nv_bfloat16>(p, pair, b0 + b1, st);
-  else if (dtype == 1) code = backward_of<__half>(p, pair, b0 + b1, st);
-  else code = backward_of<float>(p, pair, b0 + b1, st);
+  if (dtype == 0) code = backward_of<__nv_bfloat16>(p, pair, vec, b0 + b1, st);
+  else if (dtype == 1) code = backward_of<__half>(p, pair, vec, b0 + b1, st);
+  else code = backward_of<float>(p, pair, vec, b0 + b1, st);
   if (code != 0) return code;
   return launch_pdl(rotary_dw_kernel, dim3((D + 31) / 32, count), dim3(1024), 0, st,
                     static_cast<const float*>(partial), b0, b1, D, dw0, dw1);

@@ -168,7 +168,8 @@ def _check_out(out: torch.Tensor, x: torch.Tensor, name: str) -> None:
 def _new(x: torch.Tensor) -> torch.Tensor:
     """A result laid out token-major ([B, T, H, D] in memory), as a projection leaves heads."""
     B, H, T, D = x.shape
-    return torch.empty(B, T, H, D, dtype=x.dtype, device=x.device).permute(0, 2, 1, 3)
+    return torch.empty_strided((B, H, T, D), (T * H * D, D, H * D, 1), dtype=x.dtype,
+                               device=x.device)
 
 
 def _slot(slot: RotaryTensor, x, y, dy, weight) -> None:
