@@ -34,7 +34,7 @@ namespace sfl {
 namespace {
 
 constexpr int kVec = 8;        // elements of a head that one lane holds
-constexpr int kWarps = 8;      // warps per block
+constexpr int kWarps = 4;      // warps per block
 constexpr int kMaxDim = 256;   // 32 lanes of eight elements
 
 // How a lane finds the other element of a pair.
@@ -66,6 +66,7 @@ struct RotaryParams {
   float eps, sign;    // sign -1 turns by the opposite angle
   float inv_dim;
   int chunks0, chunks1;  // warp items per token on each side
+  int rounds0, rounds1;  // rounds of PER head groups that one warp item walks
   int tokens;
   float* partial;     // backward with norm: [blocks, D]
 };
@@ -80,6 +81,16 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) {
   return __float2bfloat16_rn(v);
 }
 template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
+
+// Two values in one conversion instruction.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  return pack_bf16(lo, hi);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
 
 // The eight elements as they lie in memory; converted to fp32 only when they are used, so that
 // loads in flight hold 16 bytes (32 for fp32) of registers per lane.
@@ -102,18 +113,17 @@ __device__ __forceinline__ void load_raw(Raw<T>& r, const T* row, int e0, int D,
 
 template <bool VEC, typename T>
 __device__ __forceinline__ void store_raw(T* row, const float (&f)[kVec], int e0, int D) {
-  Raw<T> r;
-#pragma unroll
-  for (int i = 0; i < kVec; ++i) r.v[i] = from_f32<T>(f[i]);
-  if constexpr (VEC) {
-    uint4* dst = reinterpret_cast<uint4*>(row + e0);
-    const uint4* src = reinterpret_cast<const uint4*>(r.v);
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(Raw<T>) / 16); ++i) dst[i] = src[i];
+  if constexpr (VEC && sizeof(T) == 4) {
+    float4* dst = reinterpret_cast<float4*>(row + e0);
+    dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+    dst[1] = make_float4(f[4], f[5], f[6], f[7]);
+  } else if constexpr (VEC) {
+    *reinterpret_cast<uint4*>(row + e0) = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]),
+                                                     pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
   } else {
 #pragma unroll
     for (int i = 0; i < kVec; ++i)
-      if (e0 + i < D) row[e0 + i] = r.v[i];
+      if (e0 + i < D) row[e0 + i] = from_f32<T>(f[i]);
   }
 }
 
@@ -218,17 +228,31 @@ __device__ __forceinline__ void combine(const RotaryParams& p, const Raw<T>& min
   }
 }
 
-// The element whose weight multiplies the partner of element e.
-template <int PAIR>
+// Eight weights from element e, zero beyond the head.
+template <bool VEC>
+__device__ __forceinline__ void load_weights(const float* weight, int e, int D, float (&w)[kVec]) {
+  if constexpr (VEC) {
+    const float4* src = reinterpret_cast<const float4*>(weight + (e < D ? e : 0));
+    const float4 a = src[0], b = src[1];
+    w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
+    w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) w[i] = e + i < D ? weight[e + i] : 0.f;
+  }
+}
+
+// Half layout: the element whose weight multiplies the partner of element e.
 __device__ __forceinline__ int partner_of(const RotaryParams& p, int e) {
   if (e >= p.rotated) return e;
-  if constexpr (PAIR == kInterleaved) return e ^ 1;
   const int half = p.rotated >> 1;
   return e < half ? e + half : e - half;
 }
 
 __device__ __forceinline__ float group_sum(float v, int group) {
-  for (int o = group >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < group) v += __shfl_xor_sync(0xffffffffu, v, o);  // group is uniform
   return v;
 }
 
@@ -251,7 +275,7 @@ __device__ __forceinline__ Where where(const RotaryParams& p) {
 // PER = 1 is for calls with few tokens, which are over sooner when every head group has a warp
 // of its own (16 tokens x 40 heads x 128: 3.0 us against 3.9 us).
 template <typename T, int PAIR, bool VEC, bool NORM, int PER>
-__global__ void __launch_bounds__(32 * kWarps, PER == 4 && VEC && sizeof(T) == 2 ? 4 : 2)
+__global__ void __launch_bounds__(32 * kWarps, PER == 4 && VEC && sizeof(T) == 2 ? 8 : 4)
 rotary_kernel(const __grid_constant__ RotaryParams p) {
   __shared__ T strips[PAIR == kHalfShared ? kWarps * 32 * kVec : 1];
   pdl_launch_dependents();
@@ -269,54 +293,76 @@ rotary_kernel(const __grid_constant__ RotaryParams p) {
   const unsigned token = block_token * kWarps + warp;
   if (token >= static_cast<unsigned>(p.tokens)) return;  // warp-uniform
   const int b = token / static_cast<unsigned>(p.T), t = token - b * p.T;
-  const int h0 = chunk * heads_per * PER + w.sub;
+  const int rounds = first ? p.rounds0 : p.rounds1;
+  int h0 = chunk * rounds * heads_per * PER + w.sub;
   const T* x = static_cast<const T*>(s.x) + b * s.x_b + t * s.x_t + h0 * s.x_h;
   T* y = static_cast<T*>(s.y) + b * s.y_b + t * s.y_t + h0 * s.y_h;
-
   Raw<T> raw[PER];
+  const long x_step = heads_per * s.x_h, y_step = heads_per * s.y_h;
+  auto load = [&] {
 #pragma unroll
-  for (int j = 0; j < PER; ++j)
-    load_raw<VEC>(raw[j], x + j * heads_per * s.x_h, w.e0, p.D,
-                  w.live && h0 + j * heads_per < s.heads);
+    for (int j = 0; j < PER; ++j)
+      load_raw<VEC>(raw[j], x + j * x_step, w.e0, p.D,
+                    w.live && h0 + j * heads_per < s.heads);
+  };
+  load();
   float C[kVec], S[kVec];
   load_angles<PAIR>(p, b, t, w.e0, C, S);
   if constexpr (NORM) {
+    float own[kVec];
+    load_weights<VEC>(s.weight, w.e0, p.D, own);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      const int e = w.e0 + i;
-      C[i] *= e < p.D ? s.weight[e] : 0.f;
-      S[i] *= e < p.D ? s.weight[partner_of<PAIR>(p, e)] : 0.f;
+    for (int i = 0; i < kVec; ++i) C[i] *= own[i];
+    if constexpr (PAIR == kInterleaved) {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) S[i] *= own[i ^ 1];
+    } else if constexpr (PAIR == kHalfShuffle) {
+      load_weights<VEC>(s.weight, partner_of(p, w.e0), p.D, own);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) S[i] *= own[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i)
+        S[i] *= w.e0 + i < p.D ? s.weight[partner_of(p, w.e0 + i)] : 0.f;
     }
   }
+  for (int round = 0;;) {
 #pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    float rstd = 1.f;
-    if constexpr (NORM) {
-      float sq = 0.f;
+    for (int j = 0; j < PER; ++j) {
+      float rstd = 1.f;
+      if constexpr (NORM) {
+        float sq = 0.f;
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) sq = fmaf(to_f32(raw[j].v[i]), to_f32(raw[j].v[i]), sq);
-      rstd = rsqrtf(fmaf(group_sum(sq, p.group), p.inv_dim, p.eps));
+        for (int i = 0; i < kVec; ++i) sq = fmaf(to_f32(raw[j].v[i]), to_f32(raw[j].v[i]), sq);
+        rstd = rsqrtf(fmaf(group_sum(sq, p.group), p.inv_dim, p.eps));
+      }
+      Raw<T> other;
+      partners<T, PAIR>(p, raw[j], other, w.e0, w.lane, strip);
+      float f[kVec];
+      combine<T, PAIR>(p, raw[j], other, C, S, w.e0, f);
+      if constexpr (NORM) {
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) f[i] *= rstd;
+      }
+      if (w.live && h0 + j * heads_per < s.heads)
+        store_raw<VEC>(y + j * y_step, f, w.e0, p.D);
     }
-    Raw<T> other;
-    partners<T, PAIR>(p, raw[j], other, w.e0, w.lane, strip);
-    float f[kVec];
-    combine<T, PAIR>(p, raw[j], other, C, S, w.e0, f);
-    if constexpr (NORM) {
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) f[i] *= rstd;
-    }
-    if (w.live && h0 + j * heads_per < s.heads)
-      store_raw<VEC>(y + j * heads_per * s.y_h, f, w.e0, p.D);
+    if (++round == rounds) break;
+    h0 += heads_per * PER;
+    if (h0 - w.sub >= s.heads) break;  // warp-uniform
+    x += PER * x_step;
+    y += PER * y_step;
+    load();
   }
 }
 
 // Backward with the norm.  A persistent grid: every warp keeps the weight gradient of its
 // eight elements in registers over all its tokens; the block folds its warps in a fixed order
 // and leaves one row of partial sums (deterministic, no atomics).
-constexpr int kBwdBlocksPerSm = 3;
+constexpr int kBwdBlocksPerSm = 5;
 
 template <typename T, int PAIR, bool VEC, int PER>
-__global__ void __launch_bounds__(32 * kWarps, VEC && sizeof(T) == 2 ? kBwdBlocksPerSm : 2)
+__global__ void __launch_bounds__(32 * kWarps, VEC && sizeof(T) == 2 ? kBwdBlocksPerSm : 4)
 rotary_bwd_kernel(const __grid_constant__ RotaryParams p) {
   __shared__ T strips[PAIR == kHalfShared ? kWarps * 32 * kVec : 1];
   __shared__ float fold[kWarps][kMaxDim];
@@ -332,6 +378,7 @@ rotary_bwd_kernel(const __grid_constant__ RotaryParams p) {
   T* strip = strips + (PAIR == kHalfShared ? warp * 32 * kVec : 0);
   const int heads_per = 32 / p.group;
   const unsigned chunks = first ? p.chunks0 : p.chunks1;
+  const int rounds = first ? p.rounds0 : p.rounds1;
   const unsigned items = static_cast<unsigned>(p.tokens) * chunks;  // below 2^31
 
   for (int e = threadIdx.x; e < kMaxDim; e += blockDim.x) weights[e] = e < p.D ? s.weight[e] : 0.f;
@@ -342,48 +389,60 @@ rotary_bwd_kernel(const __grid_constant__ RotaryParams p) {
   for (int i = 0; i < kVec; ++i) acc[i] = 0.f;
   for (unsigned item = block * kWarps + warp; item < items; item += blocks * kWarps) {
     const unsigned token = item / chunks;
-    const int h0 = static_cast<int>(item - token * chunks) * heads_per * PER + w.sub;
+    int h0 = static_cast<int>(item - token * chunks) * rounds * heads_per * PER + w.sub;
     const int b = token / static_cast<unsigned>(p.T), t = token - b * p.T;
     const T* x = static_cast<const T*>(s.x) + b * s.x_b + t * s.x_t + h0 * s.x_h;
     const T* dy = static_cast<const T*>(s.dy) + b * s.dy_b + t * s.dy_t + h0 * s.dy_h;
     T* dx = static_cast<T*>(s.y) + b * s.y_b + t * s.y_t + h0 * s.y_h;
     Raw<T> rx[PER], rg[PER];
+    auto load = [&] {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const bool live = w.live && h0 + j * heads_per < s.heads;
-      load_raw<VEC>(rx[j], x + j * heads_per * s.x_h, w.e0, p.D, live);
-      load_raw<VEC>(rg[j], dy + j * heads_per * s.dy_h, w.e0, p.D, live);
-    }
+      for (int j = 0; j < PER; ++j) {
+        const bool live = w.live && h0 + j * heads_per < s.heads;
+        load_raw<VEC>(rx[j], x + j * heads_per * s.x_h, w.e0, p.D, live);
+        load_raw<VEC>(rg[j], dy + j * heads_per * s.dy_h, w.e0, p.D, live);
+      }
+    };
+    load();
     float C[kVec], S[kVec];
     load_angles<PAIR>(p, b, t, w.e0, C, S);
+    for (int round = 0;;) {
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      Raw<T> other;
-      partners<T, PAIR>(p, rg[j], other, w.e0, w.lane, strip);
-      float v[kVec];
-      combine<T, PAIR>(p, rg[j], other, C, S, w.e0, v);
-      const float4 w0 = my_weights[0], w1 = my_weights[1];
-      const float weight[kVec] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-      float sq = 0.f, dot = 0.f;
-#pragma unroll
-      for (int i = 0; i < kVec; ++i) {
-        const float u = to_f32(rx[j].v[i]);
-        sq = fmaf(u, u, sq);
-        dot = fmaf(v[i] * weight[i], u, dot);
-      }
-      sq = group_sum(sq, p.group);
-      dot = group_sum(dot, p.group);
-      const float rstd = rsqrtf(fmaf(sq, p.inv_dim, p.eps));
-      const float pull = dot * p.inv_dim * rstd * rstd;  // mean(v w xhat) / rms
-      if (w.live && h0 + j * heads_per < s.heads) {
+      for (int j = 0; j < PER; ++j) {
+        Raw<T> other;
+        partners<T, PAIR>(p, rg[j], other, w.e0, w.lane, strip);
+        float v[kVec];
+        combine<T, PAIR>(p, rg[j], other, C, S, w.e0, v);
+        const float4 w0 = my_weights[0], w1 = my_weights[1];
+        const float weight[kVec] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+        float sq = 0.f, dot = 0.f;
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
           const float u = to_f32(rx[j].v[i]);
-          acc[i] = fmaf(v[i], u * rstd, acc[i]);
-          v[i] = rstd * fmaf(-u, pull, v[i] * weight[i]);
+          sq = fmaf(u, u, sq);
+          dot = fmaf(v[i] * weight[i], u, dot);
         }
-        store_raw<VEC>(dx + j * heads_per * s.y_h, v, w.e0, p.D);
+        sq = group_sum(sq, p.group);
+        dot = group_sum(dot, p.group);
+        const float rstd = rsqrtf(fmaf(sq, p.inv_dim, p.eps));
+        const float pull = dot * p.inv_dim * rstd * rstd;  // mean(v w xhat) / rms
+        if (w.live && h0 + j * heads_per < s.heads) {
+#pragma unroll
+          for (int i = 0; i < kVec; ++i) {
+            const float u = to_f32(rx[j].v[i]);
+            acc[i] = fmaf(v[i], u * rstd, acc[i]);
+            v[i] = rstd * fmaf(-u, pull, v[i] * weight[i]);
+          }
+          store_raw<VEC>(dx + j * heads_per * s.y_h, v, w.e0, p.D);
+        }
       }
+      if (++round == rounds) break;
+      h0 += heads_per * PER;
+      if (h0 - w.sub >= s.heads) break;  // warp-uniform
+      x += heads_per * PER * s.x_h;
+      dy += heads_per * PER * s.dy_h;
+      dx += heads_per * PER * s.y_h;
+      load();
     }
   }
   // heads of the warp, then warps of the block
@@ -464,7 +523,8 @@ int fill(RotaryParams& p, const SflRotaryTensor* tensors, int count, const SflRo
     // 16-byte accesses need every head row of x, y (and dy) to start on a 16-byte boundary
     *vec = *vec && D % kVec == 0 && aligned(q.x, q.x_b, q.x_h, q.x_t, size) &&
            aligned(q.y, q.y_b, q.y_h, q.y_t, size) &&
-           (!backward || aligned(q.dy, q.dy_b, q.dy_h, q.dy_t, size));
+           (!backward || aligned(q.dy, q.dy_b, q.dy_h, q.dy_t, size)) &&
+           (reinterpret_cast<uintptr_t>(q.weight) & 15) == 0;
   }
   if (count == 1) p.side[1] = p.side[0];
   p.cos = table->cos;
@@ -490,10 +550,19 @@ int fill(RotaryParams& p, const SflRotaryTensor* tensors, int count, const SflRo
   return 0;
 }
 
-void set_chunks(RotaryParams& p, int count, int per) {
+// Warp items per token.  A warp that walks all heads of its token reads the angles and weights
+// once for them (a third of the instructions of a one-round item at 8 heads of 128); with fewer
+// tokens than keep the SMs busy that way, the heads are spread over more warps.
+void set_chunks(RotaryParams& p, int count, int per, long warps_wanted) {
   const int each = 32 / p.group * per;
-  p.chunks0 = (p.side[0].heads + each - 1) / each;
-  p.chunks1 = count == 2 ? (p.side[1].heads + each - 1) / each : 0;
+  const int all0 = (p.side[0].heads + each - 1) / each;
+  const int all1 = count == 2 ? (p.side[1].heads + each - 1) / each : 0;
+  int rounds = all0 > all1 ? all0 : all1;
+  auto items = [&](int r) { return static_cast<long>(p.tokens) * ((all0 + r - 1) / r + (all1 + r - 1) / r); };
+  while (rounds > 1 && items(rounds) < warps_wanted) rounds = (rounds + 1) / 2;
+  p.rounds0 = p.rounds1 = rounds;
+  p.chunks0 = (all0 + rounds - 1) / rounds;
+  p.chunks1 = (all1 + rounds - 1) / rounds;
 }
 
 // Unaligned rows are read element by element; of the half layout's forms only the one through
@@ -511,10 +580,10 @@ int launch_forward(RotaryParams p, int count, int sms, cudaStream_t stream) {
     if (blocks > 0x7fffffffL) return -2;
     return launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(32 * kWarps), 0, stream, p);
   };
-  set_chunks(p, count, 4);
+  set_chunks(p, count, 4, 64L * sms);  // two rounds of 32 resident warps per SM
   if (token_blocks * (p.chunks0 + p.chunks1) >= 2L * sms)
     return go(rotary_kernel<T, PAIR, VEC, NORM, 4>);
-  set_chunks(p, count, 1);
+  set_chunks(p, count, 1, 64L * sms);
   return go(rotary_kernel<T, PAIR, VEC, NORM, 1>);
 }
 
@@ -534,7 +603,7 @@ int forward_of(const RotaryParams& p, int count, int pair, bool vec, int sms, cu
 constexpr int kBwdPer = 2;
 
 bool backward_blocks(RotaryParams& p, int count, int sms, int* b0, int* b1) {
-  set_chunks(p, count, kBwdPer);
+  set_chunks(p, count, kBwdPer, 4L * kBwdBlocksPerSm * kWarps * sms);
   const long total = static_cast<long>(sms) * kBwdBlocksPerSm;
   const long heads = p.side[0].heads + (count == 2 ? p.side[1].heads : 0);
   auto share = [&](const Side& s, int chunks) {
