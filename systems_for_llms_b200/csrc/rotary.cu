@@ -278,7 +278,9 @@ template <typename T, int PAIR, bool VEC, bool NORM, int PER>
 __global__ void __launch_bounds__(32 * kWarps, PER == 4 && VEC && sizeof(T) == 2 ? 8 : 4)
 rotary_kernel(const __grid_constant__ RotaryParams p) {
   __shared__ T strips[PAIR == kHalfShared ? kWarps * 32 * kVec : 1];
-  pdl_launch_dependents();
+  // Only the short form lets its successor in early: waiting CTAs would take the slots of this
+  // kernel's later ones (measured on the long form: 1150 us against 845 us, run by itself).
+  if constexpr (PER == 1) pdl_launch_dependents();
   pdl_wait();
   const unsigned chunks = p.chunks0 + p.chunks1;
   const unsigned block_token = blockIdx.x / chunks;
@@ -367,7 +369,6 @@ rotary_bwd_kernel(const __grid_constant__ RotaryParams p) {
   __shared__ T strips[PAIR == kHalfShared ? kWarps * 32 * kVec : 1];
   __shared__ float fold[kWarps][kMaxDim];
   __shared__ __align__(16) float weights[kMaxDim];  // eight registers per lane fewer than held there
-  pdl_launch_dependents();
   pdl_wait();
   const bool first = static_cast<int>(blockIdx.x) < p.blocks0;
   const Side& s = p.side[first ? 0 : 1];
