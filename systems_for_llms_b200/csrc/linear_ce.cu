@@ -1,0 +1,561 @@
+// Softmax cross entropy of a vocabulary projection that keeps no logits.
+//
+//   loss_i = log(sum_v exp(h_i . w_v)) - h_i . w_t(i)
+//   dl_iv  = softmax_iv - [v = t(i)]          (zero rows where the target is ignored)
+//   dh     = g dl W,   dW = g dl^T h          g = incoming gradient (over the count, for a mean)
+//
+// The reference materialises the logits, their fp32 copy and its softmax
+// (src/llmlab/training/loss.py:4-22), and this library's other head keeps them in bf16
+// (elementwise.cu).  Here the projection's accumulators go from tensor memory straight into the
+// running maximum and sum of exponentials of their row: forward writes one (max, sum) pair per
+// row and 128 columns.  Backward walks the vocabulary in pieces: the piece's logits are computed
+// again, leave the epilogue as 16-bit dl, and two products consume them (dW of the piece, whose
+// rows are then final, and the piece's share of dh).  A piece is sized to stay in the L2 cache as
+// far as the matrices allow, so what the operator moves beyond its inputs and outputs does not
+// grow with the vocabulary.  The price is the second projection: 8 N D V operations for forward
+// and backward where keeping the logits takes 6.
+//
+// Logits are never rounded: statistics and losses see fp32 accumulators.  dl is rounded once to
+// the operands' type, which is what the tensor cores multiply; fp16 holds dl times 2^12, so
+// probabilities down to 2^-26 keep full precision and 1 becomes 4096, far below the largest fp16.
+// All sums have a fixed order; there are no atomics.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "pair_gemm.cuh"
+#include "sfl.h"
+
+namespace sfl {
+namespace {
+
+using pair::EpiContext;
+using pair::Tile;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kFp16Shift = 12;
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Tiles of an mt x nt grid with m fastest inside bands of `band` row tiles: a band's rows stay in
+// the L2 cache while the vocabulary streams past them once.
+struct Grid {
+  int mt, nt, band;
+};
+__device__ __forceinline__ void grid_tile(const Grid& g, int w, int* m, int* n) {
+  const int per_band = g.band * g.nt;
+  const int b = w / per_band;
+  const int in = w - b * per_band;
+  const int left = g.mt - b * g.band;
+  const int width = left < g.band ? left : g.band;
+  *n = in / width;
+  *m = b * g.band + (in - *n * width);
+}
+
+// ---------------------------------------------------- row statistics (forward) ----
+struct StatsOp {
+  struct Params {
+    CUtensorMap a, b;
+    Grid grid;
+    int total, num_kb;
+    uint32_t idesc;
+    int* status;
+    const int64_t* targets;
+    float2* part;      // [2 * nt][rows]
+    float* picked;     // [rows]: the target's logit
+    int rows, vocab;
+  };
+  static constexpr bool kAMN = false, kBMN = false;
+  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p) { return &p.a; }
+  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p) { return &p.b; }
+  static __device__ __forceinline__ Tile tile(const Params& p, int w) {
+    int m, n;
+    grid_tile(p.grid, w, &m, &n);
+    return Tile{m * pair::kTileM, n * pair::kTileN, 0, p.num_kb};
+  }
+  static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, EpiContext& c) {
+    const int row = c.row0 + c.lane;
+    const int col0 = t.n0 + c.part * 128;
+    int64_t target = row < p.rows ? p.targets[row] : -1;
+    if (target < col0 || target >= col0 + 128 || target >= p.vocab) target = -1;
+    const int at = target < 0 ? -1 : static_cast<int>(target) - col0;  // column of this warp's 128
+    float mx = -INFINITY, sum = 0.f, mine = 0.f;
+#pragma unroll 1
+    for (int ch = 0; ch < 2; ++ch) {
+      const int begin = col0 + ch * 64;
+      if (begin >= p.vocab) break;  // warp-uniform
+      float v[64];
+      {
+        uint32_t r0[32], r1[32];
+        tmem_ld_32x32(c.acc + c.part * 128 + ch * 64, r0);
+        tmem_ld_32x32(c.acc + c.part * 128 + ch * 64 + 32, r1);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          v[j] = __uint_as_float(r0[j]);
+          v[32 + j] = __uint_as_float(r1[j]);
+        }
+      }
+      if (begin + 64 > p.vocab) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j)
+          if (begin + j >= p.vocab) v[j] = -INFINITY;
+      }
+      const int in = at - ch * 64;
+      if (__any_sync(0xffffffffu, in >= 0 && in < 64)) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j)
+          if (in == j) mine = v[j];
+      }
+      float m[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+      for (int j = 4; j < 64; ++j) m[j & 3] = fmaxf(m[j & 3], v[j]);
+      const float next = fmaxf(mx, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+      const float base = next == -INFINITY ? 0.f : next * kLog2e;  // -inf - -inf is NaN
+      float s[4] = {sum * exp2_fast(fmaf(mx, kLog2e, -base)), 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 64; ++j) s[j & 3] += exp2_fast(fmaf(v[j], kLog2e, -base));
+      sum = (s[0] + s[1]) + (s[2] + s[3]);
+      mx = next;
+    }
+    if (row < p.rows) {
+      const long strip = 2L * (t.n0 / pair::kTileN) + c.part;
+      p.part[strip * p.rows + row] = make_float2(mx, sum);
+      if (at >= 0) p.picked[row] = mine;
+    }
+  }
+};
+
+// Joins a row's strips: 32 rows per block, warps share the strips and meet in shared memory.
+constexpr int kJoinWarps = 8;
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float next = fmaxf(m, m2);
+  const float base = next == -INFINITY ? 0.f : next;
+  s = s * exp2_fast((m - base) * kLog2e) + s2 * exp2_fast((m2 - base) * kLog2e);
+  m = next;
+}
+
+__global__ void __launch_bounds__(32 * kJoinWarps)
+ce_join_kernel(const float2* __restrict__ part, int strips, const float* __restrict__ picked,
+               const int64_t* __restrict__ targets, int64_t ignore, int rows, int vocab,
+               float shift, float* __restrict__ row_loss, float* __restrict__ lse2) {
+  __shared__ float2 sh[kJoinWarps][32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int row = blockIdx.x * 32 + lane;
+  float m = -INFINITY, s = 0.f;
+  if (row < rows) {
+#pragma unroll 4
+    for (int k = warp; k < strips; k += kJoinWarps) {
+      const float2 q = part[static_cast<long>(k) * rows + row];
+      join(m, s, q.x, q.y);
+    }
+  }
+  sh[warp][lane] = make_float2(m, s);
+  __syncthreads();
+  if (warp != 0 || row >= rows) return;
+#pragma unroll
+  for (int k = 1; k < kJoinWarps; ++k) join(m, s, sh[k][lane].x, sh[k][lane].y);
+  const int64_t t = targets[row];
+  const float lse = m + logf(s);
+  float loss, out;
+  if (t == ignore) {
+    loss = 0.f;
+    out = INFINITY;  // every probability of the row becomes zero
+  } else if (t < 0 || t >= vocab) {
+    loss = out = NAN;  // a target that is no entry of the vocabulary spoils the result visibly
+  } else {
+    loss = lse - picked[row];
+    out = fmaf(lse, kLog2e, -shift);
+  }
+  row_loss[row] = loss;
+  lse2[row] = out;
+}
+
+// totals = {sum of the rows' losses, rows that count}; out = their quotient or the sum.
+__global__ void __launch_bounds__(1024)
+ce_total_kernel(const float* __restrict__ row_loss, const int64_t* __restrict__ targets,
+                int64_t ignore, int rows, int mean, float* __restrict__ totals,
+                float* __restrict__ out) {
+  __shared__ double sums[32];
+  __shared__ int counts[32];
+  pdl_launch_dependents();
+  pdl_wait();
+  double sum = 0.0;
+  int count = 0;
+  for (int i = threadIdx.x; i < rows; i += blockDim.x) {
+    sum += row_loss[i];
+    count += targets[i] != ignore;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    count += __shfl_xor_sync(0xffffffffu, count, o);
+  }
+  if ((threadIdx.x & 31) == 0) {
+    sums[threadIdx.x >> 5] = sum;
+    counts[threadIdx.x >> 5] = count;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    sum = sums[threadIdx.x];
+    count = counts[threadIdx.x];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      count += __shfl_xor_sync(0xffffffffu, count, o);
+    }
+    if (threadIdx.x == 0) {
+      totals[0] = static_cast<float>(sum);
+      totals[1] = static_cast<float>(count);
+      out[0] = static_cast<float>(mean ? sum / count : sum);  // no counted row: 0 / 0
+    }
+  }
+}
+
+// --------------------------------------------- dl of a piece of the vocabulary ----
+struct DlogitsOp {
+  struct Params {
+    CUtensorMap a, b, out;
+    Grid grid;
+    int total, num_kb;
+    uint32_t idesc;
+    int* status;
+    const int64_t* targets;
+    const float* lse2;   // log-sum-exp in powers of two, less the shift
+    float one;           // 1, or 2^12 for fp16
+    int rows, vocab_begin, width, fp16;
+  };
+  static constexpr bool kAMN = false, kBMN = false;
+  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p) { return &p.a; }
+  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p) { return &p.b; }
+  static __device__ __forceinline__ Tile tile(const Params& p, int w) {
+    int m, n;
+    grid_tile(p.grid, w, &m, &n);
+    return Tile{m * pair::kTileM, n * pair::kTileN, 0, p.num_kb};
+  }
+  static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, EpiContext& c) {
+    const int row = c.row0 + c.lane;
+    const int col0 = t.n0 + c.part * 128;
+    float lse2 = INFINITY;
+    int at = -1;
+    if (row < p.rows) {
+      lse2 = p.lse2[row];
+      const int64_t target = p.targets[row] - p.vocab_begin;
+      if (target >= col0 && target < col0 + 128) at = static_cast<int>(target) - col0;
+    }
+    if (lse2 == INFINITY) at = -1;  // ignored
+#pragma unroll 1
+    for (int ch = 0; ch < 2; ++ch) {
+      const int begin = col0 + ch * 64;
+      if (begin >= p.width || c.row0 >= p.rows) break;  // warp-uniform
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[32];
+        pair::load_acc(c.acc + c.part * 128 + ch * 64 + h * 32, v);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = exp2_fast(fmaf(v[j], kLog2e, -lse2));
+        const int in = at - ch * 64 - h * 32;
+        if (__any_sync(0xffffffffu, in >= 0 && in < 32)) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (in == j) v[j] -= p.one;
+        }
+        if (h == 0) pair::stage_reuse(c.lane);
+        pair::stage_16(c.smem, c.lane, h, v, p.fp16);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (c.lane == 0) {
+        pair::store_3d(&p.out, c.smem, begin, c.row0, 0);
+        tma_store_commit();
+      }
+    }
+  }
+};
+
+// --------------------------------------------------- products that consume dl ----
+enum OutKind : int { kOut16 = 0, kOutF32 = 1, kOutF32Add = 2 };
+
+struct GradScale {
+  const float* grad;     // incoming gradient, a device scalar (NULL: 1)
+  const float* totals;   // {sum, count}: divide by the count (NULL: do not)
+  float factor;
+};
+__device__ __forceinline__ float grad_scale(const GradScale& g) {
+  float s = g.factor;
+  if (g.grad != nullptr) s *= g.grad[0];
+  if (g.totals != nullptr) {
+    const float count = g.totals[1];
+    s = count > 0.f ? s / count : 0.f;
+  }
+  return s;
+}
+
+// out[M, N] = scale * A B^T;  A is dl (MN-major for dW, K-major for dh), B MN-major.
+template <bool AMN>
+struct GradOp {
+  struct Params {
+    CUtensorMap a, b, out;
+    Grid grid;
+    int total, num_kb;
+    uint32_t idesc;
+    int* status;
+    GradScale scale;
+    int rows, cols, kind, fp16;
+  };
+  static constexpr bool kAMN = AMN, kBMN = true;
+  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p) { return &p.a; }
+  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p) { return &p.b; }
+  static __device__ __forceinline__ Tile tile(const Params& p, int w) {
+    int m, n;
+    grid_tile(p.grid, w, &m, &n);
+    return Tile{m * pair::kTileM, n * pair::kTileN, 0, p.num_kb};
+  }
+  static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, EpiContext& c) {
+    const float scale = grad_scale(p.scale);
+    const int col0 = t.n0 + c.part * 128;
+    if (c.row0 >= p.rows) return;  // warp-uniform
+#pragma unroll 1
+    for (int ch = 0; ch < 4; ++ch) {
+      const int begin = col0 + ch * 32;
+      if (begin >= p.cols) break;  // warp-uniform
+      float v[32];
+      pair::load_acc(c.acc + c.part * 128 + ch * 32, v);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] *= scale;
+      if (p.kind == kOut16) {
+        // two 32-column steps share a 64-column line
+        if ((ch & 1) == 0) pair::stage_reuse(c.lane);
+        pair::stage_16(c.smem, c.lane, ch & 1, v, p.fp16);
+        if ((ch & 1) == 0 && begin + 32 < p.cols) continue;
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (c.lane == 0) {
+          pair::store_3d(&p.out, c.smem, begin & ~63, c.row0, 0);
+          tma_store_commit();
+        }
+      } else {
+        pair::stage_reuse(c.lane);
+        pair::stage_32(c.smem, c.lane, v);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (c.lane == 0) {
+          if (p.kind == kOutF32Add) pair::reduce_add_3d(&p.out, c.smem, begin, c.row0, 0);
+          else pair::store_3d(&p.out, c.smem, begin, c.row0, 0);
+          tma_store_commit();
+        }
+      }
+    }
+  }
+};
+
+// dh in the operands' type from the fp32 sum over the pieces; rows of `dim` (a multiple of 8).
+__global__ void __launch_bounds__(256)
+ce_dh_kernel(const float* __restrict__ sum, long vecs, int vecs_per_row, void* __restrict__ out,
+             long ld_out, GradScale g, int fp16) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const float scale = grad_scale(g);
+  for (long i = blockIdx.x * static_cast<long>(blockDim.x) + threadIdx.x; i < vecs;
+       i += static_cast<long>(gridDim.x) * blockDim.x) {
+    const float4 a = reinterpret_cast<const float4*>(sum)[2 * i];
+    const float4 b = reinterpret_cast<const float4*>(sum)[2 * i + 1];
+    const long row = i / vecs_per_row;
+    const long col = (i - row * vecs_per_row) * 8;
+    uint4 q;
+    q.x = pair::pack_16(fp16, a.x * scale, a.y * scale);
+    q.y = pair::pack_16(fp16, a.z * scale, a.w * scale);
+    q.z = pair::pack_16(fp16, b.x * scale, b.y * scale);
+    q.w = pair::pack_16(fp16, b.z * scale, b.w * scale);
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + row * ld_out + col) = q;
+  }
+}
+
+// ------------------------------------------------------------------- host ----
+bool aligned16(const void* ptr, long ld, int elem) {
+  return ptr != nullptr && (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && ld > 0 &&
+         (ld * elem) % 16 == 0;
+}
+
+int tiles_of(long n, int size) { return static_cast<int>((n + size - 1) / size); }
+
+// Row tiles of a band: at most 32 MB of rows, at least one round of the pairs.
+int band_of(int mt, int dim) {
+  const long rows = (32L << 20) / (2L * dim);
+  const int band = static_cast<int>(rows / pair::kTileM);
+  return band < 4 ? (mt < 4 ? mt : 4) : (band < mt ? band : mt);
+}
+
+int check(const SflLinearCe* a) {
+  if (a == nullptr || a->rows < 1 || a->dim < 8 || a->dim % 8 != 0 || a->vocab < 1) return -2;
+  if (!aligned16(a->hidden, a->ld_hidden, 2) || !aligned16(a->weight, a->ld_weight, 2)) return -2;
+  if (a->ld_hidden < a->dim || a->ld_weight < a->dim) return -2;
+  if (a->targets == nullptr || a->lse2 == nullptr) return -2;
+  // tile counts are 32-bit
+  if (static_cast<long>(tiles_of(a->rows, pair::kTileM)) * tiles_of(a->vocab, pair::kTileN) > 0x7fffffffL)
+    return -2;
+  return 0;
+}
+
+}  // namespace
+}  // namespace sfl
+
+extern "C" long sfl_linear_ce_part_bytes(int rows, int vocab) {
+  using namespace sfl;
+  if (rows < 1 || vocab < 1) return -1;
+  // (max, sum) per row and 128 columns, and the target's logit
+  return static_cast<long>(rows) * (2L * tiles_of(vocab, pair::kTileN) * 8 + 4);
+}
+
+extern "C" int sfl_linear_ce_fwd(const SflLinearCe* a, void* part, long part_bytes, float* row_loss,
+                                 int mean, float* totals, float* loss, void* stream_) {
+  using namespace sfl;
+  const int bad = check(a);
+  if (bad != 0) return bad;
+  if (part == nullptr || row_loss == nullptr || (totals == nullptr) != (loss == nullptr) ||
+      part_bytes < sfl_linear_ce_part_bytes(a->rows, a->vocab))
+    return -2;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  StatsOp::Params p{};
+  int rc = pair::map_operand(&p.a, a->hidden, false, a->rows, a->dim, a->ld_hidden, 1,
+                             static_cast<uint64_t>(a->rows) * a->ld_hidden);
+  if (rc == 0)
+    rc = pair::map_operand(&p.b, a->weight, false, a->vocab, a->dim, a->ld_weight, 1,
+                           static_cast<uint64_t>(a->vocab) * a->ld_weight);
+  if (rc != 0) return 1000 + rc;
+  p.grid.mt = tiles_of(a->rows, pair::kTileM);
+  p.grid.nt = tiles_of(a->vocab, pair::kTileN);
+  p.grid.band = band_of(p.grid.mt, a->dim);
+  p.total = p.grid.mt * p.grid.nt;
+  p.num_kb = tiles_of(a->dim, pair::kBK);
+  p.idesc = pair::instruction_descriptor(a->fp16, false, false);
+  p.status = a->status;
+  p.targets = a->targets;
+  p.part = static_cast<float2*>(part);
+  p.picked = reinterpret_cast<float*>(p.part + 2L * p.grid.nt * a->rows);
+  p.rows = a->rows;
+  p.vocab = a->vocab;
+  rc = pair::launch_pair<StatsOp>(p, stream);
+  if (rc != 0) return rc;
+  rc = launch_pdl(ce_join_kernel, dim3(tiles_of(a->rows, 32)), dim3(32 * kJoinWarps), 0, stream,
+                  static_cast<const float2*>(p.part), 2 * p.grid.nt,
+                  static_cast<const float*>(p.picked), a->targets, a->ignore_index, a->rows,
+                  a->vocab, a->fp16 ? static_cast<float>(kFp16Shift) : 0.f, row_loss, a->lse2);
+  if (rc != 0 || loss == nullptr) return rc;
+  return launch_pdl(ce_total_kernel, dim3(1), dim3(1024), 0, stream,
+                    static_cast<const float*>(row_loss), a->targets, a->ignore_index, a->rows, mean,
+                    totals, loss);
+}
+
+extern "C" int sfl_linear_ce_bwd(const SflLinearCe* a, const SflLinearCeGrad* g, void* stream_) {
+  using namespace sfl;
+  const int bad = check(a);
+  if (bad != 0) return bad;
+  if (g == nullptr || g->piece < pair::kTileN || g->piece % pair::kTileN != 0 ||
+      g->dw_kind < kOut16 || g->dw_kind > kOutF32Add)
+    return -2;
+  const int dw_elem = g->dw_kind == kOut16 ? 2 : 4;
+  if (!aligned16(g->dlogits, g->piece, 2) || !aligned16(g->dh, g->ld_dh, 2) ||
+      !aligned16(g->dw, g->ld_dw, dw_elem) || g->ld_dh < a->dim || g->ld_dw < a->dim)
+    return -2;
+  const int pieces = tiles_of(a->vocab, g->piece);
+  if (pieces > 1 && !aligned16(g->dh_sum, a->dim, 4)) return -2;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+  const uint64_t rows = a->rows, dim = a->dim;
+  const float factor = a->fp16 ? 1.0f / (1 << kFp16Shift) : 1.0f;
+  const GradScale scale{g->grad, g->totals, factor};
+
+  for (int i = 0; i < pieces; ++i) {
+    const long begin = static_cast<long>(i) * g->piece;
+    const int width = static_cast<int>(a->vocab - begin < g->piece ? a->vocab - begin : g->piece);
+    const uint16_t* w = static_cast<const uint16_t*>(a->weight) + begin * a->ld_weight;
+    const uint64_t dl_size = rows * g->piece;
+
+    DlogitsOp::Params d{};
+    int rc = pair::map_operand(&d.a, a->hidden, false, rows, dim, a->ld_hidden, 1,
+                               rows * a->ld_hidden);
+    if (rc == 0)
+      rc = pair::map_operand(&d.b, w, false, width, dim, a->ld_weight, 1,
+                             static_cast<uint64_t>(width) * a->ld_weight);
+    if (rc == 0)
+      rc = pair::map_3d(&d.out, g->dlogits, 2, width, rows, g->piece, 1, dl_size, 64, 32);
+    if (rc != 0) return 1000 + rc;
+    d.grid = Grid{tiles_of(rows, pair::kTileM), tiles_of(width, pair::kTileN), 0};
+    d.grid.band = band_of(d.grid.mt, a->dim);
+    d.total = d.grid.mt * d.grid.nt;
+    d.num_kb = tiles_of(dim, pair::kBK);
+    d.idesc = pair::instruction_descriptor(a->fp16, false, false);
+    d.status = a->status;
+    d.targets = a->targets;
+    d.lse2 = a->lse2;
+    d.one = a->fp16 ? static_cast<float>(1 << kFp16Shift) : 1.0f;
+    d.rows = a->rows;
+    d.vocab_begin = static_cast<int>(begin);
+    d.width = width;
+    d.fp16 = a->fp16;
+    rc = pair::launch_pair<DlogitsOp>(d, stream);
+    if (rc != 0) return rc;
+
+    GradOp<true>::Params q{};
+    rc = pair::map_operand(&q.a, g->dlogits, true, width, rows, g->piece, 1, dl_size);
+    if (rc == 0)
+      rc = pair::map_operand(&q.b, a->hidden, true, dim, rows, a->ld_hidden, 1,
+                             rows * a->ld_hidden);
+    if (rc == 0)
+      rc = pair::map_3d(&q.out, static_cast<uint8_t*>(g->dw) + begin * g->ld_dw * dw_elem, dw_elem,
+                        dim, width, g->ld_dw, 1, static_cast<uint64_t>(width) * g->ld_dw,
+                        128 / dw_elem, 32);
+    if (rc != 0) return 1000 + rc;
+    q.grid = Grid{tiles_of(width, pair::kTileM), tiles_of(dim, pair::kTileN), 0};
+    q.grid.band = q.grid.mt;
+    q.total = q.grid.mt * q.grid.nt;
+    q.num_kb = tiles_of(rows, pair::kBK);
+    q.idesc = pair::instruction_descriptor(a->fp16, true, true);
+    q.status = a->status;
+    q.scale = scale;
+    q.rows = width;
+    q.cols = a->dim;
+    q.kind = g->dw_kind;
+    q.fp16 = a->fp16;
+    rc = pair::launch_pair<GradOp<true>>(q, stream);
+    if (rc != 0) return rc;
+
+    GradOp<false>::Params h{};
+    rc = pair::map_operand(&h.a, g->dlogits, false, rows, width, g->piece, 1, dl_size);
+    if (rc == 0)
+      rc = pair::map_operand(&h.b, w, true, dim, width, a->ld_weight, 1,
+                             static_cast<uint64_t>(width) * a->ld_weight);
+    if (rc == 0 && pieces == 1)
+      rc = pair::map_3d(&h.out, g->dh, 2, dim, rows, g->ld_dh, 1, rows * g->ld_dh, 64, 32);
+    else if (rc == 0)
+      rc = pair::map_3d(&h.out, g->dh_sum, 4, dim, rows, dim, 1, rows * dim, 32, 32);
+    if (rc != 0) return 1000 + rc;
+    h.grid = Grid{tiles_of(rows, pair::kTileM), tiles_of(dim, pair::kTileN), 0};
+    h.grid.band = h.grid.mt;
+    h.total = h.grid.mt * h.grid.nt;
+    h.num_kb = tiles_of(width, pair::kBK);
+    h.idesc = pair::instruction_descriptor(a->fp16, false, true);
+    h.status = a->status;
+    h.scale = pieces == 1 ? scale : GradScale{nullptr, nullptr, 1.0f};
+    h.rows = a->rows;
+    h.cols = a->dim;
+    h.kind = pieces == 1 ? kOut16 : (i == 0 ? kOutF32 : kOutF32Add);
+    h.fp16 = a->fp16;
+    rc = pair::launch_pair<GradOp<false>>(h, stream);
+    if (rc != 0) return rc;
+  }
+  if (pieces == 1) return 0;
+  const long vecs = static_cast<long>(a->rows) * a->dim / 8;
+  const long blocks = (vecs + 255) / 256;
+  return launch_pdl(ce_dh_kernel, dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)),
+                    dim3(256), 0, stream, static_cast<const float*>(g->dh_sum), vecs, a->dim / 8,
+                    g->dh, g->ld_dh, scale, a->fp16);
+}

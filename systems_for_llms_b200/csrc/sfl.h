@@ -97,6 +97,46 @@ int sfl_rmsnorm_dw_reduce2(const float* partial_a, float* dw_a, int accumulate_a
 int sfl_cross_entropy(const void* logits_bf16, long ld, const int64_t* targets, float* row_loss,
                       void* dlogits_bf16, float grad_scale, int rows, int vocab, void* stream);
 
+/* --------------------------- cross entropy of a projection, without its logits -- */
+/* hidden 16-bit [rows, dim] and weight 16-bit [vocab, dim] (bf16, or fp16 when fp16 is set), both
+ * with 16-byte aligned rows; dim a multiple of 8.  targets int64 [rows]: rows whose target is
+ * ignore_index do not count, any other target outside [0, vocab) makes the result NaN.  lse2
+ * [rows] is written by the forward and read by the backward call. */
+typedef struct SflLinearCe {
+  const void* hidden;
+  long ld_hidden;
+  const void* weight;
+  long ld_weight;
+  const int64_t* targets;
+  int64_t ignore_index;
+  int rows, dim, vocab, fp16;
+  float* lse2;
+  int* status;
+} SflLinearCe;
+
+/* row_loss [rows] fp32.  With totals and loss (both or neither): totals = {sum, counted rows} and
+ * loss = their quotient (mean) or the sum.  part: sfl_linear_ce_part_bytes of scratch. */
+long sfl_linear_ce_part_bytes(int rows, int vocab);
+int sfl_linear_ce_fwd(const SflLinearCe* a, void* part, long part_bytes, float* row_loss, int mean,
+                      float* totals, float* loss, void* stream);
+
+/* dh 16-bit [rows, dim] and dw [vocab, dim] (dw_kind 0: 16-bit, 1: fp32, 2: added to fp32), both
+ * times the device scalar grad (NULL: 1) and over totals[1] (NULL: not).  The vocabulary is walked
+ * in pieces of `piece` entries (a multiple of 256): dlogits is 16-bit [rows, piece] scratch, dh_sum
+ * fp32 [rows, dim] scratch (NULL allowed when one piece is enough). */
+typedef struct SflLinearCeGrad {
+  const float* grad;
+  const float* totals;
+  void* dlogits;
+  float* dh_sum;
+  void* dh;
+  long ld_dh;
+  void* dw;
+  long ld_dw;
+  int dw_kind, piece;
+} SflLinearCeGrad;
+int sfl_linear_ce_bwd(const SflLinearCe* a, const SflLinearCeGrad* g, void* stream);
+
 /* ------------------------------------------------------------- optimizer -- */
 /* Sum of squares of a flat fp32 buffer -> partial[blocks]; deterministic. */
 int sfl_sqnorm_blocks(long n);

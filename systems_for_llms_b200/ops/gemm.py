@@ -35,6 +35,15 @@ def status_word(device: torch.device) -> torch.Tensor:
     return word
 
 
+def captured_status_word(device: torch.device) -> torch.Tensor:
+    """``status_word`` for operators that may be called while a CUDA graph is captured.  The word
+    lives as long as the process, so it must not come out of a graph's memory pool."""
+    if device not in _status_words and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("call the operator (or ops.gemm.status_word) once on this device before "
+                           "capturing it in a CUDA graph")
+    return status_word(device)
+
+
 def check_status(device: torch.device | None = None) -> None:
     """Raises if any kernel on ``device`` reported a timed-out wait (host sync)."""
     for dev, word in list(_status_words.items()):

@@ -1,0 +1,202 @@
+"""Softmax cross entropy of a vocabulary projection that keeps no logits.
+
+``linear_cross_entropy(hidden, weight, targets)`` is
+``cross_entropy(hidden @ weight.T, targets)`` and its gradients, computed by csrc/linear_ce.cu
+in pieces of the vocabulary: forward keeps one log-sum-exp per row, backward computes the
+logits of a piece again and consumes them at once.  Memory beyond inputs and results is
+``2 * rows * piece`` bytes for the piece in hand (``piece_size``) and 16 bytes per row and 256
+entries of the vocabulary for the statistics.
+
+The head of models/fused.py that keeps bf16 logits does fewer operations (6 N D V against
+8 N D V) and rounds them; this one is for vocabularies whose logits are too large to keep, and
+never rounds a logit.  The reference materialises logits and softmax
+(src/llmlab/training/loss.py:4-22).
+"""
+
+from __future__ import annotations
+
+from ctypes import POINTER, Structure, byref, c_int, c_int64, c_long, c_void_p
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import lib as _lib
+from .gemm import captured_status_word
+
+REDUCTIONS = ("mean", "sum", "none")
+PIECE_STEP = 256                 # a piece is whole 256-column tiles
+PIECE_BYTES = 192 << 20          # of dl in flight
+MIN_PIECE = 2048
+_DTYPES = (torch.bfloat16, torch.float16)
+_OUT_16, _OUT_F32, _OUT_F32_ADD = range(3)
+
+
+class LinearCe(Structure):
+    """Mirror of ``SflLinearCe`` in csrc/sfl.h."""
+
+    _fields_ = [("hidden", c_void_p), ("ld_hidden", c_long), ("weight", c_void_p),
+                ("ld_weight", c_long), ("targets", c_void_p), ("ignore_index", c_int64),
+                ("rows", c_int), ("dim", c_int), ("vocab", c_int), ("fp16", c_int),
+                ("lse2", c_void_p), ("status", c_void_p)]
+
+
+class LinearCeGrad(Structure):
+    """Mirror of ``SflLinearCeGrad`` in csrc/sfl.h."""
+
+    _fields_ = [("grad", c_void_p), ("totals", c_void_p), ("dlogits", c_void_p),
+                ("dh_sum", c_void_p), ("dh", c_void_p), ("ld_dh", c_long), ("dw", c_void_p),
+                ("ld_dw", c_long), ("dw_kind", c_int), ("piece", c_int)]
+
+
+_P = c_void_p
+_lib.register_signature("sfl_linear_ce_part_bytes", [c_int, c_int])
+_lib.register_signature("sfl_linear_ce_fwd", [POINTER(LinearCe), _P, c_long, _P, c_int, _P, _P, _P])
+_lib.register_signature("sfl_linear_ce_bwd", [POINTER(LinearCe), POINTER(LinearCeGrad), _P])
+
+
+def piece_size(rows: int, vocab: int) -> int:
+    """Entries of the vocabulary per piece: as many as keep dl at ``PIECE_BYTES``, at least
+    ``MIN_PIECE`` (smaller pieces leave the products too few tiles for the SMs), at most all."""
+    fit = PIECE_BYTES // (2 * rows) // PIECE_STEP * PIECE_STEP
+    return min(max(fit, MIN_PIECE), -(-vocab // PIECE_STEP) * PIECE_STEP)
+
+
+def _check(hidden, weight, targets) -> None:
+    if not isinstance(hidden, torch.Tensor) or not hidden.is_cuda:
+        raise ValueError("hidden must be a CUDA tensor")
+    if hidden.dtype not in _DTYPES or weight.dtype != hidden.dtype:
+        raise TypeError("hidden and weight must both be bf16 or both be fp16")
+    if hidden.ndim < 1 or weight.ndim != 2 or weight.shape[1] != hidden.shape[-1]:
+        raise ValueError("expected hidden [..., dim] and weight [vocab, dim]")
+    if weight.device != hidden.device or targets.device != hidden.device:
+        raise ValueError("hidden, weight and targets must be on the same device")
+    dim = hidden.shape[-1]
+    if dim == 0 or dim % 8:
+        raise ValueError("dim must be a positive multiple of 8")
+    if weight.shape[0] == 0:
+        raise ValueError("the vocabulary is empty")
+    if targets.dtype != torch.int64 or targets.shape != hidden.shape[:-1]:
+        raise ValueError("targets must be int64 with the shape of hidden without its last dimension")
+    if max(targets.numel(), weight.shape[0]) >= 2**31:
+        raise ValueError("2**31 rows or vocabulary entries are not supported")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as a matrix whose rows TMA can address (16-byte aligned, contiguous), copying only
+    what does not lie that way already."""
+    t = t.reshape(-1, t.shape[-1])
+    if t.stride(1) != 1 or t.stride(0) % 8 or t.stride(0) < t.shape[1] or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _args(hidden, weight, targets, ignore_index, lse2) -> LinearCe:
+    return LinearCe(hidden=hidden.data_ptr(), ld_hidden=hidden.stride(0), weight=weight.data_ptr(),
+                    ld_weight=weight.stride(0), targets=targets.data_ptr(),
+                    ignore_index=ignore_index, rows=hidden.shape[0], dim=hidden.shape[1],
+                    vocab=weight.shape[0], fp16=int(hidden.dtype == torch.float16),
+                    lse2=lse2.data_ptr(), status=captured_status_word(hidden.device).data_ptr())
+
+
+def linear_ce_forward(hidden, weight, targets, ignore_index: int, mean: bool | None):
+    """Kernels of the forward pass over prepared matrices: ``(row_loss, lse2, totals, loss)``.
+    ``mean`` None leaves out the reduction (totals and loss are None)."""
+    rows, vocab = hidden.shape[0], weight.shape[0]
+    dev = hidden.device
+    handle = _lib.lib()
+    size = handle.sfl_linear_ce_part_bytes(rows, vocab)
+    part = torch.empty(size, dtype=torch.uint8, device=dev)
+    stats = torch.empty(2 * rows + 3, dtype=torch.float32, device=dev)
+    row_loss, lse2, totals, loss = stats.split((rows, rows, 2, 1))
+    args = _args(hidden, weight, targets, ignore_index, lse2)
+    reduce = mean is not None
+    with _lib.on_device(dev):
+        code = handle.sfl_linear_ce_fwd(byref(args), part.data_ptr(), size, row_loss.data_ptr(),
+                                        int(bool(mean)), totals.data_ptr() if reduce else None,
+                                        loss.data_ptr() if reduce else None, _lib.stream_ptr())
+    _lib.check(code, "sfl_linear_ce_fwd")
+    return row_loss, lse2, (totals if reduce else None), (loss[0] if reduce else None)
+
+
+def linear_ce_backward(hidden, weight, targets, ignore_index: int, lse2, grad, totals, dw,
+                       accumulate: bool = False, piece: int | None = None) -> torch.Tensor:
+    """Kernels of the backward pass: writes (or, for fp32 ``dw``, adds to) the weight gradient and
+    returns dh.  ``grad`` is a device scalar; with ``totals`` both are divided by the count."""
+    rows, dim = hidden.shape
+    vocab = weight.shape[0]
+    dev = hidden.device
+    if dw.dtype == torch.float32:
+        kind = _OUT_F32_ADD if accumulate else _OUT_F32
+    elif dw.dtype == hidden.dtype and not accumulate:
+        kind = _OUT_16
+    else:
+        raise ValueError("dw must be fp32, or of the operands' type when it is overwritten")
+    if piece is None:
+        piece = piece_size(rows, vocab)
+    dlogits = torch.empty(rows, piece, dtype=hidden.dtype, device=dev)
+    dh = torch.empty(rows, dim, dtype=hidden.dtype, device=dev)
+    dh_sum = torch.empty(rows, dim, dtype=torch.float32, device=dev) if piece < vocab else None
+    args = _args(hidden, weight, targets, ignore_index, lse2)
+    grads = LinearCeGrad(grad=_lib.ptr(grad), totals=_lib.ptr(totals), dlogits=dlogits.data_ptr(),
+                         dh_sum=_lib.ptr(dh_sum), dh=dh.data_ptr(), ld_dh=dim, dw=dw.data_ptr(),
+                         ld_dw=dw.stride(0), dw_kind=kind, piece=piece)
+    with _lib.on_device(dev):
+        code = _lib.lib().sfl_linear_ce_bwd(byref(args), byref(grads), _lib.stream_ptr())
+    _lib.check(code, "sfl_linear_ce_bwd")
+    return dh
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, ignore_index, mean):
+        h, w = _rows(hidden), _rows(weight)
+        t = targets.reshape(-1).contiguous()
+        _, lse2, totals, loss = linear_ce_forward(h, w, t, ignore_index, mean)
+        ctx.save_for_backward(h, w, t, lse2, totals)
+        ctx.ignore_index, ctx.mean, ctx.shape = ignore_index, mean, hidden.shape
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        h, w, t, lse2, totals = ctx.saved_tensors
+        dw = torch.empty(w.shape, dtype=w.dtype, device=w.device)
+        dh = linear_ce_backward(h, w, t, ctx.ignore_index, lse2, grad.float(),
+                                totals if ctx.mean else None, dw)
+        return dh.view(ctx.shape), dw, None, None, None
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *,
+                         ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
+    """Cross entropy of ``hidden [..., dim] @ weight [vocab, dim].T`` with ``targets [...]``.
+
+    ``hidden`` and ``weight`` are both bf16 or both fp16, ``dim`` a multiple of 8, ``targets``
+    int64.  Rows whose target is ``ignore_index`` add nothing to the loss or the gradients (their
+    hidden states must still be finite: a product with them runs); any other target outside the
+    vocabulary makes the result NaN.  ``"mean"`` divides by the rows that count (NaN when none
+    does, with zero gradients), ``"sum"`` does not; both return an fp32 scalar that is
+    differentiable in ``hidden`` and ``weight``, with gradients in their type.  ``"none"`` returns
+    the fp32 loss of each row for scoring and is refused where a gradient would be needed.
+    """
+    if reduction not in REDUCTIONS:
+        raise ValueError("reduction must be one of " + ", ".join(REDUCTIONS))
+    if type(ignore_index) is not int or not -2**63 <= ignore_index < 2**63:
+        raise ValueError("ignore_index must be an integer")
+    _check(hidden, weight, targets)
+    needs_grad = torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad)
+    if reduction == "none" and needs_grad:
+        raise ValueError("reduction='none' is for scoring and carries no gradient: detach hidden "
+                         "and weight, or call it under torch.no_grad()")
+    if targets.numel() == 0:
+        if reduction == "none":
+            return torch.zeros(targets.shape, dtype=torch.float32, device=hidden.device)
+        # the sum of nothing keeps its place in the graph; the mean of nothing is NaN
+        nothing = hidden.float().sum() + weight[:0].float().sum()
+        return nothing + float("nan") if reduction == "mean" else nothing
+    if needs_grad:
+        return _LinearCrossEntropy.apply(hidden, weight, targets, ignore_index, reduction == "mean")
+    h, w = _rows(hidden), _rows(weight)
+    t = targets.reshape(-1).contiguous()
+    mean = None if reduction == "none" else reduction == "mean"
+    row_loss, _, _, loss = linear_ce_forward(h, w, t, ignore_index, mean)
+    return row_loss.view(targets.shape) if mean is None else loss
