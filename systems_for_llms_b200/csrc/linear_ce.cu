@@ -13,7 +13,7 @@
 // rows are then final, and the piece's share of dh).  A piece is sized to stay in the L2 cache as
 // far as the matrices allow, so what the operator moves beyond its inputs and outputs does not
 // grow with the vocabulary.  The price is the second projection: 8 N D V operations for forward
-// and backward where keeping the logits takes 6.
+// and backward where keeping the logits takes 6.  Both products of a piece run in one launch.
 //
 // Logits are never rounded: statistics and losses see fp32 accumulators.  dl is rounded once to
 // the operands' type, which is what the tensor cores multiply; fp16 holds dl times 2^12, so
@@ -24,6 +24,10 @@
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
+
+#include <algorithm>
+#include <functional>
+#include <utility>
 
 #include "pair_gemm.cuh"
 #include "sfl.h"
@@ -59,25 +63,30 @@ __device__ __forceinline__ void grid_tile(const Grid& g, int w, int* m, int* n) 
 }
 
 // ---------------------------------------------------- row statistics (forward) ----
-struct StatsOp {
+struct StatsOp : pair::RoundRobin {
   struct Params {
     CUtensorMap a, b;
     Grid grid;
     int total, num_kb;
-    uint32_t idesc;
+    bool fp16;
     int* status;
     const int64_t* targets;
     float2* part;      // [2 * nt][rows]
     float* picked;     // [rows]: the target's logit
     int rows, vocab;
   };
-  static constexpr bool kAMN = false, kBMN = false;
-  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p) { return &p.a; }
-  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p) { return &p.b; }
+  static __device__ __forceinline__ bool a_mn(const Tile&) { return false; }
+  static __device__ __forceinline__ bool b_mn(const Tile&) { return false; }
+  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile&) {
+    return &p.a;
+  }
+  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile&) {
+    return &p.b;
+  }
   static __device__ __forceinline__ Tile tile(const Params& p, int w) {
     int m, n;
     grid_tile(p.grid, w, &m, &n);
-    return Tile{m * pair::kTileM, n * pair::kTileN, 0, p.num_kb};
+    return Tile{m * pair::kTileM, n * pair::kTileN, 0, p.num_kb, 0, 0};
   }
   static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, EpiContext& c) {
     const int row = c.row0 + c.lane;
@@ -221,25 +230,30 @@ ce_total_kernel(const float* __restrict__ row_loss, const int64_t* __restrict__ 
 }
 
 // --------------------------------------------- dl of a piece of the vocabulary ----
-struct DlogitsOp {
+struct DlogitsOp : pair::RoundRobin {
   struct Params {
     CUtensorMap a, b, out;
     Grid grid;
     int total, num_kb;
-    uint32_t idesc;
+    bool fp16;
     int* status;
     const int64_t* targets;
     const float* lse2;   // log-sum-exp in powers of two, less the shift
     float one;           // 1, or 2^12 for fp16
-    int rows, vocab_begin, width, fp16;
+    int rows, vocab_begin, width;
   };
-  static constexpr bool kAMN = false, kBMN = false;
-  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p) { return &p.a; }
-  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p) { return &p.b; }
+  static __device__ __forceinline__ bool a_mn(const Tile&) { return false; }
+  static __device__ __forceinline__ bool b_mn(const Tile&) { return false; }
+  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile&) {
+    return &p.a;
+  }
+  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile&) {
+    return &p.b;
+  }
   static __device__ __forceinline__ Tile tile(const Params& p, int w) {
     int m, n;
     grid_tile(p.grid, w, &m, &n);
-    return Tile{m * pair::kTileM, n * pair::kTileN, 0, p.num_kb};
+    return Tile{m * pair::kTileM, n * pair::kTileN, 0, p.num_kb, 0, 0};
   }
   static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, EpiContext& c) {
     const int row = c.row0 + c.lane;
@@ -299,47 +313,85 @@ __device__ __forceinline__ float grad_scale(const GradScale& g) {
   return s;
 }
 
-// out[M, N] = scale * A B^T;  A is dl (MN-major for dW, K-major for dh), B MN-major.
-template <bool AMN>
+// Both products of a piece in one launch: dW = dl^T h (A = dl read MN-major) and dh = dl W, whose
+// reduction runs over the piece and may be split into parts that each leave their own fp32 sum.
+// One product after the other leaves the pairs idle at the end of each (dh of 4096 x 1024 has 64
+// tiles for 74 pairs); dealt together, the longest tiles first, only the end of both is ragged
+// (4096 x 1024 x 10000: 132 -> 103 us).  begin[c] .. begin[c + 1] are the tiles of cluster c.
+constexpr int kMaxClusters = 96;
+enum Product : int { kDw = 0, kDh = 1 };
+
 struct GradOp {
   struct Params {
-    CUtensorMap a, b, out;
-    Grid grid;
-    int total, num_kb;
-    uint32_t idesc;
+    CUtensorMap dl_mn, dl_k, h, w, dw, dh;
+    int total, dh_tiles;         // dh's tiles are the first of each cluster's range
+    bool fp16;
     int* status;
-    GradScale scale;
-    int rows, cols, kind, fp16;
+    GradScale scale;             // of dw, and of dh when it is final
+    int dw_mt, dh_mt, dh_nt;
+    int dw_kb, dh_kb, dh_part_kb;  // steps of the two reductions, and of a part of dh's
+    int rows, width, dim;
+    int dw_kind, dh_kind;
+    int dh_begin[kMaxClusters + 1], dw_begin[kMaxClusters + 1];
   };
-  static constexpr bool kAMN = AMN, kBMN = true;
-  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p) { return &p.a; }
-  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p) { return &p.b; }
+  // A tile's number: dh tiles come first, then dw tiles.
+  static __device__ __forceinline__ int first(const Params& p, int c) {
+    if (p.dh_begin[c] < p.dh_begin[c + 1]) return p.dh_begin[c];
+    return p.dw_begin[c] < p.dw_begin[c + 1] ? p.dh_tiles + p.dw_begin[c] : p.total;
+  }
+  static __device__ __forceinline__ int next(const Params& p, int w, int c, int) {
+    if (w < p.dh_tiles) {
+      if (w + 1 < p.dh_begin[c + 1]) return w + 1;
+      return p.dw_begin[c] < p.dw_begin[c + 1] ? p.dh_tiles + p.dw_begin[c] : p.total;
+    }
+    return w + 1 < p.dh_tiles + p.dw_begin[c + 1] ? w + 1 : p.total;
+  }
   static __device__ __forceinline__ Tile tile(const Params& p, int w) {
-    int m, n;
-    grid_tile(p.grid, w, &m, &n);
-    return Tile{m * pair::kTileM, n * pair::kTileN, 0, p.num_kb};
+    if (w >= p.dh_tiles) {
+      w -= p.dh_tiles;
+      return Tile{w % p.dw_mt * pair::kTileM, w / p.dw_mt * pair::kTileN, 0, p.dw_kb, 0, kDw};
+    }
+    const int per_part = p.dh_mt * p.dh_nt;
+    const int part = w / per_part;
+    w -= part * per_part;
+    const int kb0 = part * p.dh_part_kb;
+    const int left = p.dh_kb - kb0;
+    return Tile{w % p.dh_mt * pair::kTileM, w / p.dh_mt * pair::kTileN, 0,
+                left < p.dh_part_kb ? left : p.dh_part_kb, kb0, kDh + 2 * part};
+  }
+  static __device__ __forceinline__ bool a_mn(const Tile& t) { return t.kind == kDw; }
+  static __device__ __forceinline__ bool b_mn(const Tile&) { return true; }
+  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile& t) {
+    return t.kind == kDw ? &p.dl_mn : &p.dl_k;
+  }
+  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile& t) {
+    return t.kind == kDw ? &p.h : &p.w;
   }
   static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, EpiContext& c) {
-    const float scale = grad_scale(p.scale);
+    const bool dw = t.kind == kDw;
+    const int rows = dw ? p.width : p.rows, part = t.kind >> 1;
+    if (c.row0 >= rows) return;  // warp-uniform
+    const int kind = dw ? p.dw_kind : p.dh_kind;
+    const CUtensorMap* out = dw ? &p.dw : &p.dh;
+    const float scale = dw || kind == kOut16 ? grad_scale(p.scale) : 1.0f;
     const int col0 = t.n0 + c.part * 128;
-    if (c.row0 >= p.rows) return;  // warp-uniform
 #pragma unroll 1
     for (int ch = 0; ch < 4; ++ch) {
       const int begin = col0 + ch * 32;
-      if (begin >= p.cols) break;  // warp-uniform
+      if (begin >= p.dim) break;  // warp-uniform
       float v[32];
       pair::load_acc(c.acc + c.part * 128 + ch * 32, v);
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] *= scale;
-      if (p.kind == kOut16) {
+      if (kind == kOut16) {
         // two 32-column steps share a 64-column line
         if ((ch & 1) == 0) pair::stage_reuse(c.lane);
         pair::stage_16(c.smem, c.lane, ch & 1, v, p.fp16);
-        if ((ch & 1) == 0 && begin + 32 < p.cols) continue;
+        if ((ch & 1) == 0 && begin + 32 < p.dim) continue;
         fence_proxy_async_smem();
         __syncwarp();
         if (c.lane == 0) {
-          pair::store_3d(&p.out, c.smem, begin & ~63, c.row0, 0);
+          pair::store_3d(out, c.smem, begin & ~63, c.row0, part);
           tma_store_commit();
         }
       } else {
@@ -348,8 +400,8 @@ struct GradOp {
         fence_proxy_async_smem();
         __syncwarp();
         if (c.lane == 0) {
-          if (p.kind == kOutF32Add) pair::reduce_add_3d(&p.out, c.smem, begin, c.row0, 0);
-          else pair::store_3d(&p.out, c.smem, begin, c.row0, 0);
+          if (kind == kOutF32Add) pair::reduce_add_3d(out, c.smem, begin, c.row0, part);
+          else pair::store_3d(out, c.smem, begin, c.row0, part);
           tma_store_commit();
         }
       }
@@ -357,17 +409,22 @@ struct GradOp {
   }
 };
 
-// dh in the operands' type from the fp32 sum over the pieces; rows of `dim` (a multiple of 8).
+// dh in the operands' type from its fp32 parts [parts][rows][dim], added in order.
 __global__ void __launch_bounds__(256)
-ce_dh_kernel(const float* __restrict__ sum, long vecs, int vecs_per_row, void* __restrict__ out,
-             long ld_out, GradScale g, int fp16) {
+ce_dh_kernel(const float* __restrict__ sums, int parts, long vecs, int vecs_per_row,
+             void* __restrict__ out, long ld_out, GradScale g, int fp16) {
   pdl_launch_dependents();
   pdl_wait();
   const float scale = grad_scale(g);
   for (long i = blockIdx.x * static_cast<long>(blockDim.x) + threadIdx.x; i < vecs;
        i += static_cast<long>(gridDim.x) * blockDim.x) {
-    const float4 a = reinterpret_cast<const float4*>(sum)[2 * i];
-    const float4 b = reinterpret_cast<const float4*>(sum)[2 * i + 1];
+    float4 a = make_float4(0, 0, 0, 0), b = a;
+    for (int k = 0; k < parts; ++k) {
+      const float4* src = reinterpret_cast<const float4*>(sums) + 2 * (k * vecs + i);
+      const float4 c = src[0], d = src[1];
+      a.x += c.x; a.y += c.y; a.z += c.z; a.w += c.w;
+      b.x += d.x; b.y += d.y; b.z += d.z; b.w += d.w;
+    }
     const long row = i / vecs_per_row;
     const long col = (i - row * vecs_per_row) * 8;
     uint4 q;
@@ -394,6 +451,49 @@ int band_of(int mt, int dim) {
   return band < 4 ? (mt < 4 ? mt : 4) : (band < mt ? band : mt);
 }
 
+// Steps of overhead that a tile adds to its reduction (filling the ring, draining the accumulator).
+constexpr int kTileOverheadKb = 4;
+
+// Parts of dh's reduction over `width` entries: as few as keep one of its tiles within the average
+// load of a pair, so that few rows do not leave most pairs idle (1024 x 512 x 10000 has 8 tiles of
+// 157 steps: 51 us in one part, 9 us in six).  Only a vocabulary walked in one piece is split.
+int dh_parts(int rows, int dim, int width, int pairs) {
+  const long tiles = static_cast<long>(tiles_of(rows, pair::kTileM)) * tiles_of(dim, pair::kTileN);
+  const long kb = tiles_of(width, pair::kBK);
+  const long dw = static_cast<long>(tiles_of(width, pair::kTileM)) * tiles_of(dim, pair::kTileN) *
+                  (tiles_of(rows, pair::kBK) + kTileOverheadKb);
+  const long average = (dw + tiles * (kb + kTileOverheadKb)) / pairs + 1;
+  long parts = (kb + average - 1) / average;
+  if (parts > 16) parts = 16;
+  // every part has work
+  const long part_kb = (kb + parts - 1) / parts;
+  return static_cast<int>((kb + part_kb - 1) / part_kb);
+}
+
+// Deals dh's tiles, then dw's, each to the cluster with the least work so far; every cluster's
+// tiles of a kind are consecutive.
+void deal(GradOp::Params& p, int dh_tiles, int dw_tiles, int clusters) {
+  int dh_count[kMaxClusters] = {}, dw_count[kMaxClusters] = {};
+  using Load = std::pair<long, int>;  // work so far, cluster
+  Load heap[kMaxClusters];            // the least loaded cluster on top
+  for (int c = 0; c < clusters; ++c) heap[c] = Load(0, c);
+  auto give = [&](int tiles, int kb, int* count) {
+    for (int k = 0; k < tiles; ++k) {
+      std::pop_heap(heap, heap + clusters, std::greater<Load>());
+      heap[clusters - 1].first += kb + kTileOverheadKb;
+      ++count[heap[clusters - 1].second];
+      std::push_heap(heap, heap + clusters, std::greater<Load>());
+    }
+  };
+  give(dh_tiles, p.dh_part_kb, dh_count);
+  give(dw_tiles, p.dw_kb, dw_count);
+  p.dh_begin[0] = p.dw_begin[0] = 0;
+  for (int c = 0; c < kMaxClusters; ++c) {
+    p.dh_begin[c + 1] = p.dh_begin[c] + (c < clusters ? dh_count[c] : 0);
+    p.dw_begin[c + 1] = p.dw_begin[c] + (c < clusters ? dw_count[c] : 0);
+  }
+}
+
 int check(const SflLinearCe* a) {
   if (a == nullptr || a->rows < 1 || a->dim < 8 || a->dim % 8 != 0 || a->vocab < 1) return -2;
   if (!aligned16(a->hidden, a->ld_hidden, 2) || !aligned16(a->weight, a->ld_weight, 2)) return -2;
@@ -407,6 +507,15 @@ int check(const SflLinearCe* a) {
 
 }  // namespace
 }  // namespace sfl
+
+// Sizes of this file's and rotary.cu's argument records, for bindings to compare with.
+extern "C" int sfl_operator_struct_sizes(int* sizes, int capacity) {
+  const int all[] = {sizeof(SflRotaryTensor), sizeof(SflRotaryTable), sizeof(SflLinearCe),
+                     sizeof(SflLinearCeGrad)};
+  const int count = static_cast<int>(sizeof(all) / sizeof(all[0]));
+  for (int i = 0; i < count && i < capacity; ++i) sizes[i] = all[i];
+  return count;
+}
 
 extern "C" long sfl_linear_ce_part_bytes(int rows, int vocab) {
   using namespace sfl;
@@ -436,7 +545,7 @@ extern "C" int sfl_linear_ce_fwd(const SflLinearCe* a, void* part, long part_byt
   p.grid.band = band_of(p.grid.mt, a->dim);
   p.total = p.grid.mt * p.grid.nt;
   p.num_kb = tiles_of(a->dim, pair::kBK);
-  p.idesc = pair::instruction_descriptor(a->fp16, false, false);
+  p.fp16 = a->fp16 != 0;
   p.status = a->status;
   p.targets = a->targets;
   p.part = static_cast<float2*>(part);
@@ -455,6 +564,15 @@ extern "C" int sfl_linear_ce_fwd(const SflLinearCe* a, void* part, long part_byt
                     totals, loss);
 }
 
+extern "C" long sfl_linear_ce_dh_sum_bytes(int rows, int dim, int vocab, int piece) {
+  using namespace sfl;
+  if (rows < 1 || dim < 1 || vocab < 1 || piece < 1) return -1;
+  const int pairs = pair::pairs_here();
+  if (pairs < 1) return -1;
+  const int parts = piece < vocab ? 1 : dh_parts(rows, dim, vocab, pairs);
+  return piece < vocab || parts > 1 ? 4L * parts * rows * dim : 0;
+}
+
 extern "C" int sfl_linear_ce_bwd(const SflLinearCe* a, const SflLinearCeGrad* g, void* stream_) {
   using namespace sfl;
   const int bad = check(a);
@@ -467,7 +585,14 @@ extern "C" int sfl_linear_ce_bwd(const SflLinearCe* a, const SflLinearCeGrad* g,
       !aligned16(g->dw, g->ld_dw, dw_elem) || g->ld_dh < a->dim || g->ld_dw < a->dim)
     return -2;
   const int pieces = tiles_of(a->vocab, g->piece);
-  if (pieces > 1 && !aligned16(g->dh_sum, a->dim, 4)) return -2;
+  if (pieces > 1 && g->dh_sum == nullptr) return -2;
+  const int pairs = pair::pairs_here();
+  if (pairs < 1 || pairs > kMaxClusters) return -1;
+  const int parts = pieces > 1 ? 1 : dh_parts(a->rows, a->dim, a->vocab, pairs);
+  const bool summed = pieces > 1 || parts > 1;  // dh is the sum of fp32 parts
+  if (summed && (!aligned16(g->dh_sum, a->dim, 4) ||
+                 g->dh_sum_bytes < 4L * parts * a->rows * a->dim))
+    return -2;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const uint64_t rows = a->rows, dim = a->dim;
   const float factor = a->fp16 ? 1.0f / (1 << kFp16Shift) : 1.0f;
@@ -492,7 +617,7 @@ extern "C" int sfl_linear_ce_bwd(const SflLinearCe* a, const SflLinearCeGrad* g,
     d.grid.band = band_of(d.grid.mt, a->dim);
     d.total = d.grid.mt * d.grid.nt;
     d.num_kb = tiles_of(dim, pair::kBK);
-    d.idesc = pair::instruction_descriptor(a->fp16, false, false);
+    d.fp16 = a->fp16 != 0;
     d.status = a->status;
     d.targets = a->targets;
     d.lse2 = a->lse2;
@@ -500,62 +625,52 @@ extern "C" int sfl_linear_ce_bwd(const SflLinearCe* a, const SflLinearCeGrad* g,
     d.rows = a->rows;
     d.vocab_begin = static_cast<int>(begin);
     d.width = width;
-    d.fp16 = a->fp16;
     rc = pair::launch_pair<DlogitsOp>(d, stream);
     if (rc != 0) return rc;
 
-    GradOp<true>::Params q{};
-    rc = pair::map_operand(&q.a, g->dlogits, true, width, rows, g->piece, 1, dl_size);
+    GradOp::Params q{};
+    rc = pair::map_operand(&q.dl_mn, g->dlogits, true, width, rows, g->piece, 1, dl_size);
     if (rc == 0)
-      rc = pair::map_operand(&q.b, a->hidden, true, dim, rows, a->ld_hidden, 1,
+      rc = pair::map_operand(&q.dl_k, g->dlogits, false, rows, width, g->piece, 1, dl_size);
+    if (rc == 0)
+      rc = pair::map_operand(&q.h, a->hidden, true, dim, rows, a->ld_hidden, 1,
                              rows * a->ld_hidden);
     if (rc == 0)
-      rc = pair::map_3d(&q.out, static_cast<uint8_t*>(g->dw) + begin * g->ld_dw * dw_elem, dw_elem,
+      rc = pair::map_operand(&q.w, w, true, dim, width, a->ld_weight, 1,
+                             static_cast<uint64_t>(width) * a->ld_weight);
+    if (rc == 0)
+      rc = pair::map_3d(&q.dw, static_cast<uint8_t*>(g->dw) + begin * g->ld_dw * dw_elem, dw_elem,
                         dim, width, g->ld_dw, 1, static_cast<uint64_t>(width) * g->ld_dw,
                         128 / dw_elem, 32);
+    if (rc == 0 && summed)
+      rc = pair::map_3d(&q.dh, g->dh_sum, 4, dim, rows, dim, parts, rows * dim, 32, 32);
+    else if (rc == 0)
+      rc = pair::map_3d(&q.dh, g->dh, 2, dim, rows, g->ld_dh, 1, rows * g->ld_dh, 64, 32);
     if (rc != 0) return 1000 + rc;
-    q.grid = Grid{tiles_of(width, pair::kTileM), tiles_of(dim, pair::kTileN), 0};
-    q.grid.band = q.grid.mt;
-    q.total = q.grid.mt * q.grid.nt;
-    q.num_kb = tiles_of(rows, pair::kBK);
-    q.idesc = pair::instruction_descriptor(a->fp16, true, true);
+    q.fp16 = a->fp16 != 0;
     q.status = a->status;
     q.scale = scale;
-    q.rows = width;
-    q.cols = a->dim;
-    q.kind = g->dw_kind;
-    q.fp16 = a->fp16;
-    rc = pair::launch_pair<GradOp<true>>(q, stream);
-    if (rc != 0) return rc;
-
-    GradOp<false>::Params h{};
-    rc = pair::map_operand(&h.a, g->dlogits, false, rows, width, g->piece, 1, dl_size);
-    if (rc == 0)
-      rc = pair::map_operand(&h.b, w, true, dim, width, a->ld_weight, 1,
-                             static_cast<uint64_t>(width) * a->ld_weight);
-    if (rc == 0 && pieces == 1)
-      rc = pair::map_3d(&h.out, g->dh, 2, dim, rows, g->ld_dh, 1, rows * g->ld_dh, 64, 32);
-    else if (rc == 0)
-      rc = pair::map_3d(&h.out, g->dh_sum, 4, dim, rows, dim, 1, rows * dim, 32, 32);
-    if (rc != 0) return 1000 + rc;
-    h.grid = Grid{tiles_of(rows, pair::kTileM), tiles_of(dim, pair::kTileN), 0};
-    h.grid.band = h.grid.mt;
-    h.total = h.grid.mt * h.grid.nt;
-    h.num_kb = tiles_of(width, pair::kBK);
-    h.idesc = pair::instruction_descriptor(a->fp16, false, true);
-    h.status = a->status;
-    h.scale = pieces == 1 ? scale : GradScale{nullptr, nullptr, 1.0f};
-    h.rows = a->rows;
-    h.cols = a->dim;
-    h.kind = pieces == 1 ? kOut16 : (i == 0 ? kOutF32 : kOutF32Add);
-    h.fp16 = a->fp16;
-    rc = pair::launch_pair<GradOp<false>>(h, stream);
+    q.dw_mt = tiles_of(width, pair::kTileM);
+    q.dh_mt = tiles_of(rows, pair::kTileM);
+    q.dh_nt = tiles_of(dim, pair::kTileN);
+    q.dw_kb = tiles_of(rows, pair::kBK);
+    q.dh_kb = tiles_of(width, pair::kBK);
+    q.dh_part_kb = tiles_of(q.dh_kb, parts);
+    q.dh_tiles = q.dh_mt * q.dh_nt * parts;
+    q.total = q.dh_tiles + q.dw_mt * q.dh_nt;
+    q.rows = a->rows;
+    q.width = width;
+    q.dim = a->dim;
+    q.dw_kind = g->dw_kind;
+    q.dh_kind = !summed ? kOut16 : (i == 0 ? kOutF32 : kOutF32Add);
+    deal(q, q.dh_tiles, q.dw_mt * q.dh_nt, q.total < pairs ? q.total : pairs);
+    rc = pair::launch_pair<GradOp>(q, stream);
     if (rc != 0) return rc;
   }
-  if (pieces == 1) return 0;
+  if (!summed) return 0;
   const long vecs = static_cast<long>(a->rows) * a->dim / 8;
   const long blocks = (vecs + 255) / 256;
   return launch_pdl(ce_dh_kernel, dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)),
-                    dim3(256), 0, stream, static_cast<const float*>(g->dh_sum), vecs, a->dim / 8,
+                    dim3(256), 0, stream, static_cast<const float*>(g->dh_sum), parts, vecs, a->dim / 8,
                     g->dh, g->ld_dh, scale, a->fp16);
 }

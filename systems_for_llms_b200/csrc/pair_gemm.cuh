@@ -18,11 +18,13 @@
 // then leave through the common exit (copies in flight are waited for, tensor memory is freed).
 //
 // Op supplies the tile order, the tensor maps and the epilogue:
-//   struct Op::Params { ...; int total; uint32_t idesc; int* status; }
-//   static constexpr bool kAMN, kBMN;                MN-major operands (see gemm.cu)
-//   static Tile  Op::tile(p, w)                      the w-th tile
-//   static const CUtensorMap* Op::map_a(p), map_b(p) rank-3 maps {inner, rows, batch}
-//   static void  Op::epilogue(p, tile, EpiContext&)  one warp's share of the tile
+//   struct Op::Params { ...; int total; bool fp16; int* status; }
+//   static int  Op::first(p, cluster), Op::next(p, w, cluster, clusters)
+//                                  the cluster's first tile and the one after w (>= total: none)
+//   static Tile Op::tile(p, w)     where the tile lies
+//   static bool Op::a_mn(t), Op::b_mn(t)  MN-major operands (see gemm.cu)
+//   static const CUtensorMap* Op::map_a(p, t), Op::map_b(p, t)   rank-3 {inner, rows, batch}
+//   static void Op::epilogue(p, t, EpiContext&)  one warp's share of the tile
 #pragma once
 #include <cuda_fp16.h>
 
@@ -51,6 +53,8 @@ static_assert(kSmemBytes <= 232448, "more than a CTA's shared memory");
 struct Tile {
   int m0, n0, z;  // first row, first column, batch index
   int num_kb;     // 64-deep steps
+  int kb0;        // first step of the reduction
+  int kind;       // for Ops that mix products
 };
 
 struct __align__(8) Barriers {
@@ -162,11 +166,21 @@ __device__ __forceinline__ bool wait_or_leave(uint64_t* bar, uint32_t parity, vo
 }
 
 // Instruction descriptor of the pair's 256 x 256 x 16 product; both operands have one type.
-inline uint32_t instruction_descriptor(bool fp16, bool a_mn, bool b_mn) {
-  uint32_t d = umma_idesc_bf16(kTileM, kTileN, a_mn, b_mn);
-  if (fp16) d &= ~((1u << 7) | (1u << 10));  // operand format 0: fp16
-  return d;
+__device__ __forceinline__ uint32_t instruction_descriptor(bool fp16, bool a_mn, bool b_mn) {
+  const uint32_t d = umma_idesc_bf16(kTileM, kTileN, a_mn, b_mn);
+  return fp16 ? d & ~((1u << 7) | (1u << 10)) : d;  // operand format 0: fp16
 }
+
+// Tiles dealt round robin.
+struct RoundRobin {
+  template <class P> static __device__ __forceinline__ int first(const P&, int cluster) {
+    return cluster;
+  }
+  template <class P>
+  static __device__ __forceinline__ int next(const P&, int w, int, int clusters) {
+    return w + clusters;
+  }
+};
 
 // ------------------------------------------------------- epilogue helpers ----
 // A staging tile is 32 rows of 128 bytes in the 128-byte swizzle of its tensor map.
@@ -226,7 +240,7 @@ pair_kernel(const __grid_constant__ typename Op::Params p) {
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int clusters = gridDim.x >> 1;
-  const int first = blockIdx.x >> 1;
+  const int cluster = blockIdx.x >> 1;
   volatile int* abort = &bars->abort;
 
   if (threadIdx.x == 0) {
@@ -241,8 +255,6 @@ pair_kernel(const __grid_constant__ typename Op::Params p) {
     for (int s = 0; s < kEpiWarps; ++s) mbar_init(&bars->aux_full[s], 1);
     bars->abort = 0;
     mbar_fence_init();
-    prefetch_tensormap(Op::map_a(p));
-    prefetch_tensormap(Op::map_b(p));
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
@@ -262,13 +274,13 @@ pair_kernel(const __grid_constant__ typename Op::Params p) {
   if (warp == 0) {
     // ------------------------------------------------------ TMA producer ----
     if (lane == 0) {
-      const CUtensorMap* ma = Op::map_a(p);
-      const CUtensorMap* mb = Op::map_b(p);
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int w = first; w < p.total && ok; w += clusters) {
+      for (int w = Op::first(p, cluster); w < p.total && ok; w = Op::next(p, w, cluster, clusters)) {
         const Tile t = Op::tile(p, w);
+        const CUtensorMap* ma = Op::map_a(p, t);
+        const CUtensorMap* mb = Op::map_b(p, t);
         const int m0 = t.m0 + rank * kCtaM;
         const int n0 = t.n0 + rank * kHalfN;
         for (int kb = 0; kb < t.num_kb; ++kb) {
@@ -282,14 +294,14 @@ pair_kernel(const __grid_constant__ typename Op::Params p) {
           uint8_t* sb = sa + kABytes;
           const uint32_t bar = in_leader(smem_u32(&bars->full[stage]));
           if (rank == 0) mbar_expect_tx(&bars->full[stage], 2 * kStageBytes);
-          const int k0 = kb * kBK;
-          if constexpr (Op::kAMN) {
+          const int k0 = (t.kb0 + kb) * kBK;
+          if (Op::a_mn(t)) {
             load_3d(sa, ma, bar, m0, k0, t.z);
             load_3d(sa + kBK * 128, ma, bar, m0 + 64, k0, t.z);
           } else {
             load_3d(sa, ma, bar, k0, m0, t.z);
           }
-          if constexpr (Op::kBMN) {
+          if (Op::b_mn(t)) {
             load_3d(sb, mb, bar, n0, k0, t.z);
             load_3d(sb + kBK * 128, mb, bar, n0 + 64, k0, t.z);
           } else {
@@ -316,16 +328,18 @@ pair_kernel(const __grid_constant__ typename Op::Params p) {
     // The leader's warp walks converged; one elected lane issues (see gemm.cu).
     if (rank == 0) {
       const uint32_t base = smem_u32(smem);
-      const uint64_t a0 = Op::kAMN ? umma_smem_desc(base, kBK * 128, 1024)
-                                   : umma_smem_desc(base, 16, 1024);
-      const uint64_t b0 = Op::kBMN ? umma_smem_desc(base + kABytes, kBK * 128, 1024)
-                                   : umma_smem_desc(base + kABytes, 16, 1024);
-      const uint32_t idesc = p.idesc;
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int w = first; w < p.total && ok; w += clusters) {
-        const int num_kb = Op::tile(p, w).num_kb;
+      for (int w = Op::first(p, cluster); w < p.total && ok; w = Op::next(p, w, cluster, clusters)) {
+        const Tile t = Op::tile(p, w);
+        const bool a_mn = Op::a_mn(t), b_mn = Op::b_mn(t);
+        const uint64_t a0 = a_mn ? umma_smem_desc(base, kBK * 128, 1024)
+                                 : umma_smem_desc(base, 16, 1024);
+        const uint64_t b0 = b_mn ? umma_smem_desc(base + kABytes, kBK * 128, 1024)
+                                 : umma_smem_desc(base + kABytes, 16, 1024);
+        const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
+        const uint32_t idesc = instruction_descriptor(p.fp16, a_mn, b_mn);
         if (!wait_or_leave(&bars->acc_empty[acc], acc_phase ^ 1, abort)) {
           report_status(p.status, kStatusTimeoutTmemEmpty);
           *abort = 1;
@@ -333,7 +347,7 @@ pair_kernel(const __grid_constant__ typename Op::Params p) {
         }
         tc_fence_after();
         const uint32_t d = tmem_base + acc * kTileN;
-        for (int kb = 0; kb < num_kb; ++kb) {
+        for (int kb = 0; kb < t.num_kb; ++kb) {
           if (!wait_or_leave(&bars->full[stage], phase, abort)) {
             report_status(p.status, kStatusTimeoutFull);
             *abort = 1;
@@ -346,10 +360,10 @@ pair_kernel(const __grid_constant__ typename Op::Params p) {
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < kBK / 16; ++k)
-              mma_pair(d, umma_desc_advance(a, k * (Op::kAMN ? 2048 : 32)),
-                       umma_desc_advance(b, k * (Op::kBMN ? 2048 : 32)), idesc, (kb | k) != 0);
+              mma_pair(d, umma_desc_advance(a, k * a_step), umma_desc_advance(b, k * b_step), idesc,
+                       (kb | k) != 0);
             commit_pair(&bars->empty[stage]);
-            if (kb == num_kb - 1) commit_pair(&bars->acc_full[acc]);
+            if (kb == t.num_kb - 1) commit_pair(&bars->acc_full[acc]);
           }
           __syncwarp();
           if (++stage == kStages) {
@@ -377,7 +391,7 @@ pair_kernel(const __grid_constant__ typename Op::Params p) {
     c.status = p.status;
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int w = first; w < p.total; w += clusters) {
+    for (int w = Op::first(p, cluster); w < p.total; w = Op::next(p, w, cluster, clusters)) {
       const Tile t = Op::tile(p, w);
       if (!wait_or_leave(&bars->acc_full[acc], acc_phase, abort)) {
         report_status(p.status, kStatusTimeoutTmemFull);
@@ -435,6 +449,8 @@ inline int sm_count_here(int* device_out = nullptr) {
   if (device_out != nullptr) *device_out = device;
   return count;
 }
+
+inline int pairs_here() { return sm_count_here() / 2; }
 
 template <class Op>
 int launch_pair(const typename Op::Params& p, cudaStream_t stream) {

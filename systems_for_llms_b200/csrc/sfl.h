@@ -123,18 +123,20 @@ int sfl_linear_ce_fwd(const SflLinearCe* a, void* part, long part_bytes, float* 
 /* dh 16-bit [rows, dim] and dw [vocab, dim] (dw_kind 0: 16-bit, 1: fp32, 2: added to fp32), both
  * times the device scalar grad (NULL: 1) and over totals[1] (NULL: not).  The vocabulary is walked
  * in pieces of `piece` entries (a multiple of 256): dlogits is 16-bit [rows, piece] scratch, dh_sum
- * fp32 [rows, dim] scratch (NULL allowed when one piece is enough). */
+ * scratch of sfl_linear_ce_dh_sum_bytes (which may be none; asks for the current device). */
 typedef struct SflLinearCeGrad {
   const float* grad;
   const float* totals;
   void* dlogits;
   float* dh_sum;
+  long dh_sum_bytes;
   void* dh;
   long ld_dh;
   void* dw;
   long ld_dw;
   int dw_kind, piece;
 } SflLinearCeGrad;
+long sfl_linear_ce_dh_sum_bytes(int rows, int dim, int vocab, int piece);
 int sfl_linear_ce_bwd(const SflLinearCe* a, const SflLinearCeGrad* g, void* stream);
 
 /* ------------------------------------------------------------- optimizer -- */
@@ -416,6 +418,8 @@ const char* sfl_version(void);
  * sizeof(SflAttnMask), sizeof(SflComm), sizeof(SflBlockArgs), sizeof(SflTpFuse) and returns how many
  * there are; bindings compare them with their own mirrors. */
 int sfl_struct_sizes(int* sizes, int capacity);
+/* The same for SflRotaryTensor, SflRotaryTable, SflLinearCe, SflLinearCeGrad. */
+int sfl_operator_struct_sizes(int* sizes, int capacity);
 
 /* ------------------------------------------------------ transformer block -- */
 /* One pre-norm block (RMSNorm -> fused QKV + RoPE -> causal attention -> output

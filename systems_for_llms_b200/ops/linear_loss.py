@@ -44,13 +44,14 @@ class LinearCeGrad(Structure):
     """Mirror of ``SflLinearCeGrad`` in csrc/sfl.h."""
 
     _fields_ = [("grad", c_void_p), ("totals", c_void_p), ("dlogits", c_void_p),
-                ("dh_sum", c_void_p), ("dh", c_void_p), ("ld_dh", c_long), ("dw", c_void_p),
+                ("dh_sum", c_void_p), ("dh_sum_bytes", c_long), ("dh", c_void_p), ("ld_dh", c_long), ("dw", c_void_p),
                 ("ld_dw", c_long), ("dw_kind", c_int), ("piece", c_int)]
 
 
 _P = c_void_p
 _lib.register_signature("sfl_linear_ce_part_bytes", [c_int, c_int])
 _lib.register_signature("sfl_linear_ce_fwd", [POINTER(LinearCe), _P, c_long, _P, c_int, _P, _P, _P])
+_lib.register_signature("sfl_linear_ce_dh_sum_bytes", [c_int, c_int, c_int, c_int])
 _lib.register_signature("sfl_linear_ce_bwd", [POINTER(LinearCe), POINTER(LinearCeGrad), _P])
 
 
@@ -135,13 +136,16 @@ def linear_ce_backward(hidden, weight, targets, ignore_index: int, lse2, grad, t
         piece = piece_size(rows, vocab)
     dlogits = torch.empty(rows, piece, dtype=hidden.dtype, device=dev)
     dh = torch.empty(rows, dim, dtype=hidden.dtype, device=dev)
-    dh_sum = torch.empty(rows, dim, dtype=torch.float32, device=dev) if piece < vocab else None
     args = _args(hidden, weight, targets, ignore_index, lse2)
-    grads = LinearCeGrad(grad=_lib.ptr(grad), totals=_lib.ptr(totals), dlogits=dlogits.data_ptr(),
-                         dh_sum=_lib.ptr(dh_sum), dh=dh.data_ptr(), ld_dh=dim, dw=dw.data_ptr(),
-                         ld_dw=dw.stride(0), dw_kind=kind, piece=piece)
+    handle = _lib.lib()
     with _lib.on_device(dev):
-        code = _lib.lib().sfl_linear_ce_bwd(byref(args), byref(grads), _lib.stream_ptr())
+        size = handle.sfl_linear_ce_dh_sum_bytes(rows, dim, vocab, piece)
+        dh_sum = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
+        grads = LinearCeGrad(grad=_lib.ptr(grad), totals=_lib.ptr(totals),
+                             dlogits=dlogits.data_ptr(), dh_sum=_lib.ptr(dh_sum), dh_sum_bytes=size,
+                             dh=dh.data_ptr(), ld_dh=dim, dw=dw.data_ptr(), ld_dw=dw.stride(0),
+                             dw_kind=kind, piece=piece)
+        code = handle.sfl_linear_ce_bwd(byref(args), byref(grads), _lib.stream_ptr())
     _lib.check(code, "sfl_linear_ce_bwd")
     return dh
 

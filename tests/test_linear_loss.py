@@ -71,3 +71,19 @@ def test_entry_points_refuse_before_launching():
     small = dict(good, vocab=300)                                   # two pieces, no place for their sum
     assert handle.sfl_linear_ce_bwd(ctypes.byref(LinearCe(**small)),
                                     ctypes.byref(LinearCeGrad(**spec)), None) == -2
+
+
+def test_records_match_the_compiled_library():
+    from systems_for_llms_b200.ops import build as builder
+    from systems_for_llms_b200.ops import lib
+    from systems_for_llms_b200.ops.rotary import RotaryTable, RotaryTensor
+    try:
+        builder.build()
+        call = lib.lib()._handle.sfl_operator_struct_sizes
+    except Exception as error:
+        pytest.skip(f"kernel library unavailable: {error}")
+    call.argtypes, call.restype = [ctypes.POINTER(ctypes.c_int), ctypes.c_int], ctypes.c_int
+    sizes = (ctypes.c_int * 8)()
+    mirrors = [RotaryTensor, RotaryTable, LinearCe, LinearCeGrad]
+    assert call(sizes, 8) == len(mirrors)
+    assert [ctypes.sizeof(m) for m in mirrors] == list(sizes)[:len(mirrors)]
