@@ -63,7 +63,7 @@ __device__ __forceinline__ void grid_tile(const Grid& g, int w, int* m, int* n) 
 }
 
 // ---------------------------------------------------- row statistics (forward) ----
-struct StatsOp : pair::RoundRobin {
+struct StatsOp : pair::Plain, pair::RoundRobin {
   struct Params {
     CUtensorMap a, b;
     Grid grid;
@@ -230,7 +230,7 @@ ce_total_kernel(const float* __restrict__ row_loss, const int64_t* __restrict__ 
 }
 
 // --------------------------------------------- dl of a piece of the vocabulary ----
-struct DlogitsOp : pair::RoundRobin {
+struct DlogitsOp : pair::Plain, pair::RoundRobin {
   struct Params {
     CUtensorMap a, b, out;
     Grid grid;
@@ -321,7 +321,7 @@ __device__ __forceinline__ float grad_scale(const GradScale& g) {
 constexpr int kMaxClusters = 96;
 enum Product : int { kDw = 0, kDh = 1 };
 
-struct GradOp {
+struct GradOp : pair::Plain {
   struct Params {
     CUtensorMap dl_mn, dl_k, h, w, dw, dh;
     int total, dh_tiles;         // dh's tiles are the first of each cluster's range
@@ -508,10 +508,10 @@ int check(const SflLinearCe* a) {
 }  // namespace
 }  // namespace sfl
 
-// Sizes of this file's and rotary.cu's argument records, for bindings to compare with.
+// Sizes of the argument records of rotary.cu, this file and newton_schulz.cu, for bindings to compare with.
 extern "C" int sfl_operator_struct_sizes(int* sizes, int capacity) {
   const int all[] = {sizeof(SflRotaryTensor), sizeof(SflRotaryTable), sizeof(SflLinearCe),
-                     sizeof(SflLinearCeGrad)};
+                     sizeof(SflLinearCeGrad), sizeof(SflNewtonSchulz)};
   const int count = static_cast<int>(sizeof(all) / sizeof(all[0]));
   for (int i = 0; i < count && i < capacity; ++i) sizes[i] = all[i];
   return count;

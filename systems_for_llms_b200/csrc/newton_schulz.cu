@@ -1,0 +1,538 @@
+// Orthogonalised updates: Newton-Schulz products over a stack of matrices.
+//
+//   X = U / (|U|_F + eps);   repeat:  G = X X^T,  X <- a X + (b G + c G G) X
+//
+// (the Gram matrix of the shorter side: X^T X on the right for tall matrices, so nothing is
+// transposed).  Singular vectors stay, singular values go through the odd quintic
+// a s + b s^3 + c s^5 each time.  The reference trains with AdamW only (src/llmlab/train.py:169);
+// the operator serves optim.FusedMuon.
+//
+// All products run on CTA-pair tensor-core tiles (pair_gemm.cuh), one launch per product for the
+// whole stack.  The two Gram-sized products are symmetric: only tiles on and above the diagonal
+// are computed, their epilogue also writes the mirrored tile.
+//
+// Precision.  The quintic multiplies small singular values by 3.4 a step, and with them whatever
+// was rounded away: five steps in bf16 are off by 1 to 5 percent.  Operands are therefore fp16,
+// times 2^12: entries of X, G and b G + c G G are at most 1.2, 1.5 and 2.8 (X's singular values
+// never exceed 1.2), far below 65504 / 4096, and their small entries stay normal numbers down to
+// 2^-26.  X itself is carried as hi + lo, two fp16 numbers with 22 bits between them, of which hi
+// is what the tensor cores multiply: a X is then exact to fp32 and the rounding of hi does not
+// compound.  In the last two steps most singular values are near 1, where a X and P X nearly
+// cancel; there P + k I and (a - k) X are used, with k = -0.75 (b + c), three quarters of -P at 1:
+// the same sum with smaller terms to round.  Sums are fp32, the norm is accumulated in 64 bits.
+// Measured against 64 bits: 1.8e-3 to 2.3e-3 of the result's norm, of which its rounding to bf16 is
+// 1.7e-3 (without k up to 2.7e-3, with hi alone up to 7e-3).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "pair_gemm.cuh"
+#include "sfl.h"
+
+namespace sfl {
+namespace {
+
+using pair::EpiContext;
+using pair::Tile;
+
+constexpr float kScale = 4096.0f;
+
+// ------------------------------------------------------------- norm and split ----
+struct Stack {
+  const void* base;
+  long stride0, stride1, row;  // matrix z starts at (z / inner) * stride0 + (z % inner) * stride1
+  int inner;
+};
+template <typename T>
+__device__ __forceinline__ const T* matrix(const Stack& s, int z) {
+  return static_cast<const T*>(s.base) + (z / s.inner) * s.stride0 + (z % s.inner) * s.stride1;
+}
+__device__ __forceinline__ float wide(float v) { return v; }
+__device__ __forceinline__ float wide(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float wide(__half v) { return __half2float(v); }
+
+constexpr int kChunks = 64;       // blocks per matrix, and partial sums of its norm
+constexpr int kNormThreads = 256;
+
+// Four elements of a row from column c (a multiple of 4), zero beyond the row.
+template <typename T>
+__device__ __forceinline__ void load4(const T* row, int c, int n, bool vec, float (&v)[4]) {
+  if (vec && c + 4 <= n) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 q = *reinterpret_cast<const float4*>(row + c);
+      v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    } else {
+      const uint2 q = *reinterpret_cast<const uint2*>(row + c);
+      const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = wide(e[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = c + i < n ? wide(row[c + i]) : 0.f;
+  }
+}
+
+// Sum of squares of each block's share of a matrix.  64-bit sums: squares of fp32 entries neither
+// overflow nor vanish in them.
+template <typename T>
+__global__ void __launch_bounds__(kNormThreads)
+ns_norm_kernel(Stack s, int m, int n, int vec, double* __restrict__ partial) {
+  __shared__ double sums[kNormThreads / 32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const T* src = matrix<T>(s, blockIdx.y);
+  const int quads = (n + 3) >> 2;
+  const long total = static_cast<long>(m) * quads;
+  double sum = 0.0;
+  for (long i = blockIdx.x * static_cast<long>(kNormThreads) + threadIdx.x; i < total;
+       i += static_cast<long>(gridDim.x) * kNormThreads) {
+    const long r = i / quads;
+    float v[4];
+    load4(src + r * s.row, static_cast<int>(i - r * quads) * 4, n, vec, v);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum = fma(static_cast<double>(v[j]), static_cast<double>(v[j]), sum);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double all = 0.0;
+#pragma unroll
+    for (int k = 0; k < kNormThreads / 32; ++k) all += sums[k];
+    partial[static_cast<long>(blockIdx.y) * gridDim.x + blockIdx.x] = all;
+  }
+}
+
+// hi + lo = 2^12 U / (|U| + eps), rows padded to a pitch of ld (a multiple of 8) with zeros.
+template <typename T>
+__global__ void __launch_bounds__(kNormThreads)
+ns_split_kernel(Stack s, int m, int n, int ld, int vec, const double* __restrict__ partial,
+                float eps, __half* __restrict__ hi, __half* __restrict__ lo) {
+  __shared__ float inv_sh;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int z = blockIdx.y;
+  if (threadIdx.x == 0) {
+    double sum = 0.0;
+    for (unsigned k = 0; k < gridDim.x; ++k) sum += partial[static_cast<long>(z) * gridDim.x + k];
+    inv_sh = static_cast<float>(kScale / (sqrt(sum) + static_cast<double>(eps)));
+  }
+  __syncthreads();
+  const float inv = inv_sh;
+  const T* src = matrix<T>(s, z);
+  const int quads = ld >> 2;
+  const long total = static_cast<long>(m) * quads;
+  const long out0 = static_cast<long>(z) * m * ld;
+  for (long i = blockIdx.x * static_cast<long>(kNormThreads) + threadIdx.x; i < total;
+       i += static_cast<long>(gridDim.x) * kNormThreads) {
+    const long r = i / quads;
+    const int c = static_cast<int>(i - r * quads) * 4;
+    float v[4];
+    load4(src + r * s.row, c, n, vec, v);
+    __half h[4], l[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float x = v[j] * inv;
+      h[j] = __float2half_rn(x);
+      l[j] = __float2half_rn(x - __half2float(h[j]));
+    }
+    *reinterpret_cast<uint2*>(hi + out0 + r * ld + c) = *reinterpret_cast<const uint2*>(h);
+    *reinterpret_cast<uint2*>(lo + out0 + r * ld + c) = *reinterpret_cast<const uint2*>(l);
+  }
+}
+
+// ------------------------------------------------- symmetric products: G, b G + c G G ----
+// out = alpha aux + beta A B^T with A = B: tiles on and above the diagonal, mirrored.
+struct SymOp : pair::RoundRobin {
+  static constexpr int kEpiTiles = 2;
+  struct Params {
+    CUtensorMap a, b;
+    CUtensorMap aux, out;   // 64-column lines of 32 rows
+    CUtensorMap mirror;     // 32-column lines of 64 rows
+    int total, num_kb;
+    bool fp16;
+    int* status;
+    int nt, per;            // tiles along a side, tiles per matrix
+    int size;               // rows and columns of the result
+    int mn;                 // operands MN-major
+    int has_aux;
+    float alpha, beta;
+    float shift;            // added to the diagonal
+  };
+  static __device__ __forceinline__ Tile tile(const Params& p, int w) {
+    const int z = w / p.per;
+    int in = w - z * p.per, i = 0;
+    while (in >= p.nt - i) {  // row i of the upper triangle has nt - i tiles
+      in -= p.nt - i;
+      ++i;
+    }
+    return Tile{i * pair::kTileM, (i + in) * pair::kTileN, z, p.num_kb, 0, p.mn};
+  }
+  static __device__ __forceinline__ bool a_mn(const Tile& t) { return t.kind != 0; }
+  static __device__ __forceinline__ bool b_mn(const Tile& t) { return t.kind != 0; }
+  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile&) {
+    return &p.a;
+  }
+  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile&) {
+    return &p.b;
+  }
+  static __device__ __forceinline__ void load_aux(const Params& p, const Tile& t, EpiContext& c,
+                                                  int begin) {
+    if (c.lane == 0) {
+      tma_store_wait_read<0>();  // the tile's last store has read it
+      mbar_expect_tx(c.aux_bar, pair::kEpiTileBytes);
+      tma_load_3d(c.smem, &p.aux, c.aux_bar, begin, c.row0, t.z);
+    }
+  }
+  static __device__ __forceinline__ void begin(const Params& p, const Tile& t, EpiContext& c) {
+    const int col0 = t.n0 + c.part * 128;
+    if (p.has_aux && c.row0 < p.size && col0 < p.size) load_aux(p, t, c, col0);
+  }
+  static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, EpiContext& c) {
+    const int col0 = t.n0 + c.part * 128;
+    if (c.row0 >= p.size) return;  // warp-uniform
+    uint8_t* mirrored = c.smem + pair::kEpiTileBytes;
+    const bool both = t.m0 != t.n0;
+    // mirrored element (row j, column lane) of 64-byte lines in their swizzle
+    uint32_t at[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      at[k] = (((static_cast<uint32_t>(c.lane) >> 3) ^ k) << 4) + (c.lane & 7) * 2;
+#pragma unroll 1
+    for (int ch = 0; ch < 2; ++ch) {
+      const int begin = col0 + ch * 64;
+      if (begin >= p.size) break;  // warp-uniform
+      if (p.has_aux) pair::wait_aux(c);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[32];
+        pair::load_acc(c.acc + c.part * 128 + ch * 64 + h * 32, v);
+        if (p.has_aux) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint4 q = *reinterpret_cast<const uint4*>(
+                pair::tile_chunk(c.smem, c.lane, 4 * h + j));
+            const __half2* e = reinterpret_cast<const __half2*>(&q);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float2 f = __half22float2(e[k]);
+              v[8 * j + 2 * k] = fmaf(v[8 * j + 2 * k], p.beta, p.alpha * f.x);
+              v[8 * j + 2 * k + 1] = fmaf(v[8 * j + 2 * k + 1], p.beta, p.alpha * f.y);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] *= p.beta;
+        }
+        const int diagonal = c.row0 + c.lane - begin - h * 32;
+        if (p.shift != 0.f && __any_sync(0xffffffffu, diagonal >= 0 && diagonal < 32)) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (diagonal == j) v[j] += p.shift;
+        }
+        if (h == 0) pair::stage_reuse(c.lane);  // both tiles' last stores (or nothing, after a load)
+        pair::stage_16(c.smem, c.lane, h, v, true);
+        if (both) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            *reinterpret_cast<__half*>(mirrored + (h * 32 + j) * 64 + at[(j >> 1) & 3]) =
+                __float2half_rn(v[j]);
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (c.lane == 0) {
+        pair::store_3d(&p.out, c.smem, begin, c.row0, t.z);
+        if (both) pair::store_3d(&p.mirror, mirrored, c.row0, begin, t.z);
+        tma_store_commit();
+      }
+      if (p.has_aux && ch == 0 && begin + 64 < p.size) load_aux(p, t, c, begin + 64);
+    }
+  }
+};
+
+// ------------------------------------------------------------ X <- a X + P X ----
+struct ApplyOp : pair::RoundRobin {
+  static constexpr int kEpiTiles = 2;
+  struct Params {
+    CUtensorMap a, b;
+    CUtensorMap hi, lo;        // X as it was: 64-column lines of 32 rows; lo is rewritten in place
+    CUtensorMap hi_out, out;   // the next hi, or the bf16 result
+    int total, num_kb;
+    bool fp16;
+    int* status;
+    int mt, per;
+    int m, n;
+    int wide;                  // A = P and B = X (MN-major), else A = X and B = P
+    int last;                  // 0: next X, 1: result through TMA, 2: result element by element
+    float alpha, beta;
+    __nv_bfloat16* result;     // [batch, m, n]
+  };
+  static __device__ __forceinline__ Tile tile(const Params& p, int w) {
+    const int z = w / p.per;
+    const int in = w - z * p.per;
+    return Tile{in % p.mt * pair::kTileM, in / p.mt * pair::kTileN, z, p.num_kb, 0, p.wide};
+  }
+  static __device__ __forceinline__ bool a_mn(const Tile&) { return false; }
+  static __device__ __forceinline__ bool b_mn(const Tile& t) { return t.kind != 0; }
+  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile&) {
+    return &p.a;
+  }
+  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile&) {
+    return &p.b;
+  }
+  static __device__ __forceinline__ void load_aux(const Params& p, const Tile& t, EpiContext& c,
+                                                  int begin) {
+    if (c.lane == 0) {
+      tma_store_wait_read<0>();
+      mbar_expect_tx(c.aux_bar, 2 * pair::kEpiTileBytes);
+      tma_load_3d(c.smem, &p.hi, c.aux_bar, begin, c.row0, t.z);
+      tma_load_3d(c.smem + pair::kEpiTileBytes, &p.lo, c.aux_bar, begin, c.row0, t.z);
+    }
+  }
+  static __device__ __forceinline__ void begin(const Params& p, const Tile& t, EpiContext& c) {
+    const int col0 = t.n0 + c.part * 128;
+    if (c.row0 < p.m && col0 < p.n) load_aux(p, t, c, col0);
+  }
+  static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, EpiContext& c) {
+    const int col0 = t.n0 + c.part * 128;
+    if (c.row0 >= p.m) return;  // warp-uniform
+    uint8_t* low = c.smem + pair::kEpiTileBytes;
+    const int row = c.row0 + c.lane;
+#pragma unroll 1
+    for (int ch = 0; ch < 2; ++ch) {
+      const int begin = col0 + ch * 64;
+      if (begin >= p.n) break;  // warp-uniform
+      pair::wait_aux(c);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[32];
+        pair::load_acc(c.acc + c.part * 128 + ch * 64 + h * 32, v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          // each lane rewrites exactly the bytes it read
+          uint4* qh = reinterpret_cast<uint4*>(pair::tile_chunk(c.smem, c.lane, 4 * h + j));
+          uint4* ql = reinterpret_cast<uint4*>(pair::tile_chunk(low, c.lane, 4 * h + j));
+          uint4 a = *qh, b = *ql;
+          __half2* eh = reinterpret_cast<__half2*>(&a);
+          __half2* el = reinterpret_cast<__half2*>(&b);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 fh = __half22float2(eh[k]), fl = __half22float2(el[k]);
+            const float x = fmaf(v[8 * j + 2 * k], p.beta, p.alpha * (fh.x + fl.x));
+            const float y = fmaf(v[8 * j + 2 * k + 1], p.beta, p.alpha * (fh.y + fl.y));
+            if (p.last == 0) {
+              eh[k] = __floats2half2_rn(x, y);
+              const float2 r = __half22float2(eh[k]);
+              el[k] = __floats2half2_rn(x - r.x, y - r.y);
+            } else {
+              const uint32_t packed = pack_bf16(x, y);
+              eh[k] = *reinterpret_cast<const __half2*>(&packed);
+            }
+          }
+          *qh = a;
+          if (p.last == 0) *ql = b;
+          if (p.last == 2 && row < p.m) {
+            const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&a);
+            const int col = begin + h * 32 + 8 * j;
+            __nv_bfloat16* dst = p.result + (static_cast<long>(t.z) * p.m + row) * p.n + col;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (col + k < p.n) dst[k] = e[k];
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (c.lane == 0 && p.last != 2) {
+        if (p.last == 0) {
+          pair::store_3d(&p.hi_out, c.smem, begin, c.row0, t.z);
+          pair::store_3d(&p.lo, low, begin, c.row0, t.z);
+        } else {
+          pair::store_3d(&p.out, c.smem, begin, c.row0, t.z);
+        }
+        tma_store_commit();
+      }
+      if (ch == 0 && begin + 64 < p.n) load_aux(p, t, c, begin + 64);
+    }
+  }
+};
+
+// ------------------------------------------------------------------- host ----
+long round_up(long v, long to) { return (v + to - 1) / to * to; }
+
+int tiles_of(long n, int size) { return static_cast<int>((n + size - 1) / size); }
+
+struct Sizes {
+  long ld, gram_ld, x_bytes, gram_bytes, norm_bytes, total;
+};
+
+Sizes sizes_of(int batch, int m, int n) {
+  Sizes s;
+  const long side = m < n ? m : n;
+  s.ld = round_up(n, 8);
+  s.gram_ld = round_up(side, 8);
+  s.x_bytes = round_up(2L * batch * m * s.ld, 256);
+  s.gram_bytes = round_up(2L * batch * side * s.gram_ld, 256);
+  s.norm_bytes = round_up(8L * batch * kChunks, 256);
+  s.total = 3 * s.x_bytes + 2 * s.gram_bytes + s.norm_bytes;  // two hi, lo, G, P, norms
+  return s;
+}
+
+template <typename T>
+int normalise(const Stack& s, int batch, int m, int n, int ld, float eps, double* partial,
+              __half* hi, __half* lo, cudaStream_t stream) {
+  const int size = sizeof(T);
+  const int bytes = 4 * size;  // four elements at a time
+  const int vec = (reinterpret_cast<uintptr_t>(s.base) % bytes) == 0 && (s.row * size) % bytes == 0 &&
+                  (s.stride0 * size) % bytes == 0 && (s.stride1 * size) % bytes == 0;
+  const long quads = static_cast<long>(m) * (ld / 4);
+  const long want = (quads + 4L * kNormThreads - 1) / (4L * kNormThreads);
+  const int chunks = static_cast<int>(want < 1 ? 1 : (want > kChunks ? kChunks : want));
+  int rc = launch_pdl(ns_norm_kernel<T>, dim3(chunks, batch), dim3(kNormThreads), 0, stream, s, m, n,
+                      vec, partial);
+  if (rc != 0) return rc;
+  return launch_pdl(ns_split_kernel<T>, dim3(chunks, batch), dim3(kNormThreads), 0, stream, s, m, n,
+                    ld, vec, static_cast<const double*>(partial), eps, hi, lo);
+}
+
+}  // namespace
+}  // namespace sfl
+
+extern "C" long sfl_newton_schulz_bytes(int batch, int m, int n) {
+  using namespace sfl;
+  if (batch < 1 || m < 1 || n < 1 || batch > 65535) return -1;
+  return sizes_of(batch, m, n).total;
+}
+
+extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {
+  using namespace sfl;
+  if (a == nullptr || a->batch < 1 || a->batch > 65535 || a->m < 1 || a->n < 1 || a->inner < 1 ||
+      a->steps < 1 || a->steps > 64 || a->dtype < 0 || a->dtype > 2 || a->update == nullptr ||
+      a->out == nullptr || a->work == nullptr || (reinterpret_cast<uintptr_t>(a->work) & 255))
+    return -2;
+  const int batch = a->batch, m = a->m, n = a->n;
+  const Sizes z = sizes_of(batch, m, n);
+  if (a->work_bytes < z.total) return -2;
+  const int side = m < n ? m : n, longer = m < n ? n : m;
+  const bool wide = m <= n;
+  const int mt = tiles_of(m, pair::kTileM), nt = tiles_of(n, pair::kTileN);
+  if (static_cast<long>(batch) * mt * nt > 0x7fffffffL) return -2;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+
+  uint8_t* at = static_cast<uint8_t*>(a->work);
+  __half* hi[2] = {reinterpret_cast<__half*>(at), reinterpret_cast<__half*>(at + z.x_bytes)};
+  __half* lo = reinterpret_cast<__half*>(at + 2 * z.x_bytes);
+  __half* gram = reinterpret_cast<__half*>(at + 3 * z.x_bytes);
+  __half* poly = reinterpret_cast<__half*>(at + 3 * z.x_bytes + z.gram_bytes);
+  double* norms = reinterpret_cast<double*>(at + 3 * z.x_bytes + 2 * z.gram_bytes);
+
+  const Stack s{a->update, a->stride0, a->stride1, a->row, a->inner};
+  int rc;
+  const int ld = static_cast<int>(z.ld);
+  if (a->dtype == 0) rc = normalise<__nv_bfloat16>(s, batch, m, n, ld, a->eps, norms, hi[0], lo, stream);
+  else if (a->dtype == 1) rc = normalise<__half>(s, batch, m, n, ld, a->eps, norms, hi[0], lo, stream);
+  else rc = normalise<float>(s, batch, m, n, ld, a->eps, norms, hi[0], lo, stream);
+  if (rc != 0) return rc;
+
+  const uint64_t x_stride = static_cast<uint64_t>(m) * z.ld;
+  const uint64_t g_stride = static_cast<uint64_t>(side) * z.gram_ld;
+  const int gt = tiles_of(side, pair::kTileN);
+
+  SymOp::Params q{};
+  q.fp16 = true;
+  q.status = a->status;
+  q.nt = gt;
+  q.per = gt * (gt + 1) / 2;
+  q.total = batch * q.per;
+  q.size = side;
+  ApplyOp::Params x{};
+  x.fp16 = true;
+  x.status = a->status;
+  x.mt = mt;
+  x.per = mt * nt;
+  x.total = batch * x.per;
+  x.num_kb = tiles_of(side, pair::kBK);
+  x.m = m;
+  x.n = n;
+  x.wide = wide;
+  x.result = static_cast<__nv_bfloat16*>(a->out);
+  const bool out_tma = (static_cast<long>(n) * 2) % 16 == 0 &&
+                       (reinterpret_cast<uintptr_t>(a->out) & 15) == 0;
+
+  auto gram_map = [&](CUtensorMap* map, __half* g) {
+    return pair::map_3d(map, g, 2, side, side, z.gram_ld, batch, g_stride, 64, 32);
+  };
+  auto mirror_map = [&](CUtensorMap* map, __half* g) {
+    const uint64_t dims[3] = {static_cast<uint64_t>(side), static_cast<uint64_t>(side),
+                              static_cast<uint64_t>(batch)};
+    const uint64_t strides[3] = {0, static_cast<uint64_t>(z.gram_ld) * 2, g_stride * 2};
+    const uint32_t box[3] = {32, 64, 1};
+    return make_tensormap_nd(map, g, 2, 3, dims, strides, box, 2);
+  };
+  auto x_map = [&](CUtensorMap* map, __half* v) {
+    return pair::map_3d(map, v, 2, n, m, z.ld, batch, x_stride, 64, 32);
+  };
+
+  for (int step = 0; step < a->steps; ++step) {
+    __half* now = hi[step & 1];
+    __half* next = hi[(step + 1) & 1];
+    // G = X X^T (wide: X is K-major) or X^T X (tall: X read MN-major)
+    q.mn = !wide;
+    q.num_kb = tiles_of(longer, pair::kBK);
+    q.has_aux = 0;
+    q.alpha = 0.f;
+    q.beta = 1.0f / kScale;
+    q.shift = 0.f;
+    rc = pair::map_operand(&q.a, now, !wide, side, longer, z.ld, batch, x_stride);
+    q.b = q.a;
+    if (rc == 0) rc = gram_map(&q.out, gram);
+    if (rc == 0) rc = mirror_map(&q.mirror, gram);
+    if (rc != 0) return 1000 + rc;
+    q.aux = q.out;
+    rc = pair::launch_pair<SymOp>(q, stream);
+    if (rc != 0) return rc;
+    // P = b G + c G G (+ k I)
+    const float k = step + 2 >= a->steps && a->b + a->c < 0.f ? -0.75f * (a->b + a->c) : 0.f;
+    q.shift = k * kScale;
+    q.mn = 0;
+    q.num_kb = tiles_of(side, pair::kBK);
+    q.has_aux = 1;
+    q.alpha = a->b;
+    q.beta = a->c / kScale;
+    q.aux = q.out;
+    rc = pair::map_operand(&q.a, gram, false, side, side, z.gram_ld, batch, g_stride);
+    q.b = q.a;
+    if (rc == 0) rc = gram_map(&q.out, poly);
+    if (rc == 0) rc = mirror_map(&q.mirror, poly);
+    if (rc != 0) return 1000 + rc;
+    rc = pair::launch_pair<SymOp>(q, stream);
+    if (rc != 0) return rc;
+    // X <- a X + P X (wide) or a X + X P (tall; P is symmetric)
+    const bool last = step + 1 == a->steps;
+    x.last = !last ? 0 : (out_tma ? 1 : 2);
+    const float unscale = last ? 1.0f / kScale : 1.0f;
+    x.alpha = (a->a - k) * unscale;
+    x.beta = unscale / kScale;
+    if (wide) {
+      rc = pair::map_operand(&x.a, poly, false, side, side, z.gram_ld, batch, g_stride);
+      if (rc == 0) rc = pair::map_operand(&x.b, now, true, n, m, z.ld, batch, x_stride);
+    } else {
+      rc = pair::map_operand(&x.a, now, false, m, n, z.ld, batch, x_stride);
+      if (rc == 0) rc = pair::map_operand(&x.b, poly, false, side, side, z.gram_ld, batch, g_stride);
+    }
+    if (rc == 0) rc = x_map(&x.hi, now);
+    if (rc == 0) rc = x_map(&x.lo, lo);
+    if (rc == 0) rc = x_map(&x.hi_out, next);
+    if (rc == 0 && x.last == 1)
+      rc = pair::map_3d(&x.out, a->out, 2, n, m, n, batch, static_cast<uint64_t>(m) * n, 64, 32);
+    if (rc != 0) return 1000 + rc;
+    rc = pair::launch_pair<ApplyOp>(x, stream);
+    if (rc != 0) return rc;
+  }
+  return 0;
+}

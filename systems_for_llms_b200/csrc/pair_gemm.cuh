@@ -24,6 +24,8 @@
 //   static Tile Op::tile(p, w)     where the tile lies
 //   static bool Op::a_mn(t), Op::b_mn(t)  MN-major operands (see gemm.cu)
 //   static const CUtensorMap* Op::map_a(p, t), Op::map_b(p, t)   rank-3 {inner, rows, batch}
+//   static constexpr int Op::kEpiTiles           staging tiles per epilogue warp, 1 or 2
+//   static void Op::begin(p, t, EpiContext&)     before the accumulator is ready (prefetches)
 //   static void Op::epilogue(p, t, EpiContext&)  one warp's share of the tile
 #pragma once
 #include <cuda_fp16.h>
@@ -42,13 +44,20 @@ constexpr int kHalfN = kTileN / 2;       // columns of B that each CTA brings
 constexpr int kBK = 64;
 constexpr int kABytes = kCtaM * kBK * 2;
 constexpr int kStageBytes = kABytes + kHalfN * kBK * 2;
-constexpr int kStages = 6;
+constexpr int kMaxStages = 6;
 constexpr int kEpiWarps = 8;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
-constexpr int kEpiTileBytes = 32 * 128;  // 32 rows of 128 bytes per epilogue warp
-constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kEpiWarps * kEpiTileBytes + 512;
+constexpr int kEpiTileBytes = 32 * 128;  // a staging tile: 32 rows of 128 bytes
 constexpr int kTmemCols = 512;           // two accumulators of 256 columns
-static_assert(kSmemBytes <= 232448, "more than a CTA's shared memory");
+
+// Shared memory of an Op whose epilogue warps own one or two staging tiles each.
+template <class Op>
+struct Config {
+  static constexpr int kStages = Op::kEpiTiles == 1 ? 6 : 5;
+  static constexpr int kWarpBytes = Op::kEpiTiles * kEpiTileBytes;
+  static constexpr int kSmemBytes = 1024 + kStages * kStageBytes + kEpiWarps * kWarpBytes + 512;
+  static_assert(kSmemBytes <= 232448 && kStages <= kMaxStages, "more than a CTA's shared memory");
+};
 
 struct Tile {
   int m0, n0, z;  // first row, first column, batch index
@@ -58,8 +67,8 @@ struct Tile {
 };
 
 struct __align__(8) Barriers {
-  uint64_t full[kStages];
-  uint64_t empty[kStages];
+  uint64_t full[kMaxStages];
+  uint64_t empty[kMaxStages];
   uint64_t acc_full[2];
   uint64_t acc_empty[2];
   uint64_t aux_full[kEpiWarps];
@@ -72,9 +81,9 @@ struct EpiContext {
   int row0;          // global row of lane 0
   int part;          // columns [128 * part, 128 * part + 128) of the tile belong to this warp
   int lane;
-  uint8_t* smem;     // the warp's staging tile
+  uint8_t* smem;     // the warp's staging tiles
   uint64_t* aux_bar; // the warp's barrier for loads of its own
-  uint32_t* aux_phase;
+  uint32_t aux_phase;
   volatile int* abort;
   int* status;
 };
@@ -171,7 +180,22 @@ __device__ __forceinline__ uint32_t instruction_descriptor(bool fp16, bool a_mn,
   return fp16 ? d & ~((1u << 7) | (1u << 10)) : d;  // operand format 0: fp16
 }
 
-// Tiles dealt round robin.
+// The warp's own loads (the bytes it announced on aux_bar) have landed.  A wait that runs out
+// makes the CTA leave; the tile's results are then incomplete and the status word says so.
+__device__ __forceinline__ void wait_aux(EpiContext& c) {
+  if (!wait_or_leave(c.aux_bar, c.aux_phase, c.abort)) {
+    report_status(c.status, kStatusTimeoutFull);
+    *c.abort = 1;
+  }
+  c.aux_phase ^= 1;
+}
+
+// Bases for Ops whose epilogue loads nothing of its own, and whose tiles are dealt round robin.
+struct Plain {
+  static constexpr int kEpiTiles = 1;
+  template <class P, class C>
+  static __device__ __forceinline__ void begin(const P&, const Tile&, C&) {}
+};
 struct RoundRobin {
   template <class P> static __device__ __forceinline__ int first(const P&, int cluster) {
     return cluster;
@@ -230,12 +254,13 @@ __device__ __forceinline__ void load_acc(uint32_t addr, float (&v)[32]) {
 template <class Op>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 pair_kernel(const __grid_constant__ typename Op::Params p) {
+  constexpr int kStages = Config<Op>::kStages;
   extern __shared__ uint8_t smem_raw[];
   // The dynamic segment starts at the same offset in both CTAs, so this does too.
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
   uint8_t* epi_smem = smem + kStages * kStageBytes;
-  Barriers* bars = reinterpret_cast<Barriers*>(epi_smem + kEpiWarps * kEpiTileBytes);
+  Barriers* bars = reinterpret_cast<Barriers*>(epi_smem + kEpiWarps * Config<Op>::kWarpBytes);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
@@ -383,24 +408,24 @@ pair_kernel(const __grid_constant__ typename Op::Params p) {
     EpiContext c;
     c.part = (warp - 2) >> 2;
     c.lane = lane;
-    c.smem = epi_smem + (warp - 2) * kEpiTileBytes;
+    c.smem = epi_smem + (warp - 2) * Config<Op>::kWarpBytes;
     c.aux_bar = &bars->aux_full[warp - 2];
-    uint32_t aux_phase = 0;
-    c.aux_phase = &aux_phase;
+    c.aux_phase = 0;
     c.abort = abort;
     c.status = p.status;
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int w = Op::first(p, cluster); w < p.total; w = Op::next(p, w, cluster, clusters)) {
       const Tile t = Op::tile(p, w);
+      c.acc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kTileN;
+      c.row0 = t.m0 + rank * kCtaM + quarter * 32;
+      Op::begin(p, t, c);
       if (!wait_or_leave(&bars->acc_full[acc], acc_phase, abort)) {
         report_status(p.status, kStatusTimeoutTmemFull);
         *abort = 1;
         break;
       }
       tc_fence_after();
-      c.acc = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kTileN;
-      c.row0 = t.m0 + rank * kCtaM + quarter * 32;
       Op::epilogue(p, t, c);
       tc_fence_before();
       __syncwarp();
@@ -462,13 +487,13 @@ int launch_pair(const typename Op::Params& p, cudaStream_t stream) {
   static bool configured[64] = {};
   if (device >= 64 || !configured[device]) {
     const cudaError_t e = cudaFuncSetAttribute(
-        pair_kernel<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        pair_kernel<Op>, cudaFuncAttributeMaxDynamicSharedMemorySize, Config<Op>::kSmemBytes);
     if (e != cudaSuccess) return static_cast<int>(e);
     if (device < 64) configured[device] = true;
   }
   const int pairs = sms / 2;
   const int clusters = p.total < pairs ? p.total : pairs;
-  return launch_pdl(pair_kernel<Op>, dim3(2 * clusters), dim3(kThreads), kSmemBytes, stream, p);
+  return launch_pdl(pair_kernel<Op>, dim3(2 * clusters), dim3(kThreads), Config<Op>::kSmemBytes, stream, p);
 }
 
 }  // namespace pair

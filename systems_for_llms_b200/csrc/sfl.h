@@ -139,6 +139,26 @@ typedef struct SflLinearCeGrad {
 long sfl_linear_ce_dh_sum_bytes(int rows, int dim, int vocab, int piece);
 int sfl_linear_ce_bwd(const SflLinearCe* a, const SflLinearCeGrad* g, void* stream);
 
+/* ------------------------------------------------- orthogonalised updates -- */
+/* out bf16 [batch, m, n] (contiguous) = `steps` Newton-Schulz steps X <- aX + (bG + cGG)X from
+ * X = update / (its Frobenius norm + eps), G the Gram matrix of X's shorter side, for every matrix
+ * of the stack.  Matrix z starts at update + (z / inner) * stride0 + (z % inner) * stride1, its rows
+ * `row` elements apart and contiguous.  dtype 0 bf16, 1 fp16, 2 fp32.  Meant for coefficients that
+ * keep singular values of at most 1 within 1.2 (see newton_schulz.cu on precision).  work:
+ * sfl_newton_schulz_bytes of scratch, 256-byte aligned; batch <= 65535. */
+typedef struct SflNewtonSchulz {
+  const void* update;
+  long stride0, stride1, row;
+  int inner, batch, m, n, steps, dtype;
+  float a, b, c, eps;
+  void* out;
+  void* work;
+  long work_bytes;
+  int* status;
+} SflNewtonSchulz;
+long sfl_newton_schulz_bytes(int batch, int m, int n);
+int sfl_newton_schulz(const SflNewtonSchulz* args, void* stream);
+
 /* ------------------------------------------------------------- optimizer -- */
 /* Sum of squares of a flat fp32 buffer -> partial[blocks]; deterministic. */
 int sfl_sqnorm_blocks(long n);
@@ -418,7 +438,7 @@ const char* sfl_version(void);
  * sizeof(SflAttnMask), sizeof(SflComm), sizeof(SflBlockArgs), sizeof(SflTpFuse) and returns how many
  * there are; bindings compare them with their own mirrors. */
 int sfl_struct_sizes(int* sizes, int capacity);
-/* The same for SflRotaryTensor, SflRotaryTable, SflLinearCe, SflLinearCeGrad. */
+/* The same for SflRotaryTensor, SflRotaryTable, SflLinearCe, SflLinearCeGrad, SflNewtonSchulz. */
 int sfl_operator_struct_sizes(int* sizes, int capacity);
 
 /* ------------------------------------------------------ transformer block -- */

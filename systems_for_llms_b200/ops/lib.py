@@ -106,6 +106,7 @@ def register_signature(name: str, argtypes: list) -> None:
 _KERNELS_PER_CALL = {"sfl_attn_bwd": 2, "sfl_rotary_bwd": 2, "sfl_rotary_bwd_partial_bytes": 0,
                      "sfl_linear_ce_part_bytes": 0, "sfl_linear_ce_dh_sum_bytes": 0,
                      "sfl_linear_ce_fwd": 3, "sfl_linear_ce_bwd": 2,
+                     "sfl_newton_schulz_bytes": 0, "sfl_newton_schulz": 17,
                      "sfl_embedding_bwd": 2, "sfl_block_forward": 7, "sfl_block_backward": 11,
                      "sfl_block_saved_bytes": 0, "sfl_block_scratch_bytes": 0, "sfl_rmsnorm_bwd_blocks": 0, "sfl_sqnorm_blocks": 0,
                      "sfl_ipc_alloc": 0, "sfl_ipc_free": 0, "sfl_ipc_get_handle": 0,

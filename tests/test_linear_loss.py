@@ -76,6 +76,7 @@ def test_entry_points_refuse_before_launching():
 def test_records_match_the_compiled_library():
     from systems_for_llms_b200.ops import build as builder
     from systems_for_llms_b200.ops import lib
+    from systems_for_llms_b200.ops.newton_schulz import NewtonSchulz
     from systems_for_llms_b200.ops.rotary import RotaryTable, RotaryTensor
     try:
         builder.build()
@@ -84,6 +85,6 @@ def test_records_match_the_compiled_library():
         pytest.skip(f"kernel library unavailable: {error}")
     call.argtypes, call.restype = [ctypes.POINTER(ctypes.c_int), ctypes.c_int], ctypes.c_int
     sizes = (ctypes.c_int * 8)()
-    mirrors = [RotaryTensor, RotaryTable, LinearCe, LinearCeGrad]
+    mirrors = [RotaryTensor, RotaryTable, LinearCe, LinearCeGrad, NewtonSchulz]
     assert call(sizes, 8) == len(mirrors)
     assert [ctypes.sizeof(m) for m in mirrors] == list(sizes)[:len(mirrors)]
