@@ -20,6 +20,12 @@ CHECKPOINT_POLICIES = ("none", "block")
 DEVICES = ("cpu", "cuda", "mps", "auto")
 PRECISIONS = ("fp32", "bf16")
 DATA_KINDS = ("synthetic", "npy")
+HEAD_LOSSES = ("logits", "pieces")
+OPTIMIZERS = ("adamw", "muon")
+# Options the reference's schema lacks.  ``to_dict`` leaves them out at these values, so a
+# configuration that uses none of them has the form (and hash) it has there.
+EXTENSIONS = {"model": {"qk_norm": False, "head_loss": "logits"},
+              "top": {"optimizer": "adamw", "muon_momentum": 0.95}}
 
 
 @dataclass(frozen=True)
@@ -33,6 +39,8 @@ class ModelConfig:
     rope_theta: float = 10000.0
     attention_backend: str = "eager"
     activation_checkpointing: str = "none"
+    qk_norm: bool = False          # RMS norm of queries and keys per head, before the rotation
+    head_loss: str = "logits"      # "pieces": never keep the logits (ops/linear_loss.py)
 
 
 @dataclass(frozen=True)
@@ -73,6 +81,8 @@ class TrainConfig:
     eval_batches: int = 4
     eval_batch_size: int = 2
     checkpoint_interval: int = 10
+    optimizer: str = "adamw"       # "muon": orthogonalised updates of the blocks' matrices
+    muon_momentum: float = 0.95
 
     _COUNT_FIELDS = ("num_threads", "batch_size", "grad_accum_steps", "max_steps",
                      "eval_interval", "eval_batches", "eval_batch_size", "checkpoint_interval")
@@ -101,10 +111,16 @@ class TrainConfig:
             raise ValueError("require 0 <= min_learning_rate <= learning_rate and learning_rate > 0")
         if self.weight_decay < 0 or self.grad_clip <= 0:
             raise ValueError("weight_decay must be nonnegative and grad_clip positive")
+        if type(self.model.qk_norm) is not bool:
+            raise ValueError("model.qk_norm must be true or false")
+        if not _finite_number(self.muon_momentum) or not 0 <= self.muon_momentum < 1:
+            raise ValueError("muon_momentum must be in [0, 1)")
         choices = (("device", self.device, DEVICES), ("precision", self.precision, PRECISIONS),
                    ("model.attention_backend", self.model.attention_backend, ATTENTION_BACKENDS),
                    ("model.activation_checkpointing", self.model.activation_checkpointing,
                     CHECKPOINT_POLICIES),
+                   ("model.head_loss", self.model.head_loss, HEAD_LOSSES),
+                   ("optimizer", self.optimizer, OPTIMIZERS),
                    ("data.kind", self.data.kind, DATA_KINDS))
         for name, value, allowed in choices:
             if value not in allowed:
@@ -121,6 +137,10 @@ class TrainConfig:
         plain = {f.name: getattr(self, f.name) for f in dataclasses.fields(self)}
         plain["model"] = dataclasses.asdict(self.model)
         plain["data"] = dataclasses.asdict(self.data)
+        for fields, holder in ((EXTENSIONS["model"], plain["model"]), (EXTENSIONS["top"], plain)):
+            for name, default in fields.items():
+                if holder[name] == default:
+                    del holder[name]
         return json.loads(json.dumps(plain, default=str))
 
 

@@ -145,6 +145,64 @@ ns_split_kernel(Stack s, int m, int n, int ld, int vec, const double* __restrict
   }
 }
 
+// ------------------------------------------------------------- Muon around it ----
+// Rows are layers: `len` consecutive elements (a multiple of 4) of a parameter, `stride` apart in
+// the flat buffers and packed in u / o.
+//   v <- momentum v + coef g,   u = coef g + momentum v   (or u = v without Nesterov's look-ahead)
+__global__ void __launch_bounds__(256)
+muon_momentum_kernel(const float* __restrict__ g, float* __restrict__ v, float* __restrict__ u,
+                     long quads, long stride, float momentum, int nesterov,
+                     const float* __restrict__ coef, const float* __restrict__ ok) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const float c = coef == nullptr ? 1.f : *coef;
+  const bool keep = ok != nullptr && *ok == 0.f;  // non-finite gradients: the momentum stays
+  const long row = blockIdx.y * stride;
+  float4* out = reinterpret_cast<float4*>(u) + blockIdx.y * quads;
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < quads; i += gridDim.x * 256L) {
+    const float4 a = reinterpret_cast<const float4*>(g + row)[i];
+    float4 b = reinterpret_cast<const float4*>(v + row)[i];
+    const float4 s = make_float4(a.x * c, a.y * c, a.z * c, a.w * c);
+    b = make_float4(fmaf(momentum, b.x, s.x), fmaf(momentum, b.y, s.y), fmaf(momentum, b.z, s.z),
+                    fmaf(momentum, b.w, s.w));
+    if (!keep) reinterpret_cast<float4*>(v + row)[i] = b;
+    out[i] = nesterov ? make_float4(fmaf(momentum, b.x, s.x), fmaf(momentum, b.y, s.y),
+                                    fmaf(momentum, b.z, s.z), fmaf(momentum, b.w, s.w))
+                      : b;
+  }
+}
+
+// p <- decay p - rate o, and its bf16 copy
+__global__ void __launch_bounds__(256)
+muon_apply_kernel(float* __restrict__ p, __nv_bfloat16* __restrict__ shadow,
+                  const __nv_bfloat16* __restrict__ o, long quads, long stride, float decay,
+                  float rate, const float* __restrict__ ok) {
+  pdl_launch_dependents();
+  pdl_wait();
+  if (ok != nullptr && *ok == 0.f) return;
+  const long row = blockIdx.y * stride;
+  const uint2* src = reinterpret_cast<const uint2*>(o) + blockIdx.y * quads;
+  for (long i = blockIdx.x * 256L + threadIdx.x; i < quads; i += gridDim.x * 256L) {
+    float4 a = reinterpret_cast<const float4*>(p + row)[i];
+    const uint2 q = src[i];
+    const float2 x = unpack_bf16(q.x), y = unpack_bf16(q.y);
+    a = make_float4(fmaf(-rate, x.x, a.x * decay), fmaf(-rate, x.y, a.y * decay),
+                    fmaf(-rate, y.x, a.z * decay), fmaf(-rate, y.y, a.w * decay));
+    reinterpret_cast<float4*>(p + row)[i] = a;
+    if (shadow != nullptr)
+      reinterpret_cast<uint2*>(shadow + row)[i] = make_uint2(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w));
+  }
+}
+
+bool rows_ok(const void* p, int rows, long len, long stride, int align) {
+  return p != nullptr && (reinterpret_cast<uintptr_t>(p) % align) == 0 && rows >= 1 &&
+         rows <= 65535 && len >= 4 && len % 4 == 0 && (rows == 1 || (stride >= len && stride % 4 == 0));
+}
+dim3 rows_grid(int rows, long len) {
+  const long blocks = (len / 4 + 1023) / 1024;  // four steps per thread
+  return dim3(static_cast<unsigned>(blocks < 1 ? 1 : (blocks > 65535 ? 65535 : blocks)), rows);
+}
+
 // ------------------------------------------------- symmetric products: G, b G + c G G ----
 // out = alpha aux + beta A B^T with A = B: tiles on and above the diagonal, mirrored.
 struct SymOp : pair::RoundRobin {
@@ -402,6 +460,32 @@ int normalise(const Stack& s, int batch, int m, int n, int ld, float eps, double
 
 }  // namespace
 }  // namespace sfl
+
+extern "C" int sfl_muon_momentum(const float* grad, float* momentum_buffer, float* update, int rows,
+                                 long len, long stride, float momentum, int nesterov,
+                                 const float* grad_coef, const float* ok_flag, void* stream) {
+  using namespace sfl;
+  if (!rows_ok(grad, rows, len, stride, 16) || !rows_ok(momentum_buffer, rows, len, stride, 16) ||
+      !rows_ok(update, rows, len, stride, 16))
+    return -2;
+  return launch_pdl(muon_momentum_kernel, rows_grid(rows, len), dim3(256), 0,
+                    static_cast<cudaStream_t>(stream), grad, momentum_buffer, update, len / 4, stride,
+                    momentum, nesterov, grad_coef, ok_flag);
+}
+
+extern "C" int sfl_muon_apply(float* param, void* bf16_shadow, const void* update_bf16, int rows,
+                              long len, long stride, float decay, float rate, const float* ok_flag,
+                              void* stream) {
+  using namespace sfl;
+  if (!rows_ok(param, rows, len, stride, 16) || !rows_ok(update_bf16, rows, len, stride, 8) ||
+      (bf16_shadow != nullptr && !rows_ok(bf16_shadow, rows, len, stride, 8)))
+    return -2;
+  return launch_pdl(muon_apply_kernel, rows_grid(rows, len), dim3(256), 0,
+                    static_cast<cudaStream_t>(stream), param,
+                    static_cast<__nv_bfloat16*>(bf16_shadow),
+                    static_cast<const __nv_bfloat16*>(update_bf16), len / 4, stride, decay, rate,
+                    ok_flag);
+}
 
 extern "C" long sfl_newton_schulz_bytes(int batch, int m, int n) {
   using namespace sfl;

@@ -159,6 +159,18 @@ typedef struct SflNewtonSchulz {
 long sfl_newton_schulz_bytes(int batch, int m, int n);
 int sfl_newton_schulz(const SflNewtonSchulz* args, void* stream);
 
+/* Muon around it.  The same parameter of `rows` layers: `len` consecutive fp32 elements (a multiple
+ * of 4), `stride` apart in the flat buffers, packed in the update.  The gradient is multiplied by
+ * *grad_coef (may be NULL); nothing is changed when ok_flag != NULL and *ok_flag == 0.
+ *   momentum_buffer <- momentum * momentum_buffer + grad
+ *   update           = grad + momentum * momentum_buffer  (nesterov), or momentum_buffer */
+int sfl_muon_momentum(const float* grad, float* momentum_buffer, float* update, int rows, long len,
+                      long stride, float momentum, int nesterov, const float* grad_coef,
+                      const float* ok_flag, void* stream);
+/* param <- decay * param - rate * update, and the bf16 copy (may be NULL). */
+int sfl_muon_apply(float* param, void* bf16_shadow, const void* update_bf16, int rows, long len,
+                   long stride, float decay, float rate, const float* ok_flag, void* stream);
+
 /* ------------------------------------------------------------- optimizer -- */
 /* Sum of squares of a flat fp32 buffer -> partial[blocks]; deterministic. */
 int sfl_sqnorm_blocks(long n);

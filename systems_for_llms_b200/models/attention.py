@@ -15,7 +15,7 @@ import torch
 from torch import nn
 from torch.nn import functional as F
 
-from .layers import Linear
+from .layers import Linear, RMSNorm
 
 
 class RotaryPositionalEmbedding(nn.Module):
@@ -65,7 +65,7 @@ def scaled_dot_product_attention(query, key, value, mask=None):
 class MultiHeadSelfAttention(nn.Module):
     def __init__(self, d_model: int, num_heads: int, theta: float | None = None,
                  max_seq_len: int | None = None, device=None, dtype=None,
-                 attention_backend: str = "eager"):
+                 attention_backend: str = "eager", qk_norm: bool = False):
         super().__init__()
         if d_model <= 0 or num_heads <= 0:
             raise ValueError("d_model and num_heads must be positive")
@@ -83,6 +83,9 @@ class MultiHeadSelfAttention(nn.Module):
         self.k_proj = Linear(d_model, d_model, device=device, dtype=dtype)
         self.v_proj = Linear(d_model, d_model, device=device, dtype=dtype)
         self.output_proj = Linear(d_model, d_model, device=device, dtype=dtype)
+        # Statistics and weights per head dimension, shared by the heads of the layer.
+        self.q_norm = RMSNorm(self.d_k, device=device, dtype=dtype) if qk_norm else None
+        self.k_norm = RMSNorm(self.d_k, device=device, dtype=dtype) if qk_norm else None
         self.rope = (RotaryPositionalEmbedding(theta, self.d_k, max_seq_len, device=device)
                      if theta is not None else None)
 
@@ -102,6 +105,8 @@ class MultiHeadSelfAttention(nn.Module):
         query = self._split_heads(self.q_proj(x))
         key = self._split_heads(self.k_proj(x))
         value = self._split_heads(self.v_proj(x))
+        if self.q_norm is not None:
+            query, key = self.q_norm(query), self.k_norm(key)
         if self.rope is not None:
             query = self.rope(query, token_positions)
             key = self.rope(key, token_positions)

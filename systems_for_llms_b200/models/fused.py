@@ -31,6 +31,8 @@ from ..attention import flash
 from ..ops import functional as K
 from ..ops import gemm as G
 from ..ops import lib as _lib
+from ..ops import linear_loss as L
+from ..ops import rotary as R
 
 ALIGN = 64  # elements; keeps every parameter 256-byte (fp32) / 128-byte (bf16) aligned
 
@@ -83,7 +85,9 @@ class FusedEngine:
         self._grad_views: dict = {}
         # Run whole blocks through one library call (csrc/block.cu) instead of one
         # Python-driven launch per kernel; tensor-parallel engines keep the latter.
-        self.native_blocks = os.environ.get("SFL_PYTHON_BLOCKS", "0") != "1"
+        # The native runner rotates in the projection's epilogue and has no per-head norm.
+        self.native_blocks = (os.environ.get("SFL_PYTHON_BLOCKS", "0") != "1"
+                              and not model.qk_norm)
         self._native_args: dict = {}
         self._native_sizes: dict = {}
         self._native_keep: list = []
@@ -104,7 +108,10 @@ class FusedEngine:
         # a data-parallel wrapper can reduce fixed-size buckets.
         order = [model.token_embeddings.weight]
         for layer in model.layers:
-            order += [layer.attn_norm.weight, layer.attn.q_proj.weight, layer.attn.k_proj.weight,
+            order += [layer.attn_norm.weight]
+            if model.qk_norm:
+                order += [layer.attn.q_norm.weight, layer.attn.k_norm.weight]
+            order += [layer.attn.q_proj.weight, layer.attn.k_proj.weight,
                       layer.attn.v_proj.weight, layer.attn.output_proj.weight,
                       layer.ffn_norm.weight, layer.ffn.w1.weight, layer.ffn.w3.weight,
                       layer.ffn.w2.weight]
@@ -271,6 +278,10 @@ class FusedEngine:
         ids, B, T = self._prepare(input_ids)
         x = self._trunk(ids, B, T)
         flat_targets = targets.reshape(-1).contiguous()
+        if self.model.head_loss == "pieces":
+            if torch.is_grad_enabled():
+                return _HeadLossPieces.apply(x, flat_targets, self, float(scale))
+            return head_loss_pieces(self, x, flat_targets)[0] * scale
         if torch.is_grad_enabled():
             return _HeadLoss.apply(x, flat_targets, self, float(scale))
         logits = head_logits(self, x)[0]
@@ -391,6 +402,12 @@ def _use_native(engine: FusedEngine) -> bool:
 
 
 # ------------------------------------------------------------ block kernels --
+def _head_views(flat: torch.Tensor, B: int, T: int, parts: int, H: int, dk: int):
+    """``[B, H, T, dk]`` views of the parts (q | k | v) of a projection ``[B*T, parts*H*dk]``."""
+    heads = flat.view(B, T, parts, H, dk)
+    return tuple(heads[:, :, i].permute(0, 2, 1, 3) for i in range(parts))
+
+
 def block_forward(engine: FusedEngine, index: int, x: torch.Tensor, B: int, T: int):
     """Returns ``(x_out, saved)`` where ``saved`` holds what backward needs."""
     if _use_native(engine):
@@ -403,9 +420,19 @@ def block_forward(engine: FusedEngine, index: int, x: torch.Tensor, B: int, T: i
     x2 = x.reshape(M, d)
     h1, rstd1 = K.rmsnorm(x2, layer.attn_norm.weight, layer.attn_norm.eps)
     wqkv = engine.shadow(layer.attn.q_proj.weight, 3 * aw)
-    qkv = G.linear_fwd_rope(h1, wqkv, engine.cos, engine.sin, T, 2 * aw, dk)
-    heads = qkv.view(B, T, 3, H, dk)
-    q, k, v = (heads[:, :, i].permute(0, 2, 1, 3) for i in range(3))
+    if engine.model.qk_norm:
+        # the raw projection is kept for backward; the normed and turned q | k get a buffer
+        qkv = G.linear_fwd(h1, wqkv)
+        turned = torch.empty(M, 2 * aw, dtype=torch.bfloat16, device=x.device)
+        q, k = _head_views(turned, B, T, 2, H, dk)
+        q_raw, k_raw, v = _head_views(qkv, B, T, 3, H, dk)
+        q_norm, k_norm = layer.attn.q_norm, layer.attn.k_norm
+        R.qk_norm_rotary_into(q_raw, k_raw, q_norm.weight, k_norm.weight, engine.cos, engine.sin,
+                              eps=q_norm.eps, out=(q, k))
+    else:
+        turned = None
+        qkv = G.linear_fwd_rope(h1, wqkv, engine.cos, engine.sin, T, 2 * aw, dk)
+        q, k, v = _head_views(qkv, B, T, 3, H, dk)
     attn = torch.empty(M, aw, dtype=torch.bfloat16, device=x.device)
     lse = torch.empty(B, H, T, dtype=torch.float32, device=x.device)
     mask = flash.causal_mask(x.device, T)
@@ -426,7 +453,7 @@ def block_forward(engine: FusedEngine, index: int, x: torch.Tensor, B: int, T: i
         x_out = tp.gemm_reduce_residual(g, w2, x_mid, 2 * index + 1)
     else:
         x_out = tp.reduce_residual(G.linear_fwd(g, w2, tp.partial(M, d)), x_mid, 2 * index + 1)
-    saved = (x2, rstd1, h1, qkv, attn, lse, x_mid, rstd2, h2, a13, g)
+    saved = (x2, rstd1, h1, qkv, attn, lse, x_mid, rstd2, h2, a13, g, turned)
     return x_out.view(B, T, d), saved
 
 
@@ -437,7 +464,7 @@ def block_backward(engine: FusedEngine, index: int, saved, d_out: torch.Tensor, 
     d, dk, H, dff, aw = engine.d_model, engine.d_k, engine.num_heads, engine.d_ff, engine.attn_width
     tp = engine.tp
     M = B * T
-    x2, rstd1, h1, qkv, attn, lse, x_mid, rstd2, h2, a13, g = saved
+    x2, rstd1, h1, qkv, attn, lse, x_mid, rstd2, h2, a13, g, turned = saved
     dres = d_out.reshape(M, d)
     if not dres.is_contiguous():
         dres = dres.contiguous()
@@ -470,14 +497,22 @@ def block_backward(engine: FusedEngine, index: int, saved, d_out: torch.Tensor, 
     wgrads.append((dres2_bf16, attn, engine.grad_view(attn_p.output_proj.weight),
                    engine.claim(attn_p.output_proj.weight)))
     dqkv = torch.empty_like(qkv)
-    heads = qkv.view(B, T, 3, H, dk)
-    dheads = dqkv.view(B, T, 3, H, dk)
-    q, k, v = (heads[:, :, i].permute(0, 2, 1, 3) for i in range(3))
-    dq, dkk, dv = (dheads[:, :, i].permute(0, 2, 1, 3) for i in range(3))
+    q, k, v = _head_views(qkv, B, T, 3, H, dk)
+    dq, dkk, dv = _head_views(dqkv, B, T, 3, H, dk)
     as_heads = lambda t: t.view(B, T, H, dk).permute(0, 2, 1, 3)
     mask = flash.causal_mask(d_out.device, T)
-    flash.flash_bwd(q, k, v, as_heads(attn), as_heads(d_attn), lse, dq, dkk, dv, mask, dk ** -0.5,
-                    rope=(engine.cos, engine.sin))   # dq, dk come back un-rotated
+    if turned is None:
+        flash.flash_bwd(q, k, v, as_heads(attn), as_heads(d_attn), lse, dq, dkk, dv, mask,
+                        dk ** -0.5, rope=(engine.cos, engine.sin))  # dq, dk come back un-rotated
+    else:
+        flash.flash_bwd(*_head_views(turned, B, T, 2, H, dk), v, as_heads(attn), as_heads(d_attn),
+                        lse, dq, dkk, dv, mask, dk ** -0.5)
+        weights = (attn_p.q_norm.weight, attn_p.k_norm.weight)
+        grads = R.qk_norm_rotary_grad(q, k, *weights, engine.cos, engine.sin, None, dq, dkk,
+                                      eps=attn_p.q_norm.eps, layout="interleaved", out=(dq, dkk))
+        for weight, grad in zip(weights, grads[2:]):
+            accumulate, view = engine.claim(weight), engine.grad_view(weight)
+            view.add_(grad) if accumulate else view.copy_(grad)
     if tp is None:
         dh1 = G.linear_dgrad(dqkv, engine.shadow(attn_p.q_proj.weight, 3 * aw))
     elif tp.can_fuse(d):
@@ -521,6 +556,12 @@ def head_backward(engine: FusedEngine, saved, dlogits: torch.Tensor) -> torch.Te
     grad = engine.grad_view(model.lm_head.weight)
     epi = G.GemmEpilogue(kind=G.EPI_F32, beta=int(acc), out=grad.data_ptr(), ldo=grad.stride(0))
     G.gemm(dl, h, V, engine.d_model, h.shape[0], epi, a_mn=True, b_mn=True)
+    return _final_norm_backward(engine, x2, rstd, dh)
+
+
+def _final_norm_backward(engine: FusedEngine, x2: torch.Tensor, rstd: torch.Tensor,
+                         dh: torch.Tensor) -> torch.Tensor:
+    model = engine.model
     acc = engine.claim(model.ln_final.weight)
     dx, dx_bf16 = K.rmsnorm_bwd(dh, x2, model.ln_final.weight, rstd, None,
                                 engine.grad_view(model.ln_final.weight), acc, want_bf16=True)
@@ -528,6 +569,26 @@ def head_backward(engine: FusedEngine, saved, dlogits: torch.Tensor) -> torch.Te
     if engine.on_block_backward is not None:
         engine.on_block_backward(engine.head_offset)
     return dx
+
+
+def head_loss_pieces(engine: FusedEngine, x: torch.Tensor, targets: torch.Tensor):
+    """Mean loss of the final norm and projection without keeping logits, and what its backward
+    needs."""
+    model = engine.model
+    x2 = x.reshape(-1, engine.d_model)
+    h, rstd = K.rmsnorm(x2, model.ln_final.weight, model.ln_final.eps)
+    _, lse2, totals, loss = L.linear_ce_forward(h, engine.shadow(model.lm_head.weight), targets,
+                                                -100, True)
+    return loss, (x2, h, rstd, targets, lse2, totals)
+
+
+def head_loss_pieces_backward(engine: FusedEngine, saved, grad: torch.Tensor) -> torch.Tensor:
+    weight = engine.model.lm_head.weight
+    x2, h, rstd, targets, lse2, totals = saved
+    accumulate = engine.claim(weight)
+    dh = L.linear_ce_backward(h, engine.shadow(weight), targets, -100, lse2, grad, totals,
+                              engine.grad_view(weight), accumulate)
+    return _final_norm_backward(engine, x2, rstd, dh)
 
 
 # ------------------------------------------------------------ autograd nodes --
@@ -612,4 +673,19 @@ class _HeadLoss(torch.autograd.Function):
         dlogits, *saved = ctx.saved_tensors
         K.scale_bf16_unless_one(dlogits, grad)    # the incoming gradient is normally 1
         dx = head_backward(ctx.engine, saved, dlogits)
+        return dx.view(ctx.shape), None, None, None
+
+
+class _HeadLossPieces(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, targets, engine, scale):
+        loss, saved = head_loss_pieces(engine, x, targets)
+        ctx.engine, ctx.shape, ctx.scale = engine, x.shape, scale
+        ctx.save_for_backward(*saved)
+        return loss * scale
+
+    @staticmethod
+    def backward(ctx, grad):
+        grad = grad.float() * ctx.scale
+        dx = head_loss_pieces_backward(ctx.engine, ctx.saved_tensors, grad)
         return dx.view(ctx.shape), None, None, None

@@ -13,7 +13,10 @@ implementations chosen per call:
 
 ``loss(input_ids, targets, scale)`` is the training entry point: on the fused
 path it never materialises fp32 logits (vocabulary projection, log-sum-exp, loss
-and the logit gradient are produced together).
+and the logit gradient are produced together); with ``head_loss="pieces"`` it
+keeps no logits at all (ops/linear_loss.py), for vocabularies whose logits are too
+large.  ``qk_norm=True`` norms queries and keys per head before the rotation, in one
+kernel with it on the fused path (ops/rotary.py).  The reference has neither option.
 """
 
 from __future__ import annotations
@@ -28,12 +31,14 @@ from .layers import Embedding, Linear, RMSNorm, SwiGLU
 
 class TransformerBlock(nn.Module):
     def __init__(self, d_model: int, num_heads: int, d_ff: int, theta: float, max_seq_len: int,
-                 device=None, dtype=None, attention_backend: str = "eager"):
+                 device=None, dtype=None, attention_backend: str = "eager",
+                 qk_norm: bool = False):
         super().__init__()
         self.attn_norm = RMSNorm(d_model, device=device, dtype=dtype)
         self.attn = MultiHeadSelfAttention(d_model=d_model, num_heads=num_heads, theta=theta,
                                            max_seq_len=max_seq_len, device=device, dtype=dtype,
-                                           attention_backend=attention_backend)
+                                           attention_backend=attention_backend,
+                                           qk_norm=qk_norm)
         self.ffn_norm = RMSNorm(d_model, device=device, dtype=dtype)
         self.ffn = SwiGLU(d_model=d_model, d_ff=d_ff, device=device, dtype=dtype)
 
@@ -45,7 +50,8 @@ class TransformerBlock(nn.Module):
 class TransformerLM(nn.Module):
     def __init__(self, vocab_size: int, context_length: int, d_model: int, num_layers: int,
                  num_heads: int, d_ff: int, rope_theta: float, device=None, dtype=None,
-                 attention_backend: str = "eager", activation_checkpointing: str = "none"):
+                 attention_backend: str = "eager", activation_checkpointing: str = "none",
+                 qk_norm: bool = False, head_loss: str = "logits"):
         super().__init__()
         sizes = dict(vocab_size=vocab_size, context_length=context_length, d_model=d_model,
                      num_layers=num_layers, num_heads=num_heads, d_ff=d_ff)
@@ -54,15 +60,18 @@ class TransformerLM(nn.Module):
                 raise ValueError(f"{name} must be a positive integer")
         if activation_checkpointing not in ("none", "block"):
             raise ValueError("activation_checkpointing must be 'none' or 'block'")
+        if head_loss not in ("logits", "pieces"):
+            raise ValueError("head_loss must be 'logits' or 'pieces'")
         for name, value in sizes.items():
             setattr(self, name, value)
         self.theta = rope_theta
         self.attention_backend = attention_backend
         self.activation_checkpointing = activation_checkpointing
+        self.qk_norm, self.head_loss = qk_norm, head_loss
         self.token_embeddings = Embedding(vocab_size, d_model, device=device, dtype=dtype)
         self.layers = nn.ModuleList([
             TransformerBlock(d_model, num_heads, d_ff, rope_theta, context_length, device=device,
-                             dtype=dtype, attention_backend=attention_backend)
+                             dtype=dtype, attention_backend=attention_backend, qk_norm=qk_norm)
             for _ in range(num_layers)])
         self.ln_final = RMSNorm(d_model, device=device, dtype=dtype)
         self.lm_head = Linear(d_model, vocab_size, device=device, dtype=dtype)

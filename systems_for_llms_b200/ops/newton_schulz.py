@@ -38,6 +38,46 @@ _lib.register_signature("sfl_newton_schulz_bytes", [c_int, c_int, c_int])
 _lib.register_signature("sfl_newton_schulz", [POINTER(NewtonSchulz), _P])
 
 
+_lib.register_signature("sfl_muon_momentum", [_P, _P, _P, c_int, c_long, c_long, c_float, c_int, _P,
+                                              _P, _P])
+_lib.register_signature("sfl_muon_apply", [_P, _P, _P, c_int, c_long, c_long, c_float, c_float, _P,
+                                           _P])
+
+
+def muon_momentum(grad: torch.Tensor, buffer: torch.Tensor, update: torch.Tensor, *,
+                  momentum: float, nesterov: bool, coef: torch.Tensor | None = None,
+                  ok_flag: torch.Tensor | None = None) -> None:
+    """Momentum of the rows (layers) of two equally strided fp32 views ``[rows, len]`` and the
+    packed ``update`` that is to be orthogonalised."""
+    rows, length = grad.shape
+    if buffer.shape != grad.shape or buffer.stride() != grad.stride() or grad.stride(1) != 1:
+        raise ValueError("grad and buffer must be equally strided rows")
+    if update.numel() != grad.numel() or not update.is_contiguous():
+        raise ValueError("update must be contiguous with the elements of grad")
+    with _lib.on_device(grad.device):
+        code = _lib.lib().sfl_muon_momentum(grad.data_ptr(), buffer.data_ptr(), update.data_ptr(),
+                                            rows, length, grad.stride(0), float(momentum),
+                                            int(nesterov), _lib.ptr(coef), _lib.ptr(ok_flag),
+                                            _lib.stream_ptr())
+    _lib.check(code, "sfl_muon_momentum")
+
+
+def muon_apply(param: torch.Tensor, shadow: torch.Tensor | None, update: torch.Tensor, *,
+               decay: float, rate: float, ok_flag: torch.Tensor | None = None) -> None:
+    """``param <- decay * param - rate * update`` on the rows of a view ``[rows, len]``, and the
+    equally strided bf16 copy."""
+    rows, length = param.shape
+    if shadow is not None and (shadow.shape != param.shape or shadow.stride() != param.stride()):
+        raise ValueError("shadow must have the rows of param")
+    if update.numel() != param.numel() or not update.is_contiguous() or param.stride(1) != 1:
+        raise ValueError("update must be contiguous with the elements of param")
+    with _lib.on_device(param.device):
+        code = _lib.lib().sfl_muon_apply(param.data_ptr(), _lib.ptr(shadow), update.data_ptr(), rows,
+                                         length, param.stride(0), float(decay), float(rate),
+                                         _lib.ptr(ok_flag), _lib.stream_ptr())
+    _lib.check(code, "sfl_muon_apply")
+
+
 def largest_singular_value(coefficients=QUINTIC, steps: int = 5) -> float:
     """Largest value that singular values starting in [0, 1] reach within ``steps`` applications
     of ``a s + b s^3 + c s^5``; infinite when they run away."""
@@ -138,3 +178,17 @@ def newton_schulz(update: torch.Tensor, *, steps: int = 5, coefficients=QUINTIC,
         code = handle.sfl_newton_schulz(byref(args), _lib.stream_ptr())
     _lib.check(code, "sfl_newton_schulz")
     return out
+
+
+def newton_schulz_portable(update: torch.Tensor, *, steps: int = 5, coefficients=QUINTIC,
+                           eps: float = 1e-7) -> torch.Tensor:
+    """The same in fp32 PyTorch operators, for devices without the kernels; fp32 result."""
+    a, b, c = coefficients
+    x = update.float()
+    x = x / (torch.linalg.matrix_norm(x, keepdim=True) + eps)
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.mT if tall else x
+    for _ in range(steps):
+        gram = x @ x.mT
+        x = a * x + (b * gram + c * gram @ gram) @ x
+    return x.mT if tall else x

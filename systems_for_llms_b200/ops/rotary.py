@@ -256,8 +256,9 @@ class _QKNormRotary(torch.autograd.Function):
 def qk_norm_rotary_grad(q, k, q_weight, k_weight, cos, sin, positions, dq_out, dk_out, *,
                         eps: float, layout: str, out=None):
     """Gradients ``(dq, dk, dq_weight, dk_weight)`` of ``qk_norm_rotary`` for the gradients of its
-    results; ``out`` names the tensors that receive dq and dk.  The weight gradients are summed
-    in a fixed order."""
+    results; ``out`` names the tensors that receive dq and dk, which may be the incoming gradients
+    themselves (a warp reads a head before it writes it).  The weight gradients are summed in a
+    fixed order."""
     xs, gs = (q, k), (_rows(dq_out, q), _rows(dk_out, k))
     dxs = out if out is not None else (_new(q), _new(k))
     B, _, T, D = q.shape
@@ -280,6 +281,13 @@ def qk_norm_rotary_grad(q, k, q_weight, k_weight, cos, sin, positions, dq_out, d
                                      _lib.stream_ptr())
     _lib.check(code, "sfl_rotary_bwd")
     return (*dxs, dws[0], dws[1])
+
+
+def qk_norm_rotary_into(q, k, q_weight, k_weight, cos, sin, positions=None, *, eps: float,
+                        layout: str = "interleaved", out) -> None:
+    """``qk_norm_rotary`` into ``out`` without argument checks or autograd: the building block of
+    models/fused.py, next to ``qk_norm_rotary_grad``."""
+    _launch([q, k], out, [q_weight, k_weight], cos, sin, positions, eps, layout)
 
 
 def _no_grad_out(out, *inputs) -> None:

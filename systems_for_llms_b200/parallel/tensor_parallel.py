@@ -154,6 +154,8 @@ def parallelize_model(model, group=None):
     Every rank must hold the same full model.  All layers are validated before
     any is changed, and no random numbers are drawn.  Build the optimizer after.
     """
+    if getattr(model, "qk_norm", False):
+        raise ValueError("per-head query/key norms are not supported under tensor parallelism")
     world_size, _ = _world(group)
     if getattr(model, "_tp_parallelized", False):
         raise ValueError("Model is already tensor parallel")

@@ -46,7 +46,7 @@ import torch.distributed as dist
 from ..config import TrainConfig, load_config
 from ..data import batch_at, load_data
 from ..models.transformer import TransformerLM
-from ..optim import FusedAdamW
+from ..optim import FusedAdamW, FusedMuon
 from ..train import autocast, check_precision, learning_rate, synchronize
 
 MODES = ("single", "naive", "ddp", "zero1", "fsdp", "tp")
@@ -136,6 +136,19 @@ def fsdp_clip_grad_norm(model, max_norm):
     return clip_grad_norm_sharded(model.parameters(), max_norm)
 
 
+def check_extensions(config, mode: str) -> None:
+    """Options that a mode's sharding does not cover are refused before anything is wrapped."""
+    if mode in ("fsdp", "tp"):
+        if config.model.qk_norm:
+            raise ValueError(f"model.qk_norm is not supported in mode {mode}")
+        if config.model.head_loss != "logits":
+            raise ValueError(f"model.head_loss={config.model.head_loss!r} is not supported in mode "
+                             f"{mode}")
+    if mode in ("zero1", "fsdp", "tp") and config.optimizer != "adamw":
+        raise ValueError(f"optimizer={config.optimizer!r} needs whole gradient matrices on every "
+                         f"rank; mode {mode} shards them")
+
+
 class Strategy:
     """Everything mode-specific: wrapping, the per-microbatch context, reduction, update."""
 
@@ -148,6 +161,7 @@ class Strategy:
         self.engine = None
         self.sharding = None
         kwargs = dict(lr=config.learning_rate, betas=(0.9, 0.95), weight_decay=config.weight_decay)
+        check_extensions(config, mode)
         fused_possible = device.type == "cuda" and config.precision == "bf16"
         if mode == "tp":
             from .tensor_parallel import describe_sharding, parallelize_model
@@ -187,6 +201,9 @@ class Strategy:
             self.optimizer = ShardedStepper(self.model, **kwargs)
         elif mode == "fsdp":
             self.optimizer = torch.optim.AdamW(self.model.parameters(), **kwargs)
+        elif config.optimizer == "muon":
+            self.optimizer = FusedMuon.from_model(base_model, engine=self.engine,
+                                                  momentum=config.muon_momentum, **kwargs)
         else:
             self.optimizer = FusedAdamW(base_model.parameters(), engine=self.engine, **kwargs)
 
@@ -241,7 +258,7 @@ class Strategy:
             norm = fsdp_clip_grad_norm(self.model, config.grad_clip)
             self.optimizer.step()
             return norm
-        if isinstance(self.optimizer, FusedAdamW):
+        if isinstance(self.optimizer, (FusedAdamW, FusedMuon)):
             return self.optimizer.clip_and_step(config.grad_clip)
         norm = torch.nn.utils.clip_grad_norm_(self.base.parameters(), config.grad_clip,
                                               error_if_nonfinite=True)

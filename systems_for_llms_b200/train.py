@@ -34,7 +34,7 @@ import torch
 from .config import TrainConfig, load_config
 from .data import batch_at, file_sha256, load_data
 from .models.transformer import TransformerLM
-from .optim import FusedAdamW
+from .optim import FusedAdamW, FusedMuon
 from .training.loss import cross_entropy  # noqa: F401  (re-exported for API parity)
 
 TIMING_SCOPE = ("run() entry to summary construction; excludes interpreter/import startup, "
@@ -90,14 +90,18 @@ def learning_rate(step: int, config: TrainConfig) -> float:
     return floor + 0.5 * (peak - floor) * (1 + math.cos(math.pi * progress))
 
 
-def make_optimizer(model: TransformerLM, config: TrainConfig) -> FusedAdamW:
+def make_optimizer(model: TransformerLM, config: TrainConfig) -> FusedAdamW | FusedMuon:
+    if config.optimizer == "muon":
+        return FusedMuon.from_model(model, lr=config.learning_rate, betas=(0.9, 0.95),
+                                    momentum=config.muon_momentum,
+                                    weight_decay=config.weight_decay)
     return FusedAdamW(model.parameters(), lr=config.learning_rate, betas=(0.9, 0.95),
                       weight_decay=config.weight_decay, engine=None)
 
 
 def _attach_engine(model: TransformerLM, optimizer, config: TrainConfig, device) -> None:
     """Give the optimizer the model's fused engine once it exists."""
-    if isinstance(optimizer, FusedAdamW) and optimizer.engine is None and device.type == "cuda":
+    if isinstance(optimizer, (FusedAdamW, FusedMuon)) and optimizer.engine is None and device.type == "cuda":
         with autocast(config, device):
             optimizer.engine = model.fused_engine()
 
@@ -122,7 +126,7 @@ def train_step(model: TransformerLM, optimizer: torch.optim.Optimizer, data: np.
         loss.backward()
         del x, y, loss
     _attach_engine(model, optimizer, config, device)
-    if isinstance(optimizer, FusedAdamW):
+    if isinstance(optimizer, (FusedAdamW, FusedMuon)):
         norm = optimizer.clip_and_step(config.grad_clip)
     else:
         norm = torch.nn.utils.clip_grad_norm_(model.parameters(), config.grad_clip,
@@ -405,6 +409,8 @@ def main() -> None:
     parser.add_argument("--batch-size", type=int, help="sequences per microbatch")
     parser.add_argument("--grad-accum-steps", type=int)
     parser.add_argument("--activation-checkpointing", choices=["none", "block"])
+    parser.add_argument("--head-loss", choices=["logits", "pieces"])
+    parser.add_argument("--optimizer", choices=["adamw", "muon"])
     args = parser.parse_args()
     config = load_config(args.config)
     model_overrides = {}
@@ -412,10 +418,12 @@ def main() -> None:
         model_overrides["attention_backend"] = args.attention_backend
     if args.activation_checkpointing is not None:
         model_overrides["activation_checkpointing"] = args.activation_checkpointing
+    if args.head_loss is not None:
+        model_overrides["head_loss"] = args.head_loss
     if model_overrides:
         config = replace(config, model=replace(config.model, **model_overrides))
     top = {name: getattr(args, name) for name in ("device", "precision", "batch_size",
-                                                  "grad_accum_steps")
+                                                  "grad_accum_steps", "optimizer")
            if getattr(args, name) is not None}
     config = replace(config, **top)
     summary = run(config, args.output_dir, args.resume, args.stop_after)

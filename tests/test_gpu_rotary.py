@@ -198,6 +198,13 @@ def test_strides_positions_and_out(dev):
     mine = q.contiguous()
     assert rotary(mine, cos, sin, out=mine) is mine
     assert torch.equal(mine, rotary(q, cos, sin))
+    # gradients in place of the incoming ones
+    from systems_for_llms_b200.ops.rotary import qk_norm_rotary_grad
+    grads = [torch.randn(B, n, T, D, device=dev).to(q.dtype) for n in (H, G)]
+    kw = dict(eps=1e-5, layout="half")
+    want = qk_norm_rotary_grad(q, k, *weights, cos, sin, None, *grads, **kw)
+    got = qk_norm_rotary_grad(q, k, *weights, cos, sin, None, *grads, out=tuple(grads), **kw)
+    assert got[0] is grads[0] and all(torch.equal(a, b) for a, b in zip(got, want))
     # an expanded tensor: heads that share one key
     one = k[:, :1].expand(B, 3, T, D)
     assert torch.equal(rotary(one, cos, sin)[:, 2], rotary(k[:, :1], cos, sin)[:, 0])
