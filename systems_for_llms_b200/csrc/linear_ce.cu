@@ -75,12 +75,12 @@ struct StatsOp : pair::Plain, pair::RoundRobin {
     float* picked;     // [rows]: the target's logit
     int rows, vocab;
   };
-  static __device__ __forceinline__ bool a_mn(const Tile&) { return false; }
-  static __device__ __forceinline__ bool b_mn(const Tile&) { return false; }
-  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile&) {
+  static __device__ __forceinline__ bool a_mn(const Tile&, int) { return false; }
+  static __device__ __forceinline__ bool b_mn(const Tile&, int) { return false; }
+  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile&, int) {
     return &p.a;
   }
-  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile&) {
+  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile&, int) {
     return &p.b;
   }
   static __device__ __forceinline__ Tile tile(const Params& p, int w) {
@@ -242,12 +242,12 @@ struct DlogitsOp : pair::Plain, pair::RoundRobin {
     float one;           // 1, or 2^12 for fp16
     int rows, vocab_begin, width;
   };
-  static __device__ __forceinline__ bool a_mn(const Tile&) { return false; }
-  static __device__ __forceinline__ bool b_mn(const Tile&) { return false; }
-  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile&) {
+  static __device__ __forceinline__ bool a_mn(const Tile&, int) { return false; }
+  static __device__ __forceinline__ bool b_mn(const Tile&, int) { return false; }
+  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile&, int) {
     return &p.a;
   }
-  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile&) {
+  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile&, int) {
     return &p.b;
   }
   static __device__ __forceinline__ Tile tile(const Params& p, int w) {
@@ -359,12 +359,12 @@ struct GradOp : pair::Plain {
     return Tile{w % p.dh_mt * pair::kTileM, w / p.dh_mt * pair::kTileN, 0,
                 left < p.dh_part_kb ? left : p.dh_part_kb, kb0, kDh + 2 * part};
   }
-  static __device__ __forceinline__ bool a_mn(const Tile& t) { return t.kind == kDw; }
-  static __device__ __forceinline__ bool b_mn(const Tile&) { return true; }
-  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile& t) {
+  static __device__ __forceinline__ bool a_mn(const Tile& t, int) { return t.kind == kDw; }
+  static __device__ __forceinline__ bool b_mn(const Tile&, int) { return true; }
+  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile& t, int) {
     return t.kind == kDw ? &p.dl_mn : &p.dl_k;
   }
-  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile& t) {
+  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile& t, int) {
     return t.kind == kDw ? &p.h : &p.w;
   }
   static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, EpiContext& c) {

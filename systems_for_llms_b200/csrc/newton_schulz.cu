@@ -9,7 +9,9 @@
 //
 // All products run on CTA-pair tensor-core tiles (pair_gemm.cuh), one launch per product for the
 // whole stack.  The two Gram-sized products are symmetric: only tiles on and above the diagonal
-// are computed, their epilogue also writes the mirrored tile.
+// are computed and stored.  Where a later product needs a tile below it, it loads the stored one
+// as an MN-major operand - the tensor cores read either orientation, step by step.  A tile on the
+// diagonal has the same rows as both operands and loads them once.
 //
 // Precision.  The quintic multiplies small singular values by 3.4 a step, and with them whatever
 // was rounded away: five steps in bf16 are off by 1 to 5 percent.  Operands are therefore fp16,
@@ -17,11 +19,11 @@
 // never exceed 1.2), far below 65504 / 4096, and their small entries stay normal numbers down to
 // 2^-26.  X itself is carried as hi + lo, two fp16 numbers with 22 bits between them, of which hi
 // is what the tensor cores multiply: a X is then exact to fp32 and the rounding of hi does not
-// compound.  In the last two steps most singular values are near 1, where a X and P X nearly
-// cancel; there P + k I and (a - k) X are used, with k = -0.75 (b + c), three quarters of -P at 1:
-// the same sum with smaller terms to round.  Sums are fp32, the norm is accumulated in 64 bits.
+// compound.  In the last two steps singular values are spread less and most are near 1, where a X
+// and P X nearly cancel; there lo is dropped and X <- (P + a I) hi, one product whose factors are
+// smaller than the terms they replace.  Sums are fp32, the norm is accumulated in 64 bits.
 // Measured against 64 bits: 1.8e-3 to 2.3e-3 of the result's norm, of which its rounding to bf16 is
-// 1.7e-3 (without k up to 2.7e-3, with hi alone up to 7e-3).
+// 1.7e-3 (hi alone throughout: up to 1e-2; a X apart in every step: up to 2.7e-3).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -75,6 +77,20 @@ __device__ __forceinline__ void load4(const T* row, int c, int n, bool vec, floa
   }
 }
 
+// A block's share of a matrix: rows r0, r0 + step, ... with its threads side by side along a row
+// (or several short rows at a time), kDepth independent loads in flight per thread.
+constexpr int kDepth = 4;
+template <class F>
+__device__ __forceinline__ void walk(int m, int quads, F&& visit) {
+  const unsigned across = quads < kNormThreads ? quads : kNormThreads;
+  const unsigned down = kNormThreads / across;
+  const unsigned r_in = threadIdx.x / across, c_in = threadIdx.x - r_in * across;
+  if (r_in >= down) return;
+  for (long r = blockIdx.x * static_cast<long>(down) + r_in; r < m;
+       r += static_cast<long>(gridDim.x) * down)
+    for (int q = c_in; q < quads; q += across * kDepth) visit(r, q, across);
+}
+
 // Sum of squares of each block's share of a matrix.  64-bit sums: squares of fp32 entries neither
 // overflow nor vanish in them.
 template <typename T>
@@ -85,16 +101,23 @@ ns_norm_kernel(Stack s, int m, int n, int vec, double* __restrict__ partial) {
   pdl_wait();
   const T* src = matrix<T>(s, blockIdx.y);
   const int quads = (n + 3) >> 2;
-  const long total = static_cast<long>(m) * quads;
   double sum = 0.0;
-  for (long i = blockIdx.x * static_cast<long>(kNormThreads) + threadIdx.x; i < total;
-       i += static_cast<long>(gridDim.x) * kNormThreads) {
-    const long r = i / quads;
-    float v[4];
-    load4(src + r * s.row, static_cast<int>(i - r * quads) * 4, n, vec, v);
+  walk(m, quads, [&](long r, int q, int across) {
+    float v[kDepth][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum = fma(static_cast<double>(v[j]), static_cast<double>(v[j]), sum);
-  }
+    for (int d = 0; d < kDepth; ++d) {
+      const int at = q + d * across;
+      load4(src + r * s.row, at < quads ? at * 4 : n, n, vec, v[d]);
+    }
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const double x = v[d][j];
+        sum = fma(x, x, sum);
+      }
+    }
+  });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = sum;
@@ -111,38 +134,48 @@ ns_norm_kernel(Stack s, int m, int n, int vec, double* __restrict__ partial) {
 template <typename T>
 __global__ void __launch_bounds__(kNormThreads)
 ns_split_kernel(Stack s, int m, int n, int ld, int vec, const double* __restrict__ partial,
-                float eps, __half* __restrict__ hi, __half* __restrict__ lo) {
+                float eps, __half* __restrict__ hi, __half* __restrict__ lo /* may be NULL */) {
   __shared__ float inv_sh;
   pdl_launch_dependents();
   pdl_wait();
   const int z = blockIdx.y;
-  if (threadIdx.x == 0) {
-    double sum = 0.0;
-    for (unsigned k = 0; k < gridDim.x; ++k) sum += partial[static_cast<long>(z) * gridDim.x + k];
-    inv_sh = static_cast<float>(kScale / (sqrt(sum) + static_cast<double>(eps)));
+  if (threadIdx.x < 32) {  // lanes add pairs of the partial sums, then each other
+    static_assert(kChunks <= 64, "two partial sums per lane");
+    const double* mine = partial + static_cast<long>(z) * gridDim.x;
+    double sum = threadIdx.x < gridDim.x ? mine[threadIdx.x] : 0.0;
+    if (threadIdx.x + 32 < gridDim.x) sum += mine[threadIdx.x + 32];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (threadIdx.x == 0) inv_sh = static_cast<float>(kScale / (sqrt(sum) + static_cast<double>(eps)));
   }
   __syncthreads();
   const float inv = inv_sh;
   const T* src = matrix<T>(s, z);
-  const int quads = ld >> 2;
-  const long total = static_cast<long>(m) * quads;
   const long out0 = static_cast<long>(z) * m * ld;
-  for (long i = blockIdx.x * static_cast<long>(kNormThreads) + threadIdx.x; i < total;
-       i += static_cast<long>(gridDim.x) * kNormThreads) {
-    const long r = i / quads;
-    const int c = static_cast<int>(i - r * quads) * 4;
-    float v[4];
-    load4(src + r * s.row, c, n, vec, v);
-    __half h[4], l[4];
+  const int quads = ld >> 2;
+  walk(m, quads, [&](long r, int q, int across) {
+    float v[kDepth][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float x = v[j] * inv;
-      h[j] = __float2half_rn(x);
-      l[j] = __float2half_rn(x - __half2float(h[j]));
+    for (int d = 0; d < kDepth; ++d) {
+      const int at = q + d * across;
+      load4(src + r * s.row, at < quads ? at * 4 : n, n, vec, v[d]);
     }
-    *reinterpret_cast<uint2*>(hi + out0 + r * ld + c) = *reinterpret_cast<const uint2*>(h);
-    *reinterpret_cast<uint2*>(lo + out0 + r * ld + c) = *reinterpret_cast<const uint2*>(l);
-  }
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      const int at = q + d * across;
+      if (at >= quads) break;
+      __half h[4], l[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float x = v[d][j] * inv;
+        h[j] = __float2half_rn(x);
+        l[j] = __float2half_rn(x - __half2float(h[j]));
+      }
+      *reinterpret_cast<uint2*>(hi + out0 + r * ld + at * 4) = *reinterpret_cast<const uint2*>(h);
+      if (lo != nullptr)
+        *reinterpret_cast<uint2*>(lo + out0 + r * ld + at * 4) = *reinterpret_cast<const uint2*>(l);
+    }
+  });
 }
 
 // ------------------------------------------------------------- Muon around it ----
@@ -204,23 +237,28 @@ dim3 rows_grid(int rows, long len) {
 }
 
 // ------------------------------------------------- symmetric products: G, b G + c G G ----
-// out = alpha aux + beta A B^T with A = B: tiles on and above the diagonal, mirrored.
+// A symmetric matrix of which the 256 x 256 tiles on and above the diagonal are stored, as an
+// operand: rows of tile `i`, reduction step kb.  Tiles below the diagonal are read transposed.
+__device__ __forceinline__ bool below(int i, int kb) { return (kb * pair::kBK) / pair::kTileN < i; }
+
+// out = alpha aux + beta A B^T (+ shift I) on and above the diagonal.  Gram matrix: A = B = X;
+// polynomial: A = B = G, aux = G.
 struct SymOp : pair::RoundRobin {
   static constexpr int kEpiTiles = 2;
   struct Params {
-    CUtensorMap a, b;
-    CUtensorMap aux, out;   // 64-column lines of 32 rows
-    CUtensorMap mirror;     // 32-column lines of 64 rows
+    CUtensorMap k_major, mn_major;  // the operand (X in one orientation, G in both)
+    CUtensorMap aux, out;           // 64-column lines of 32 rows
     int total, num_kb;
     bool fp16;
     int* status;
-    int nt, per;            // tiles along a side, tiles per matrix
-    int size;               // rows and columns of the result
-    int mn;                 // operands MN-major
-    int has_aux;
+    int nt, per;                    // tiles along a side, tiles per matrix
+    int size;                       // rows and columns of the result
+    int mn;                         // X is read MN-major
+    int gram;                       // 1: Gram matrix, 0: polynomial
     float alpha, beta;
-    float shift;            // added to the diagonal
+    float shift;                    // added to the diagonal
   };
+  // Tile::kind: 0 X K-major, 1 X MN-major, 2 G
   static __device__ __forceinline__ Tile tile(const Params& p, int w) {
     const int z = w / p.per;
     int in = w - z * p.per, i = 0;
@@ -228,52 +266,56 @@ struct SymOp : pair::RoundRobin {
       in -= p.nt - i;
       ++i;
     }
-    return Tile{i * pair::kTileM, (i + in) * pair::kTileN, z, p.num_kb, 0, p.mn};
+    return Tile{i * pair::kTileM, (i + in) * pair::kTileN, z, p.num_kb, 0, p.gram ? p.mn : 2};
   }
-  static __device__ __forceinline__ bool a_mn(const Tile& t) { return t.kind != 0; }
-  static __device__ __forceinline__ bool b_mn(const Tile& t) { return t.kind != 0; }
-  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile&) {
-    return &p.a;
+  static __device__ __forceinline__ bool a_mn(const Tile& t, int kb) {
+    return t.kind == 2 ? below(t.m0 / pair::kTileM, kb) : t.kind != 0;
   }
-  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile&) {
-    return &p.b;
+  static __device__ __forceinline__ bool b_mn(const Tile& t, int kb) {
+    return t.kind == 2 ? below(t.n0 / pair::kTileN, kb) : t.kind != 0;
   }
-  static __device__ __forceinline__ void load_aux(const Params& p, const Tile& t, EpiContext& c,
-                                                  int begin) {
-    if (c.lane == 0) {
-      tma_store_wait_read<0>();  // the tile's last store has read it
-      mbar_expect_tx(c.aux_bar, pair::kEpiTileBytes);
-      tma_load_3d(c.smem, &p.aux, c.aux_bar, begin, c.row0, t.z);
-    }
+  static __device__ __forceinline__ bool same(const Tile& t) { return t.m0 == t.n0; }
+  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile& t, int kb) {
+    return a_mn(t, kb) ? &p.mn_major : &p.k_major;
   }
+  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile& t, int kb) {
+    return b_mn(t, kb) ? &p.mn_major : &p.k_major;
+  }
+  // The warp's two 64-column chunks have a staging tile each: aux arrives in it, the result
+  // replaces it.
   static __device__ __forceinline__ void begin(const Params& p, const Tile& t, EpiContext& c) {
     const int col0 = t.n0 + c.part * 128;
-    if (p.has_aux && c.row0 < p.size && col0 < p.size) load_aux(p, t, c, col0);
+    if (p.gram || c.row0 >= p.size || col0 >= p.size || c.lane != 0) return;
+    const bool two = col0 + 64 < p.size;
+    tma_store_wait_read<0>();  // the tiles' last stores have read them
+    mbar_expect_tx(c.aux_bar, (two ? 2 : 1) * pair::kEpiTileBytes);
+    tma_load_3d(c.smem, &p.aux, c.aux_bar, col0, c.row0, t.z);
+    if (two) tma_load_3d(c.smem + pair::kEpiTileBytes, &p.aux, c.aux_bar, col0 + 64, c.row0, t.z);
   }
   static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, EpiContext& c) {
     const int col0 = t.n0 + c.part * 128;
-    if (c.row0 >= p.size) return;  // warp-uniform
-    uint8_t* mirrored = c.smem + pair::kEpiTileBytes;
-    const bool both = t.m0 != t.n0;
-    // mirrored element (row j, column lane) of 64-byte lines in their swizzle
-    uint32_t at[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      at[k] = (((static_cast<uint32_t>(c.lane) >> 3) ^ k) << 4) + (c.lane & 7) * 2;
+    if (c.row0 >= p.size || col0 >= p.size) return;  // warp-uniform
+    if (!p.gram) pair::wait_aux(c);
 #pragma unroll 1
     for (int ch = 0; ch < 2; ++ch) {
       const int begin = col0 + ch * 64;
       if (begin >= p.size) break;  // warp-uniform
-      if (p.has_aux) pair::wait_aux(c);
+      uint8_t* tile = c.smem + ch * pair::kEpiTileBytes;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float v[32];
         pair::load_acc(c.acc + c.part * 128 + ch * 64 + h * 32, v);
-        if (p.has_aux) {
+        if (p.gram) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] *= p.beta;
+          if (h == 0) {  // this tile's store is the one before the last
+            if (c.lane == 0) tma_store_wait_read<1>();
+            __syncwarp();
+          }
+        } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint4 q = *reinterpret_cast<const uint4*>(
-                pair::tile_chunk(c.smem, c.lane, 4 * h + j));
+            const uint4 q = *reinterpret_cast<const uint4*>(pair::tile_chunk(tile, c.lane, 4 * h + j));
             const __half2* e = reinterpret_cast<const __half2*>(&q);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -282,33 +324,21 @@ struct SymOp : pair::RoundRobin {
               v[8 * j + 2 * k + 1] = fmaf(v[8 * j + 2 * k + 1], p.beta, p.alpha * f.y);
             }
           }
-        } else {
+          const int diagonal = c.row0 + c.lane - begin - h * 32;
+          if (p.shift != 0.f && __any_sync(0xffffffffu, diagonal >= 0 && diagonal < 32)) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] *= p.beta;
+            for (int j = 0; j < 32; ++j)
+              if (diagonal == j) v[j] += p.shift;
+          }
         }
-        const int diagonal = c.row0 + c.lane - begin - h * 32;
-        if (p.shift != 0.f && __any_sync(0xffffffffu, diagonal >= 0 && diagonal < 32)) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (diagonal == j) v[j] += p.shift;
-        }
-        if (h == 0) pair::stage_reuse(c.lane);  // both tiles' last stores (or nothing, after a load)
-        pair::stage_16(c.smem, c.lane, h, v, true);
-        if (both) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            *reinterpret_cast<__half*>(mirrored + (h * 32 + j) * 64 + at[(j >> 1) & 3]) =
-                __float2half_rn(v[j]);
-        }
+        pair::stage_16(tile, c.lane, h, v, true);
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (c.lane == 0) {
-        pair::store_3d(&p.out, c.smem, begin, c.row0, t.z);
-        if (both) pair::store_3d(&p.mirror, mirrored, c.row0, begin, t.z);
+        pair::store_3d(&p.out, tile, begin, c.row0, t.z);
         tma_store_commit();
       }
-      if (p.has_aux && ch == 0 && begin + 64 < p.size) load_aux(p, t, c, begin + 64);
     }
   }
 };
@@ -317,7 +347,8 @@ struct SymOp : pair::RoundRobin {
 struct ApplyOp : pair::RoundRobin {
   static constexpr int kEpiTiles = 2;
   struct Params {
-    CUtensorMap a, b;
+    CUtensorMap x;                 // X: B read MN-major (wide) or A read K-major (tall)
+    CUtensorMap p_k, p_mn;         // P, symmetric, in both orientations
     CUtensorMap hi, lo;        // X as it was: 64-column lines of 32 rows; lo is rewritten in place
     CUtensorMap hi_out, out;   // the next hi, or the bf16 result
     int total, num_kb;
@@ -325,24 +356,38 @@ struct ApplyOp : pair::RoundRobin {
     int* status;
     int mt, per;
     int m, n;
+    int band;                  // row tiles that are walked before the next column tile
+    int nt;
     int wide;                  // A = P and B = X (MN-major), else A = X and B = P
+    int folded;                // 1: P holds a X as well; hi + lo of X are not read
+    int keep_lo;               // 1: write lo of the next X
     int last;                  // 0: next X, 1: result through TMA, 2: result element by element
     float alpha, beta;
     __nv_bfloat16* result;     // [batch, m, n]
   };
   static __device__ __forceinline__ Tile tile(const Params& p, int w) {
     const int z = w / p.per;
-    const int in = w - z * p.per;
-    return Tile{in % p.mt * pair::kTileM, in / p.mt * pair::kTileN, z, p.num_kb, 0, p.wide};
+    int in = w - z * p.per;
+    const int b = in / (p.band * p.nt);
+    in -= b * p.band * p.nt;
+    const int width = p.mt - b * p.band < p.band ? p.mt - b * p.band : p.band;
+    const int n = in / width;
+    return Tile{(b * p.band + in - n * width) * pair::kTileM, n * pair::kTileN, z, p.num_kb, 0,
+                p.wide};
   }
-  static __device__ __forceinline__ bool a_mn(const Tile&) { return false; }
-  static __device__ __forceinline__ bool b_mn(const Tile& t) { return t.kind != 0; }
-  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile&) {
-    return &p.a;
+  static __device__ __forceinline__ bool a_mn(const Tile& t, int kb) {
+    return t.kind != 0 && below(t.m0 / pair::kTileM, kb);
   }
-  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile&) {
-    return &p.b;
+  static __device__ __forceinline__ bool b_mn(const Tile& t, int kb) {
+    return t.kind != 0 || below(t.n0 / pair::kTileN, kb);
   }
+  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile& t, int kb) {
+    return t.kind == 0 ? &p.x : (a_mn(t, kb) ? &p.p_mn : &p.p_k);
+  }
+  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile& t, int kb) {
+    return t.kind != 0 ? &p.x : (b_mn(t, kb) ? &p.p_mn : &p.p_k);
+  }
+  static __device__ __forceinline__ bool same(const Tile&) { return false; }
   static __device__ __forceinline__ void load_aux(const Params& p, const Tile& t, EpiContext& c,
                                                   int begin) {
     if (c.lane == 0) {
@@ -354,18 +399,25 @@ struct ApplyOp : pair::RoundRobin {
   }
   static __device__ __forceinline__ void begin(const Params& p, const Tile& t, EpiContext& c) {
     const int col0 = t.n0 + c.part * 128;
-    if (c.row0 < p.m && col0 < p.n) load_aux(p, t, c, col0);
+    if (!p.folded && c.row0 < p.m && col0 < p.n) load_aux(p, t, c, col0);
   }
   static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, EpiContext& c) {
     const int col0 = t.n0 + c.part * 128;
     if (c.row0 >= p.m) return;  // warp-uniform
-    uint8_t* low = c.smem + pair::kEpiTileBytes;
     const int row = c.row0 + c.lane;
 #pragma unroll 1
     for (int ch = 0; ch < 2; ++ch) {
       const int begin = col0 + ch * 64;
       if (begin >= p.n) break;  // warp-uniform
-      pair::wait_aux(c);
+      // hi and lo of a chunk take both staging tiles; without them the chunks alternate
+      uint8_t* tile = p.folded ? c.smem + ch * pair::kEpiTileBytes : c.smem;
+      uint8_t* low = c.smem + pair::kEpiTileBytes;
+      if (p.folded) {
+        if (c.lane == 0) tma_store_wait_read<1>();
+        __syncwarp();
+      } else {
+        pair::wait_aux(c);
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float v[32];
@@ -373,9 +425,13 @@ struct ApplyOp : pair::RoundRobin {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           // each lane rewrites exactly the bytes it read
-          uint4* qh = reinterpret_cast<uint4*>(pair::tile_chunk(c.smem, c.lane, 4 * h + j));
+          uint4* qh = reinterpret_cast<uint4*>(pair::tile_chunk(tile, c.lane, 4 * h + j));
           uint4* ql = reinterpret_cast<uint4*>(pair::tile_chunk(low, c.lane, 4 * h + j));
-          uint4 a = *qh, b = *ql;
+          uint4 a = make_uint4(0, 0, 0, 0), b = a;
+          if (!p.folded) {
+            a = *qh;
+            b = *ql;
+          }
           __half2* eh = reinterpret_cast<__half2*>(&a);
           __half2* el = reinterpret_cast<__half2*>(&b);
 #pragma unroll
@@ -385,15 +441,17 @@ struct ApplyOp : pair::RoundRobin {
             const float y = fmaf(v[8 * j + 2 * k + 1], p.beta, p.alpha * (fh.y + fl.y));
             if (p.last == 0) {
               eh[k] = __floats2half2_rn(x, y);
-              const float2 r = __half22float2(eh[k]);
-              el[k] = __floats2half2_rn(x - r.x, y - r.y);
+              if (p.keep_lo) {
+                const float2 r = __half22float2(eh[k]);
+                el[k] = __floats2half2_rn(x - r.x, y - r.y);
+              }
             } else {
               const uint32_t packed = pack_bf16(x, y);
               eh[k] = *reinterpret_cast<const __half2*>(&packed);
             }
           }
           *qh = a;
-          if (p.last == 0) *ql = b;
+          if (p.keep_lo) *ql = b;
           if (p.last == 2 && row < p.m) {
             const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&a);
             const int col = begin + h * 32 + 8 * j;
@@ -408,14 +466,14 @@ struct ApplyOp : pair::RoundRobin {
       __syncwarp();
       if (c.lane == 0 && p.last != 2) {
         if (p.last == 0) {
-          pair::store_3d(&p.hi_out, c.smem, begin, c.row0, t.z);
-          pair::store_3d(&p.lo, low, begin, c.row0, t.z);
+          pair::store_3d(&p.hi_out, tile, begin, c.row0, t.z);
+          if (p.keep_lo) pair::store_3d(&p.lo, low, begin, c.row0, t.z);
         } else {
-          pair::store_3d(&p.out, c.smem, begin, c.row0, t.z);
+          pair::store_3d(&p.out, tile, begin, c.row0, t.z);
         }
         tma_store_commit();
       }
-      if (ch == 0 && begin + 64 < p.n) load_aux(p, t, c, begin + 64);
+      if (!p.folded && ch == 0 && begin + 64 < p.n) load_aux(p, t, c, begin + 64);
     }
   }
 };
@@ -518,9 +576,10 @@ extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {
   const Stack s{a->update, a->stride0, a->stride1, a->row, a->inner};
   int rc;
   const int ld = static_cast<int>(z.ld);
-  if (a->dtype == 0) rc = normalise<__nv_bfloat16>(s, batch, m, n, ld, a->eps, norms, hi[0], lo, stream);
-  else if (a->dtype == 1) rc = normalise<__half>(s, batch, m, n, ld, a->eps, norms, hi[0], lo, stream);
-  else rc = normalise<float>(s, batch, m, n, ld, a->eps, norms, hi[0], lo, stream);
+  __half* first_lo = a->steps > 2 ? lo : nullptr;  // folded steps read hi alone
+  if (a->dtype == 0) rc = normalise<__nv_bfloat16>(s, batch, m, n, ld, a->eps, norms, hi[0], first_lo, stream);
+  else if (a->dtype == 1) rc = normalise<__half>(s, batch, m, n, ld, a->eps, norms, hi[0], first_lo, stream);
+  else rc = normalise<float>(s, batch, m, n, ld, a->eps, norms, hi[0], first_lo, stream);
   if (rc != 0) return rc;
 
   const uint64_t x_stride = static_cast<uint64_t>(m) * z.ld;
@@ -541,6 +600,8 @@ extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {
   x.per = mt * nt;
   x.total = batch * x.per;
   x.num_kb = tiles_of(side, pair::kBK);
+  x.nt = nt;
+  x.band = mt < 8 ? mt : 8;
   x.m = m;
   x.n = n;
   x.wide = wide;
@@ -551,12 +612,11 @@ extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {
   auto gram_map = [&](CUtensorMap* map, __half* g) {
     return pair::map_3d(map, g, 2, side, side, z.gram_ld, batch, g_stride, 64, 32);
   };
-  auto mirror_map = [&](CUtensorMap* map, __half* g) {
-    const uint64_t dims[3] = {static_cast<uint64_t>(side), static_cast<uint64_t>(side),
-                              static_cast<uint64_t>(batch)};
-    const uint64_t strides[3] = {0, static_cast<uint64_t>(z.gram_ld) * 2, g_stride * 2};
-    const uint32_t box[3] = {32, 64, 1};
-    return make_tensormap_nd(map, g, 2, 3, dims, strides, box, 2);
+  // G and P as operands, in both orientations
+  auto symmetric = [&](CUtensorMap* k_major, CUtensorMap* mn_major, __half* g) {
+    const int bad = pair::map_operand(k_major, g, false, side, side, z.gram_ld, batch, g_stride);
+    return bad != 0 ? bad
+                    : pair::map_operand(mn_major, g, true, side, side, z.gram_ld, batch, g_stride);
   };
   auto x_map = [&](CUtensorMap* map, __half* v) {
     return pair::map_3d(map, v, 2, n, m, z.ld, batch, x_stride, 64, 32);
@@ -566,33 +626,29 @@ extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {
     __half* now = hi[step & 1];
     __half* next = hi[(step + 1) & 1];
     // G = X X^T (wide: X is K-major) or X^T X (tall: X read MN-major)
+    q.gram = 1;
     q.mn = !wide;
     q.num_kb = tiles_of(longer, pair::kBK);
-    q.has_aux = 0;
     q.alpha = 0.f;
     q.beta = 1.0f / kScale;
     q.shift = 0.f;
-    rc = pair::map_operand(&q.a, now, !wide, side, longer, z.ld, batch, x_stride);
-    q.b = q.a;
+    rc = pair::map_operand(wide ? &q.k_major : &q.mn_major, now, !wide, side, longer, z.ld, batch,
+                           x_stride);
     if (rc == 0) rc = gram_map(&q.out, gram);
-    if (rc == 0) rc = mirror_map(&q.mirror, gram);
     if (rc != 0) return 1000 + rc;
-    q.aux = q.out;
     rc = pair::launch_pair<SymOp>(q, stream);
     if (rc != 0) return rc;
-    // P = b G + c G G (+ k I)
-    const float k = step + 2 >= a->steps && a->b + a->c < 0.f ? -0.75f * (a->b + a->c) : 0.f;
-    q.shift = k * kScale;
-    q.mn = 0;
+    // P = b G + c G G (+ a I)
+    const bool folded = step + 2 >= a->steps;
+    const float k = folded ? a->a : 0.f;
+    q.gram = 0;
     q.num_kb = tiles_of(side, pair::kBK);
-    q.has_aux = 1;
     q.alpha = a->b;
     q.beta = a->c / kScale;
+    q.shift = k * kScale;
     q.aux = q.out;
-    rc = pair::map_operand(&q.a, gram, false, side, side, z.gram_ld, batch, g_stride);
-    q.b = q.a;
+    rc = symmetric(&q.k_major, &q.mn_major, gram);
     if (rc == 0) rc = gram_map(&q.out, poly);
-    if (rc == 0) rc = mirror_map(&q.mirror, poly);
     if (rc != 0) return 1000 + rc;
     rc = pair::launch_pair<SymOp>(q, stream);
     if (rc != 0) return rc;
@@ -600,15 +656,14 @@ extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {
     const bool last = step + 1 == a->steps;
     x.last = !last ? 0 : (out_tma ? 1 : 2);
     const float unscale = last ? 1.0f / kScale : 1.0f;
+    x.folded = folded;
+    x.keep_lo = step + 3 < a->steps;  // the next step is not folded either
     x.alpha = (a->a - k) * unscale;
     x.beta = unscale / kScale;
-    if (wide) {
-      rc = pair::map_operand(&x.a, poly, false, side, side, z.gram_ld, batch, g_stride);
-      if (rc == 0) rc = pair::map_operand(&x.b, now, true, n, m, z.ld, batch, x_stride);
-    } else {
-      rc = pair::map_operand(&x.a, now, false, m, n, z.ld, batch, x_stride);
-      if (rc == 0) rc = pair::map_operand(&x.b, poly, false, side, side, z.gram_ld, batch, g_stride);
-    }
+    rc = symmetric(&x.p_k, &x.p_mn, poly);
+    if (rc == 0)
+      rc = wide ? pair::map_operand(&x.x, now, true, n, m, z.ld, batch, x_stride)
+                : pair::map_operand(&x.x, now, false, m, n, z.ld, batch, x_stride);
     if (rc == 0) rc = x_map(&x.hi, now);
     if (rc == 0) rc = x_map(&x.lo, lo);
     if (rc == 0) rc = x_map(&x.hi_out, next);

@@ -22,8 +22,9 @@
 //   static int  Op::first(p, cluster), Op::next(p, w, cluster, clusters)
 //                                  the cluster's first tile and the one after w (>= total: none)
 //   static Tile Op::tile(p, w)     where the tile lies
-//   static bool Op::a_mn(t), Op::b_mn(t)  MN-major operands (see gemm.cu)
-//   static const CUtensorMap* Op::map_a(p, t), Op::map_b(p, t)   rank-3 {inner, rows, batch}
+//   static bool Op::a_mn(t, kb), Op::b_mn(t, kb)  MN-major operands (see gemm.cu), step by step
+//   static const CUtensorMap* Op::map_a(p, t, kb), Op::map_b(p, t, kb)  rank-3 {inner, rows, batch}
+//   static bool Op::same(t)        B's rows are A's: one copy serves as both operands
 //   static constexpr int Op::kEpiTiles           staging tiles per epilogue warp, 1 or 2
 //   static void Op::begin(p, t, EpiContext&)     before the accumulator is ready (prefetches)
 //   static void Op::epilogue(p, t, EpiContext&)  one warp's share of the tile
@@ -193,6 +194,7 @@ __device__ __forceinline__ void wait_aux(EpiContext& c) {
 // Bases for Ops whose epilogue loads nothing of its own, and whose tiles are dealt round robin.
 struct Plain {
   static constexpr int kEpiTiles = 1;
+  static __device__ __forceinline__ bool same(const Tile&) { return false; }
   template <class P, class C>
   static __device__ __forceinline__ void begin(const P&, const Tile&, C&) {}
 };
@@ -304,8 +306,6 @@ pair_kernel(const __grid_constant__ typename Op::Params p) {
       bool ok = true;
       for (int w = Op::first(p, cluster); w < p.total && ok; w = Op::next(p, w, cluster, clusters)) {
         const Tile t = Op::tile(p, w);
-        const CUtensorMap* ma = Op::map_a(p, t);
-        const CUtensorMap* mb = Op::map_b(p, t);
         const int m0 = t.m0 + rank * kCtaM;
         const int n0 = t.n0 + rank * kHalfN;
         for (int kb = 0; kb < t.num_kb; ++kb) {
@@ -318,15 +318,20 @@ pair_kernel(const __grid_constant__ typename Op::Params p) {
           uint8_t* sa = smem + stage * kStageBytes;
           uint8_t* sb = sa + kABytes;
           const uint32_t bar = in_leader(smem_u32(&bars->full[stage]));
-          if (rank == 0) mbar_expect_tx(&bars->full[stage], 2 * kStageBytes);
+          const bool same = Op::same(t);
+          if (rank == 0)
+            mbar_expect_tx(&bars->full[stage], 2 * (same ? kABytes : kStageBytes));
           const int k0 = (t.kb0 + kb) * kBK;
-          if (Op::a_mn(t)) {
+          const CUtensorMap* ma = Op::map_a(p, t, kb);
+          const CUtensorMap* mb = Op::map_b(p, t, kb);
+          if (Op::a_mn(t, kb)) {
             load_3d(sa, ma, bar, m0, k0, t.z);
             load_3d(sa + kBK * 128, ma, bar, m0 + 64, k0, t.z);
           } else {
             load_3d(sa, ma, bar, k0, m0, t.z);
           }
-          if (Op::b_mn(t)) {
+          if (same) {
+          } else if (Op::b_mn(t, kb)) {
             load_3d(sb, mb, bar, n0, k0, t.z);
             load_3d(sb + kBK * 128, mb, bar, n0 + 64, k0, t.z);
           } else {
@@ -352,19 +357,13 @@ pair_kernel(const __grid_constant__ typename Op::Params p) {
     // -------------------------------------------------------- MMA issuer ----
     // The leader's warp walks converged; one elected lane issues (see gemm.cu).
     if (rank == 0) {
-      const uint32_t base = smem_u32(smem);
+      const uint64_t k0 = umma_smem_desc(smem_u32(smem), 16, 1024);           // K-major
+      const uint64_t mn0 = umma_smem_desc(smem_u32(smem), kBK * 128, 1024);   // MN-major
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
       for (int w = Op::first(p, cluster); w < p.total && ok; w = Op::next(p, w, cluster, clusters)) {
         const Tile t = Op::tile(p, w);
-        const bool a_mn = Op::a_mn(t), b_mn = Op::b_mn(t);
-        const uint64_t a0 = a_mn ? umma_smem_desc(base, kBK * 128, 1024)
-                                 : umma_smem_desc(base, 16, 1024);
-        const uint64_t b0 = b_mn ? umma_smem_desc(base + kABytes, kBK * 128, 1024)
-                                 : umma_smem_desc(base + kABytes, 16, 1024);
-        const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
-        const uint32_t idesc = instruction_descriptor(p.fp16, a_mn, b_mn);
         if (!wait_or_leave(&bars->acc_empty[acc], acc_phase ^ 1, abort)) {
           report_status(p.status, kStatusTimeoutTmemEmpty);
           *abort = 1;
@@ -380,8 +379,12 @@ pair_kernel(const __grid_constant__ typename Op::Params p) {
             break;
           }
           tc_fence_after();
-          const uint64_t a = umma_desc_advance(a0, stage * kStageBytes);
-          const uint64_t b = umma_desc_advance(b0, stage * kStageBytes);
+          const bool a_mn = Op::a_mn(t, kb), b_mn = Op::b_mn(t, kb);
+          const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
+          const uint32_t idesc = instruction_descriptor(p.fp16, a_mn, b_mn);
+          const uint64_t a = umma_desc_advance(a_mn ? mn0 : k0, stage * kStageBytes);
+          const uint64_t b =
+              umma_desc_advance(b_mn ? mn0 : k0, stage * kStageBytes + (Op::same(t) ? 0 : kABytes));
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < kBK / 16; ++k)

@@ -1,8 +1,8 @@
 """Newton-Schulz orthogonalisation against the formula in 64 bits (needs a B200).
 
 Tolerance.  Let u = 2^-11 (half a step of fp16), s the shorter side, F the Frobenius norm.  A step
-rounds hi (dX = u |X|F), the Gram matrix (dG = u |G|F, and X dX^T twice), P = b G + c G G + k I
-(dP = (|b| + 2 |c| |G|) dG + u |P|F) and multiplies: dP X and P dX.  hi + lo keep X to 2^-21 of each entry and,
+rounds hi (dX = u |X|F), the Gram matrix (dG = u |G|F, and X dX^T twice), P = b G + c G G, in the
+last two steps with a I added and hi standing for X (dP = (|b| + 2 |c| |G|) dG + u |P|F) and multiplies: dP X and P dX.  hi + lo keep X to 2^-21 of each entry and,
 since fp16 numbers are at least 2^-24 apart and X is held times 2^12, to 2^-37 absolutely (half of
 2^-24 over 2^12; it matters where eps dwarfs the norm: X is then far below 1).  Sums of K products in fp32 add K 2^-24 of the product of the norms (rms: the root of K).  What a step leaves is carried by the
 steps after it: in the singular basis of that step's X entry (i, j) of an error is multiplied by
@@ -95,7 +95,7 @@ def exact(update, steps=5, coefficients=QUINTIC, eps=1e-7):
         if step < 0:
             errors.append(start * carried(x, after, typical))
             continue
-        k = max(0.0, -0.75 * (b + c)) if step + 2 >= steps else 0.0
+        k = a if step + 2 >= steps else 0.0
         g = x @ x.t()
         p = b * g + c * g @ g + k * torch.eye(s, dtype=x.dtype, device=x.device)
         # |A d| = act(A) |d|
