@@ -31,6 +31,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "launch.cuh"
 #include "ptx.cuh"
 #include "tensormap.cuh"
@@ -379,20 +381,35 @@ pair_kernel(const __grid_constant__ typename Op::Params p) {
             break;
           }
           tc_fence_after();
-          const bool a_mn = Op::a_mn(t, kb), b_mn = Op::b_mn(t, kb);
-          const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
-          const uint32_t idesc = instruction_descriptor(p.fp16, a_mn, b_mn);
-          const uint64_t a = umma_desc_advance(a_mn ? mn0 : k0, stage * kStageBytes);
-          const uint64_t b =
-              umma_desc_advance(b_mn ? mn0 : k0, stage * kStageBytes + (Op::same(t) ? 0 : kABytes));
-          if (elect_one()) {
+          // Each orientation has code of its own: descriptors are then the sum of warp-uniform
+          // values and stay in uniform registers.  Chosen by arithmetic on the tile they would be
+          // moved there for every product, which the issuing lane has no time for.
+          auto issue = [&](auto a_mn, auto b_mn, uint32_t b_at) {
+            constexpr bool kA = decltype(a_mn)::value, kB = decltype(b_mn)::value;
+            const uint64_t a = umma_desc_advance(kA ? mn0 : k0, stage * kStageBytes);
+            const uint64_t b = umma_desc_advance(kB ? mn0 : k0, stage * kStageBytes + b_at);
+            const uint32_t idesc = instruction_descriptor(p.fp16, kA, kB);
+            if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < kBK / 16; ++k)
-              mma_pair(d, umma_desc_advance(a, k * a_step), umma_desc_advance(b, k * b_step), idesc,
-                       (kb | k) != 0);
-            commit_pair(&bars->empty[stage]);
-            if (kb == t.num_kb - 1) commit_pair(&bars->acc_full[acc]);
+              for (int k = 0; k < kBK / 16; ++k)
+                mma_pair(d, umma_desc_advance(a, k * (kA ? 2048 : 32)),
+                         umma_desc_advance(b, k * (kB ? 2048 : 32)), idesc, (kb | k) != 0);
+              commit_pair(&bars->empty[stage]);
+            }
+          };
+          const std::true_type mn;
+          const std::false_type km;
+          if (Op::same(t)) {
+            if (Op::a_mn(t, kb)) issue(mn, mn, 0);
+            else issue(km, km, 0);
+          } else if (Op::a_mn(t, kb)) {
+            if (Op::b_mn(t, kb)) issue(mn, mn, kABytes);
+            else issue(mn, km, kABytes);
+          } else {
+            if (Op::b_mn(t, kb)) issue(km, mn, kABytes);
+            else issue(km, km, kABytes);
           }
+          if (kb == t.num_kb - 1 && elect_one()) commit_pair(&bars->acc_full[acc]);
           __syncwarp();
           if (++stage == kStages) {
             stage = 0;
