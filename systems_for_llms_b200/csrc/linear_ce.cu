@@ -63,7 +63,7 @@ __device__ __forceinline__ void grid_tile(const Grid& g, int w, int* m, int* n) 
 }
 
 // ---------------------------------------------------- row statistics (forward) ----
-struct StatsOp : pair::Plain, pair::RoundRobin {
+struct StatsOp : pair::NoMaps, pair::Plain, pair::RoundRobin {
   struct Params {
     CUtensorMap a, b;
     Grid grid;
@@ -75,12 +75,11 @@ struct StatsOp : pair::Plain, pair::RoundRobin {
     float* picked;     // [rows]: the target's logit
     int rows, vocab;
   };
-  static __device__ __forceinline__ bool a_mn(const Tile&, int) { return false; }
-  static __device__ __forceinline__ bool b_mn(const Tile&, int) { return false; }
-  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile&, int) {
+  static constexpr int kForms = pair::kFormKK;
+  static __device__ __forceinline__ const CUtensorMap* map_a_k(const Params& p, const Tile&) {
     return &p.a;
   }
-  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile&, int) {
+  static __device__ __forceinline__ const CUtensorMap* map_b_k(const Params& p, const Tile&) {
     return &p.b;
   }
   static __device__ __forceinline__ Tile tile(const Params& p, int w) {
@@ -230,7 +229,7 @@ ce_total_kernel(const float* __restrict__ row_loss, const int64_t* __restrict__ 
 }
 
 // --------------------------------------------- dl of a piece of the vocabulary ----
-struct DlogitsOp : pair::Plain, pair::RoundRobin {
+struct DlogitsOp : pair::NoMaps, pair::Plain, pair::RoundRobin {
   struct Params {
     CUtensorMap a, b, out;
     Grid grid;
@@ -242,12 +241,11 @@ struct DlogitsOp : pair::Plain, pair::RoundRobin {
     float one;           // 1, or 2^12 for fp16
     int rows, vocab_begin, width;
   };
-  static __device__ __forceinline__ bool a_mn(const Tile&, int) { return false; }
-  static __device__ __forceinline__ bool b_mn(const Tile&, int) { return false; }
-  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile&, int) {
+  static constexpr int kForms = pair::kFormKK;
+  static __device__ __forceinline__ const CUtensorMap* map_a_k(const Params& p, const Tile&) {
     return &p.a;
   }
-  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile&, int) {
+  static __device__ __forceinline__ const CUtensorMap* map_b_k(const Params& p, const Tile&) {
     return &p.b;
   }
   static __device__ __forceinline__ Tile tile(const Params& p, int w) {
@@ -321,7 +319,7 @@ __device__ __forceinline__ float grad_scale(const GradScale& g) {
 constexpr int kMaxClusters = 96;
 enum Product : int { kDw = 0, kDh = 1 };
 
-struct GradOp : pair::Plain {
+struct GradOp : pair::NoMaps, pair::Plain {
   struct Params {
     CUtensorMap dl_mn, dl_k, h, w, dw, dh;
     int total, dh_tiles;         // dh's tiles are the first of each cluster's range
@@ -359,12 +357,16 @@ struct GradOp : pair::Plain {
     return Tile{w % p.dh_mt * pair::kTileM, w / p.dh_mt * pair::kTileN, 0,
                 left < p.dh_part_kb ? left : p.dh_part_kb, kb0, kDh + 2 * part};
   }
-  static __device__ __forceinline__ bool a_mn(const Tile& t, int) { return t.kind == kDw; }
+  static constexpr int kForms = pair::kFormMM | pair::kFormKM;
+  static __device__ __forceinline__ bool a_mn(const Tile& t, int) { return (t.kind & 1) == kDw; }
   static __device__ __forceinline__ bool b_mn(const Tile&, int) { return true; }
-  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile& t, int) {
-    return t.kind == kDw ? &p.dl_mn : &p.dl_k;
+  static __device__ __forceinline__ const CUtensorMap* map_a_mn(const Params& p, const Tile&) {
+    return &p.dl_mn;
   }
-  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile& t, int) {
+  static __device__ __forceinline__ const CUtensorMap* map_a_k(const Params& p, const Tile&) {
+    return &p.dl_k;
+  }
+  static __device__ __forceinline__ const CUtensorMap* map_b_mn(const Params& p, const Tile& t) {
     return t.kind == kDw ? &p.h : &p.w;
   }
   static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, EpiContext& c) {

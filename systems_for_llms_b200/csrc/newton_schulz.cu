@@ -243,7 +243,7 @@ __device__ __forceinline__ bool below(int i, int kb) { return (kb * pair::kBK) /
 
 // out = alpha aux + beta A B^T (+ shift I) on and above the diagonal.  Gram matrix: A = B = X;
 // polynomial: A = B = G, aux = G.
-struct SymOp : pair::RoundRobin {
+struct SymOp : pair::NoMaps, pair::RoundRobin {
   static constexpr int kEpiTiles = 2;
   struct Params {
     CUtensorMap k_major, mn_major;  // the operand (X in one orientation, G in both)
@@ -275,11 +275,19 @@ struct SymOp : pair::RoundRobin {
     return t.kind == 2 ? below(t.n0 / pair::kTileN, kb) : t.kind != 0;
   }
   static __device__ __forceinline__ bool same(const Tile& t) { return t.m0 == t.n0; }
-  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile& t, int kb) {
-    return a_mn(t, kb) ? &p.mn_major : &p.k_major;
+  static constexpr int kForms =
+      pair::kFormKK | pair::kFormMM | pair::kFormKM | pair::kFormMK | pair::kFormSame;
+  static __device__ __forceinline__ const CUtensorMap* map_a_k(const Params& p, const Tile&) {
+    return &p.k_major;
   }
-  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile& t, int kb) {
-    return b_mn(t, kb) ? &p.mn_major : &p.k_major;
+  static __device__ __forceinline__ const CUtensorMap* map_b_k(const Params& p, const Tile&) {
+    return &p.k_major;
+  }
+  static __device__ __forceinline__ const CUtensorMap* map_a_mn(const Params& p, const Tile&) {
+    return &p.mn_major;
+  }
+  static __device__ __forceinline__ const CUtensorMap* map_b_mn(const Params& p, const Tile&) {
+    return &p.mn_major;
   }
   // The warp's two 64-column chunks have a staging tile each: aux arrives in it, the result
   // replaces it.
@@ -344,7 +352,7 @@ struct SymOp : pair::RoundRobin {
 };
 
 // ------------------------------------------------------------ X <- a X + P X ----
-struct ApplyOp : pair::RoundRobin {
+struct ApplyOp : pair::NoMaps, pair::RoundRobin {
   static constexpr int kEpiTiles = 2;
   struct Params {
     CUtensorMap x;                 // X: B read MN-major (wide) or A read K-major (tall)
@@ -381,13 +389,20 @@ struct ApplyOp : pair::RoundRobin {
   static __device__ __forceinline__ bool b_mn(const Tile& t, int kb) {
     return t.kind != 0 || below(t.n0 / pair::kTileN, kb);
   }
-  static __device__ __forceinline__ const CUtensorMap* map_a(const Params& p, const Tile& t, int kb) {
-    return t.kind == 0 ? &p.x : (a_mn(t, kb) ? &p.p_mn : &p.p_k);
+  // wide: A = P in either orientation, B = X MN-major; tall: A = X K-major, B = P in either
+  static constexpr int kForms = pair::kFormKK | pair::kFormMM | pair::kFormKM;
+  static __device__ __forceinline__ const CUtensorMap* map_a_k(const Params& p, const Tile& t) {
+    return t.kind != 0 ? &p.p_k : &p.x;
   }
-  static __device__ __forceinline__ const CUtensorMap* map_b(const Params& p, const Tile& t, int kb) {
-    return t.kind != 0 ? &p.x : (b_mn(t, kb) ? &p.p_mn : &p.p_k);
+  static __device__ __forceinline__ const CUtensorMap* map_a_mn(const Params& p, const Tile&) {
+    return &p.p_mn;
   }
-  static __device__ __forceinline__ bool same(const Tile&) { return false; }
+  static __device__ __forceinline__ const CUtensorMap* map_b_k(const Params& p, const Tile&) {
+    return &p.p_k;
+  }
+  static __device__ __forceinline__ const CUtensorMap* map_b_mn(const Params& p, const Tile& t) {
+    return t.kind != 0 ? &p.x : &p.p_mn;
+  }
   static __device__ __forceinline__ void load_aux(const Params& p, const Tile& t, EpiContext& c,
                                                   int begin) {
     if (c.lane == 0) {

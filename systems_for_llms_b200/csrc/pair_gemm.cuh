@@ -23,7 +23,9 @@
 //                                  the cluster's first tile and the one after w (>= total: none)
 //   static Tile Op::tile(p, w)     where the tile lies
 //   static bool Op::a_mn(t, kb), Op::b_mn(t, kb)  MN-major operands (see gemm.cu), step by step
-//   static const CUtensorMap* Op::map_a(p, t, kb), Op::map_b(p, t, kb)  rank-3 {inner, rows, batch}
+//   static constexpr int Op::kForms  the combinations of orientations that occur
+//   static const CUtensorMap* Op::map_a_k(p, t), map_a_mn, map_b_k, map_b_mn   rank-3 maps
+//                                    {inner, rows, batch} of the orientations that occur
 //   static bool Op::same(t)        B's rows are A's: one copy serves as both operands
 //   static constexpr int Op::kEpiTiles           staging tiles per epilogue warp, 1 or 2
 //   static void Op::begin(p, t, EpiContext&)     before the accumulator is ready (prefetches)
@@ -193,10 +195,20 @@ __device__ __forceinline__ void wait_aux(EpiContext& c) {
   c.aux_phase ^= 1;
 }
 
+// Names for the orientations that an Op does not use.
+struct NoMaps {
+  template <class P> static __device__ const CUtensorMap* map_a_k(const P&, const Tile&) { return nullptr; }
+  template <class P> static __device__ const CUtensorMap* map_a_mn(const P&, const Tile&) { return nullptr; }
+  template <class P> static __device__ const CUtensorMap* map_b_k(const P&, const Tile&) { return nullptr; }
+  template <class P> static __device__ const CUtensorMap* map_b_mn(const P&, const Tile&) { return nullptr; }
+  static __device__ __forceinline__ bool a_mn(const Tile&, int) { return false; }
+  static __device__ __forceinline__ bool b_mn(const Tile&, int) { return false; }
+  static __device__ __forceinline__ bool same(const Tile&) { return false; }
+};
+
 // Bases for Ops whose epilogue loads nothing of its own, and whose tiles are dealt round robin.
 struct Plain {
   static constexpr int kEpiTiles = 1;
-  static __device__ __forceinline__ bool same(const Tile&) { return false; }
   template <class P, class C>
   static __device__ __forceinline__ void begin(const P&, const Tile&, C&) {}
 };
@@ -254,6 +266,45 @@ __device__ __forceinline__ void load_acc(uint32_t addr, float (&v)[32]) {
   for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
 }
 
+// Calls f(a_mn, b_mn, only_a) with constants for the step's orientations; only the combinations
+// that Op::kForms names are compiled.
+enum Form : int {
+  kFormKK = 1, kFormMM = 2, kFormKM = 4, kFormMK = 8,  // A and B K-major / MN-major
+  kFormSame = 16,                                      // KK and MM also with one copy for both
+};
+template <class Op, class F>
+__device__ __forceinline__ void by_orientation(const Tile& t, int kb, F&& f) {
+  const std::true_type yes;
+  const std::false_type no;
+  constexpr int kForms = Op::kForms;
+  if constexpr ((kForms & kFormSame) != 0) {
+    if (Op::same(t)) {
+      if ((kForms & kFormMM) != 0 && Op::a_mn(t, kb)) f(yes, yes, yes);
+      else f(no, no, yes);
+      return;
+    }
+  }
+  if constexpr (kForms == kFormKK) {
+    f(no, no, no);
+  } else if constexpr (kForms == kFormMM) {
+    f(yes, yes, no);
+  } else {
+    const bool a = Op::a_mn(t, kb), b = Op::b_mn(t, kb);
+    if constexpr ((kForms & kFormKK) != 0) {
+      if (!a && !b) f(no, no, no);
+    }
+    if constexpr ((kForms & kFormMM) != 0) {
+      if (a && b) f(yes, yes, no);
+    }
+    if constexpr ((kForms & kFormKM) != 0) {
+      if (!a && b) f(no, yes, no);
+    }
+    if constexpr ((kForms & kFormMK) != 0) {
+      if (a && !b) f(yes, no, no);
+    }
+  }
+}
+
 // ----------------------------------------------------------------- kernel ----
 template <class Op>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
@@ -302,57 +353,64 @@ pair_kernel(const __grid_constant__ typename Op::Params p) {
 
   if (warp == 0) {
     // ------------------------------------------------------ TMA producer ----
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int w = Op::first(p, cluster); w < p.total && ok; w = Op::next(p, w, cluster, clusters)) {
-        const Tile t = Op::tile(p, w);
-        const int m0 = t.m0 + rank * kCtaM;
-        const int n0 = t.n0 + rank * kHalfN;
-        for (int kb = 0; kb < t.num_kb; ++kb) {
-          if (!wait_or_leave(&bars->empty[stage], phase ^ 1, abort)) {
-            report_status(p.status, kStatusTimeoutEmpty);
-            *abort = 1;
-            ok = false;
-            break;
-          }
-          uint8_t* sa = smem + stage * kStageBytes;
-          uint8_t* sb = sa + kABytes;
-          const uint32_t bar = in_leader(smem_u32(&bars->full[stage]));
-          const bool same = Op::same(t);
-          if (rank == 0)
-            mbar_expect_tx(&bars->full[stage], 2 * (same ? kABytes : kStageBytes));
-          const int k0 = (t.kb0 + kb) * kBK;
-          const CUtensorMap* ma = Op::map_a(p, t, kb);
-          const CUtensorMap* mb = Op::map_b(p, t, kb);
-          if (Op::a_mn(t, kb)) {
-            load_3d(sa, ma, bar, m0, k0, t.z);
-            load_3d(sa + kBK * 128, ma, bar, m0 + 64, k0, t.z);
-          } else {
-            load_3d(sa, ma, bar, k0, m0, t.z);
-          }
-          if (same) {
-          } else if (Op::b_mn(t, kb)) {
-            load_3d(sb, mb, bar, n0, k0, t.z);
-            load_3d(sb + kBK * 128, mb, bar, n0 + 64, k0, t.z);
-          } else {
-            load_3d(sb, mb, bar, k0, n0, t.z);
-          }
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
+    // The whole warp walks the loops and one elected lane issues, with code of its own for each
+    // orientation, for the reason given at the MMA issuer: the operands of a TMA instruction are
+    // uniform registers too, and a lane that has to move coordinates and map addresses there takes
+    // 770 cycles per step where the products take 512.
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const uint32_t full0 = in_leader(smem_u32(&bars->full[0]));
+    for (int w = Op::first(p, cluster); w < p.total && ok; w = Op::next(p, w, cluster, clusters)) {
+      const Tile t = Op::tile(p, w);
+      const int m0 = t.m0 + rank * kCtaM;
+      const int n0 = t.n0 + rank * kHalfN;
+      for (int kb = 0; kb < t.num_kb; ++kb) {
+        if (!wait_or_leave(&bars->empty[stage], phase ^ 1, abort)) {
+          if (lane == 0) report_status(p.status, kStatusTimeoutEmpty);
+          *abort = 1;
+          ok = false;
+          break;
         }
-      }
-      // Leave only when every stage has been handed back: no commit from the leader and no copy
-      // is then still on its way into this CTA's shared memory.
-      for (int s = 0; s < kStages; ++s) {
-        if (!mbar_wait(&bars->empty[stage], phase ^ 1)) break;
+        uint8_t* sa = smem + stage * kStageBytes;
+        const uint32_t bar = full0 + stage * static_cast<uint32_t>(sizeof(uint64_t));
+        const int k0 = (t.kb0 + kb) * kBK;
+        auto bring = [&](auto a_mn, auto b_mn, auto only_a) {
+          if (elect_one()) {
+            if (rank == 0)
+              mbar_expect_tx(&bars->full[stage],
+                             2 * (decltype(only_a)::value ? kABytes : kStageBytes));
+            if constexpr (decltype(a_mn)::value) {
+              load_3d(sa, Op::map_a_mn(p, t), bar, m0, k0, t.z);
+              load_3d(sa + kBK * 128, Op::map_a_mn(p, t), bar, m0 + 64, k0, t.z);
+            } else {
+              load_3d(sa, Op::map_a_k(p, t), bar, k0, m0, t.z);
+            }
+            if constexpr (!decltype(only_a)::value) {
+              if constexpr (decltype(b_mn)::value) {
+                load_3d(sa + kABytes, Op::map_b_mn(p, t), bar, n0, k0, t.z);
+                load_3d(sa + kABytes + kBK * 128, Op::map_b_mn(p, t), bar, n0 + 64, k0, t.z);
+              } else {
+                load_3d(sa + kABytes, Op::map_b_k(p, t), bar, k0, n0, t.z);
+              }
+            }
+          }
+          __syncwarp();
+        };
+        by_orientation<Op>(t, kb, bring);
         if (++stage == kStages) {
           stage = 0;
           phase ^= 1;
         }
+      }
+    }
+    // Leave only when every stage has been handed back: no commit from the leader and no copy
+    // is then still on its way into this CTA's shared memory.
+    for (int s = 0; s < kStages; ++s) {
+      if (!mbar_wait(&bars->empty[stage], phase ^ 1)) break;
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1;
       }
     }
   } else if (warp == 1) {
@@ -384,8 +442,9 @@ pair_kernel(const __grid_constant__ typename Op::Params p) {
           // Each orientation has code of its own: descriptors are then the sum of warp-uniform
           // values and stay in uniform registers.  Chosen by arithmetic on the tile they would be
           // moved there for every product, which the issuing lane has no time for.
-          auto issue = [&](auto a_mn, auto b_mn, uint32_t b_at) {
+          auto issue = [&](auto a_mn, auto b_mn, auto only_a) {
             constexpr bool kA = decltype(a_mn)::value, kB = decltype(b_mn)::value;
+            constexpr uint32_t b_at = decltype(only_a)::value ? 0 : kABytes;
             const uint64_t a = umma_desc_advance(kA ? mn0 : k0, stage * kStageBytes);
             const uint64_t b = umma_desc_advance(kB ? mn0 : k0, stage * kStageBytes + b_at);
             const uint32_t idesc = instruction_descriptor(p.fp16, kA, kB);
@@ -397,18 +456,7 @@ pair_kernel(const __grid_constant__ typename Op::Params p) {
               commit_pair(&bars->empty[stage]);
             }
           };
-          const std::true_type mn;
-          const std::false_type km;
-          if (Op::same(t)) {
-            if (Op::a_mn(t, kb)) issue(mn, mn, 0);
-            else issue(km, km, 0);
-          } else if (Op::a_mn(t, kb)) {
-            if (Op::b_mn(t, kb)) issue(mn, mn, kABytes);
-            else issue(mn, km, kABytes);
-          } else {
-            if (Op::b_mn(t, kb)) issue(km, mn, kABytes);
-            else issue(km, km, kABytes);
-          }
+          by_orientation<Op>(t, kb, issue);
           if (kb == t.num_kb - 1 && elect_one()) commit_pair(&bars->acc_full[acc]);
           __syncwarp();
           if (++stage == kStages) {
