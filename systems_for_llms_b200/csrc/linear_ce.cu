@@ -85,7 +85,7 @@ struct StatsOp : pair::NoMaps, pair::Plain, pair::RoundRobin {
   static __device__ __forceinline__ Tile tile(const Params& p, int w) {
     int m, n;
     grid_tile(p.grid, w, &m, &n);
-    return Tile{m * pair::kTileM, n * pair::kTileN, 0, p.num_kb, 0, 0};
+    return Tile{m * pair::kTileM, n * pair::kTileN, 0, p.num_kb, 0, 0, 0, 0, false};
   }
   static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, EpiContext& c) {
     const int row = c.row0 + c.lane;
@@ -251,7 +251,7 @@ struct DlogitsOp : pair::NoMaps, pair::Plain, pair::RoundRobin {
   static __device__ __forceinline__ Tile tile(const Params& p, int w) {
     int m, n;
     grid_tile(p.grid, w, &m, &n);
-    return Tile{m * pair::kTileM, n * pair::kTileN, 0, p.num_kb, 0, 0};
+    return Tile{m * pair::kTileM, n * pair::kTileN, 0, p.num_kb, 0, 0, 0, 0, false};
   }
   static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, EpiContext& c) {
     const int row = c.row0 + c.lane;
@@ -347,7 +347,8 @@ struct GradOp : pair::NoMaps, pair::Plain {
   static __device__ __forceinline__ Tile tile(const Params& p, int w) {
     if (w >= p.dh_tiles) {
       w -= p.dh_tiles;
-      return Tile{w % p.dw_mt * pair::kTileM, w / p.dw_mt * pair::kTileN, 0, p.dw_kb, 0, kDw};
+      return Tile{w % p.dw_mt * pair::kTileM, w / p.dw_mt * pair::kTileN, 0, p.dw_kb, 0, kDw,
+                  p.dw_kb, p.dw_kb, false};
     }
     const int per_part = p.dh_mt * p.dh_nt;
     const int part = w / per_part;
@@ -355,11 +356,10 @@ struct GradOp : pair::NoMaps, pair::Plain {
     const int kb0 = part * p.dh_part_kb;
     const int left = p.dh_kb - kb0;
     return Tile{w % p.dh_mt * pair::kTileM, w / p.dh_mt * pair::kTileN, 0,
-                left < p.dh_part_kb ? left : p.dh_part_kb, kb0, kDh + 2 * part};
+                left < p.dh_part_kb ? left : p.dh_part_kb, kb0, kDh + 2 * part, 0, p.dh_part_kb,
+                false};
   }
   static constexpr int kForms = pair::kFormMM | pair::kFormKM;
-  static __device__ __forceinline__ bool a_mn(const Tile& t, int) { return (t.kind & 1) == kDw; }
-  static __device__ __forceinline__ bool b_mn(const Tile&, int) { return true; }
   static __device__ __forceinline__ const CUtensorMap* map_a_mn(const Params& p, const Tile&) {
     return &p.dl_mn;
   }

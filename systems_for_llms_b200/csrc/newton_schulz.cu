@@ -77,8 +77,8 @@ __device__ __forceinline__ void load4(const T* row, int c, int n, bool vec, floa
   }
 }
 
-// A block's share of a matrix: rows r0, r0 + step, ... with its threads side by side along a row
-// (or several short rows at a time), kDepth independent loads in flight per thread.
+// A block's share of a matrix: its threads lie side by side along a row (or along several short
+// rows), and each visits kDepth rows at a time so that as many loads are in flight.
 constexpr int kDepth = 4;
 template <class F>
 __device__ __forceinline__ void walk(int m, int quads, F&& visit) {
@@ -86,9 +86,10 @@ __device__ __forceinline__ void walk(int m, int quads, F&& visit) {
   const unsigned down = kNormThreads / across;
   const unsigned r_in = threadIdx.x / across, c_in = threadIdx.x - r_in * across;
   if (r_in >= down) return;
-  for (long r = blockIdx.x * static_cast<long>(down) + r_in; r < m;
-       r += static_cast<long>(gridDim.x) * down)
-    for (int q = c_in; q < quads; q += across * kDepth) visit(r, q, across);
+  const long step = static_cast<long>(gridDim.x) * down;
+  for (int q = c_in; q < quads; q += across)
+    for (long r = blockIdx.x * static_cast<long>(down) + r_in; r < m; r += step * kDepth)
+      visit(r, step, q);
 }
 
 // Sum of squares of each block's share of a matrix.  64-bit sums: squares of fp32 entries neither
@@ -102,12 +103,12 @@ ns_norm_kernel(Stack s, int m, int n, int vec, double* __restrict__ partial) {
   const T* src = matrix<T>(s, blockIdx.y);
   const int quads = (n + 3) >> 2;
   double sum = 0.0;
-  walk(m, quads, [&](long r, int q, int across) {
+  walk(m, quads, [&](long r, long step, int q) {
     float v[kDepth][4];
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
-      const int at = q + d * across;
-      load4(src + r * s.row, at < quads ? at * 4 : n, n, vec, v[d]);
+      const bool in = r + d * step < m;
+      load4(src + (in ? r + d * step : r) * s.row, in ? q * 4 : n, n, vec, v[d]);
     }
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
@@ -153,17 +154,17 @@ ns_split_kernel(Stack s, int m, int n, int ld, int vec, const double* __restrict
   const T* src = matrix<T>(s, z);
   const long out0 = static_cast<long>(z) * m * ld;
   const int quads = ld >> 2;
-  walk(m, quads, [&](long r, int q, int across) {
+  walk(m, quads, [&](long r, long step, int q) {
     float v[kDepth][4];
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
-      const int at = q + d * across;
-      load4(src + r * s.row, at < quads ? at * 4 : n, n, vec, v[d]);
+      const bool in = r + d * step < m;
+      load4(src + (in ? r + d * step : r) * s.row, in ? q * 4 : n, n, vec, v[d]);
     }
 #pragma unroll
     for (int d = 0; d < kDepth; ++d) {
-      const int at = q + d * across;
-      if (at >= quads) break;
+      if (r + d * step >= m) break;
+      const long at = out0 + (r + d * step) * ld + q * 4;
       __half h[4], l[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -171,9 +172,8 @@ ns_split_kernel(Stack s, int m, int n, int ld, int vec, const double* __restrict
         h[j] = __float2half_rn(x);
         l[j] = __float2half_rn(x - __half2float(h[j]));
       }
-      *reinterpret_cast<uint2*>(hi + out0 + r * ld + at * 4) = *reinterpret_cast<const uint2*>(h);
-      if (lo != nullptr)
-        *reinterpret_cast<uint2*>(lo + out0 + r * ld + at * 4) = *reinterpret_cast<const uint2*>(l);
+      *reinterpret_cast<uint2*>(hi + at) = *reinterpret_cast<const uint2*>(h);
+      if (lo != nullptr) *reinterpret_cast<uint2*>(lo + at) = *reinterpret_cast<const uint2*>(l);
     }
   });
 }
@@ -237,9 +237,9 @@ dim3 rows_grid(int rows, long len) {
 }
 
 // ------------------------------------------------- symmetric products: G, b G + c G G ----
-// A symmetric matrix of which the 256 x 256 tiles on and above the diagonal are stored, as an
-// operand: rows of tile `i`, reduction step kb.  Tiles below the diagonal are read transposed.
-__device__ __forceinline__ bool below(int i, int kb) { return (kb * pair::kBK) / pair::kTileN < i; }
+// Of a symmetric matrix the 256 x 256 tiles on and above the diagonal are stored.  As an operand
+// with rows of tile i, the steps before turn(i) lie below the diagonal and are read transposed.
+__device__ __forceinline__ int turn(int i) { return i * (pair::kTileN / pair::kBK); }
 
 // out = alpha aux + beta A B^T (+ shift I) on and above the diagonal.  Gram matrix: A = B = X;
 // polynomial: A = B = G, aux = G.
@@ -258,7 +258,6 @@ struct SymOp : pair::NoMaps, pair::RoundRobin {
     float alpha, beta;
     float shift;                    // added to the diagonal
   };
-  // Tile::kind: 0 X K-major, 1 X MN-major, 2 G
   static __device__ __forceinline__ Tile tile(const Params& p, int w) {
     const int z = w / p.per;
     int in = w - z * p.per, i = 0;
@@ -266,15 +265,10 @@ struct SymOp : pair::NoMaps, pair::RoundRobin {
       in -= p.nt - i;
       ++i;
     }
-    return Tile{i * pair::kTileM, (i + in) * pair::kTileN, z, p.num_kb, 0, p.gram ? p.mn : 2};
+    const int j = i + in;
+    return Tile{i * pair::kTileM, j * pair::kTileN, z, p.num_kb, 0, 0,
+                p.gram ? p.mn * p.num_kb : turn(i), p.gram ? p.mn * p.num_kb : turn(j), in == 0};
   }
-  static __device__ __forceinline__ bool a_mn(const Tile& t, int kb) {
-    return t.kind == 2 ? below(t.m0 / pair::kTileM, kb) : t.kind != 0;
-  }
-  static __device__ __forceinline__ bool b_mn(const Tile& t, int kb) {
-    return t.kind == 2 ? below(t.n0 / pair::kTileN, kb) : t.kind != 0;
-  }
-  static __device__ __forceinline__ bool same(const Tile& t) { return t.m0 == t.n0; }
   static constexpr int kForms =
       pair::kFormKK | pair::kFormMM | pair::kFormKM | pair::kFormMK | pair::kFormSame;
   static __device__ __forceinline__ const CUtensorMap* map_a_k(const Params& p, const Tile&) {
@@ -380,14 +374,9 @@ struct ApplyOp : pair::NoMaps, pair::RoundRobin {
     in -= b * p.band * p.nt;
     const int width = p.mt - b * p.band < p.band ? p.mt - b * p.band : p.band;
     const int n = in / width;
-    return Tile{(b * p.band + in - n * width) * pair::kTileM, n * pair::kTileN, z, p.num_kb, 0,
-                p.wide};
-  }
-  static __device__ __forceinline__ bool a_mn(const Tile& t, int kb) {
-    return t.kind != 0 && below(t.m0 / pair::kTileM, kb);
-  }
-  static __device__ __forceinline__ bool b_mn(const Tile& t, int kb) {
-    return t.kind != 0 || below(t.n0 / pair::kTileN, kb);
+    const int m = b * p.band + in - n * width;
+    return Tile{m * pair::kTileM, n * pair::kTileN, z, p.num_kb, 0, p.wide,
+                p.wide ? turn(m) : 0, p.wide ? p.num_kb : turn(n), false};
   }
   // wide: A = P in either orientation, B = X MN-major; tall: A = X K-major, B = P in either
   static constexpr int kForms = pair::kFormKK | pair::kFormMM | pair::kFormKM;

@@ -22,11 +22,9 @@
 //   static int  Op::first(p, cluster), Op::next(p, w, cluster, clusters)
 //                                  the cluster's first tile and the one after w (>= total: none)
 //   static Tile Op::tile(p, w)     where the tile lies
-//   static bool Op::a_mn(t, kb), Op::b_mn(t, kb)  MN-major operands (see gemm.cu), step by step
 //   static constexpr int Op::kForms  the combinations of orientations that occur
 //   static const CUtensorMap* Op::map_a_k(p, t), map_a_mn, map_b_k, map_b_mn   rank-3 maps
 //                                    {inner, rows, batch} of the orientations that occur
-//   static bool Op::same(t)        B's rows are A's: one copy serves as both operands
 //   static constexpr int Op::kEpiTiles           staging tiles per epilogue warp, 1 or 2
 //   static void Op::begin(p, t, EpiContext&)     before the accumulator is ready (prefetches)
 //   static void Op::epilogue(p, t, EpiContext&)  one warp's share of the tile
@@ -69,6 +67,8 @@ struct Tile {
   int num_kb;     // 64-deep steps
   int kb0;        // first step of the reduction
   int kind;       // for Ops that mix products
+  int a_mn, b_mn; // steps before this one read A / B MN-major (see gemm.cu), the others K-major
+  bool same;      // B's rows are A's: one copy serves as both operands
 };
 
 struct __align__(8) Barriers {
@@ -201,9 +201,6 @@ struct NoMaps {
   template <class P> static __device__ const CUtensorMap* map_a_mn(const P&, const Tile&) { return nullptr; }
   template <class P> static __device__ const CUtensorMap* map_b_k(const P&, const Tile&) { return nullptr; }
   template <class P> static __device__ const CUtensorMap* map_b_mn(const P&, const Tile&) { return nullptr; }
-  static __device__ __forceinline__ bool a_mn(const Tile&, int) { return false; }
-  static __device__ __forceinline__ bool b_mn(const Tile&, int) { return false; }
-  static __device__ __forceinline__ bool same(const Tile&) { return false; }
 };
 
 // Bases for Ops whose epilogue loads nothing of its own, and whose tiles are dealt round robin.
@@ -278,8 +275,8 @@ __device__ __forceinline__ void by_orientation(const Tile& t, int kb, F&& f) {
   const std::false_type no;
   constexpr int kForms = Op::kForms;
   if constexpr ((kForms & kFormSame) != 0) {
-    if (Op::same(t)) {
-      if ((kForms & kFormMM) != 0 && Op::a_mn(t, kb)) f(yes, yes, yes);
+    if (t.same) {
+      if ((kForms & kFormMM) != 0 && kb < t.a_mn) f(yes, yes, yes);
       else f(no, no, yes);
       return;
     }
@@ -289,7 +286,7 @@ __device__ __forceinline__ void by_orientation(const Tile& t, int kb, F&& f) {
   } else if constexpr (kForms == kFormMM) {
     f(yes, yes, no);
   } else {
-    const bool a = Op::a_mn(t, kb), b = Op::b_mn(t, kb);
+    const bool a = kb < t.a_mn, b = kb < t.b_mn;
     if constexpr ((kForms & kFormKK) != 0) {
       if (!a && !b) f(no, no, no);
     }
