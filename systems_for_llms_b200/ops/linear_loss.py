@@ -107,16 +107,19 @@ def linear_ce_forward(hidden, weight, targets, ignore_index: int, mean: bool | N
     handle = _lib.lib()
     size = handle.sfl_linear_ce_part_bytes(rows, vocab)
     part = torch.empty(size, dtype=torch.uint8, device=dev)
-    stats = torch.empty(2 * rows + 3, dtype=torch.float32, device=dev)
-    row_loss, lse2, totals, loss = stats.split((rows, rows, 2, 1))
-    args = _args(hidden, weight, targets, ignore_index, lse2)
+    row_loss, lse2 = torch.empty(2, rows, dtype=torch.float32, device=dev).unbind(0)
     reduce = mean is not None
+    totals, loss = None, None
+    if reduce:
+        totals = torch.empty(2, dtype=torch.float32, device=dev)
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+    args = _args(hidden, weight, targets, ignore_index, lse2)
     with _lib.on_device(dev):
         code = handle.sfl_linear_ce_fwd(byref(args), part.data_ptr(), size, row_loss.data_ptr(),
-                                        int(bool(mean)), totals.data_ptr() if reduce else None,
-                                        loss.data_ptr() if reduce else None, _lib.stream_ptr())
+                                        int(bool(mean)), _lib.ptr(totals), _lib.ptr(loss),
+                                        _lib.stream_ptr())
     _lib.check(code, "sfl_linear_ce_fwd")
-    return row_loss, lse2, (totals if reduce else None), (loss[0] if reduce else None)
+    return row_loss, lse2, totals, loss
 
 
 def linear_ce_backward(hidden, weight, targets, ignore_index: int, lse2, grad, totals, dw,

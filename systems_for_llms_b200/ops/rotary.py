@@ -15,8 +15,10 @@ The reference has the interleaved rotation of whole heads only, without a norm
 from __future__ import annotations
 
 import math
-from ctypes import POINTER, Structure, byref, c_float, c_int, c_long, c_void_p
+from ctypes import Structure, c_float, c_int, c_long, c_void_p
 from dataclasses import dataclass
+from functools import lru_cache
+from struct import Struct
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -45,13 +47,17 @@ class RotaryTable(Structure):
                 ("pos_b", c_long), ("pos_t", c_long), ("rows", c_int), ("rotated", c_int)]
 
 
+# Calls pass the two records as packed bytes (the layouts above): filling ctypes structures field
+# by field costs several microseconds, which a decode step pays per layer.
+_TENSOR = Struct("4P9li4x")
+_TABLE = Struct("3P2l2i")
+
 _P = c_void_p
-_lib.register_signature("sfl_rotary", [POINTER(RotaryTensor), c_int, POINTER(RotaryTable), c_int,
-                                       c_int, c_int, c_float, c_int, c_int, c_int, _P])
+_lib.register_signature("sfl_rotary", [_P, c_int, _P, c_int, c_int, c_int, c_float, c_int, c_int,
+                                       c_int, _P])
 _lib.register_signature("sfl_rotary_bwd_partial_bytes", [c_int, c_int, c_int, c_int, c_int])
-_lib.register_signature("sfl_rotary_bwd", [POINTER(RotaryTensor), c_int, POINTER(RotaryTable),
-                                           c_int, c_int, c_int, c_float, c_int, c_int, _P, c_long,
-                                           _P, _P, _P])
+_lib.register_signature("sfl_rotary_bwd", [_P, c_int, _P, c_int, c_int, c_int, c_float, c_int, c_int,
+                                           _P, c_long, _P, _P, _P])
 
 
 # ------------------------------------------------------------------------ tables --
@@ -126,32 +132,36 @@ def _check_heads(x: torch.Tensor, name: str) -> None:
         raise TypeError(f"{name} must be bf16, fp16 or fp32")
     if not x.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if x.shape[1] < 1 or not 1 <= x.shape[3] <= MAX_HEAD_DIM:
+    _, heads, _, dim = x.shape
+    if heads < 1 or not 1 <= dim <= MAX_HEAD_DIM:
         raise ValueError(f"{name} needs at least one head and a head dimension of 1 to "
                          f"{MAX_HEAD_DIM}")
-    if x.shape[3] > 1 and x.stride(3) != 1:
+    if dim > 1 and x.stride(3) != 1:
         raise ValueError(f"{name} must have a contiguous last dimension")
 
 
 def _check_table(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions) -> None:
+    device = x.device
     for t, name in ((cos, "cos"), (sin, "sin")):
-        if t.ndim != 2 or t.dtype != torch.float32 or not t.is_contiguous() or t.device != x.device:
+        if (t.dtype != torch.float32 or t.ndim != 2 or t.device != device
+                or not t.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous fp32 [positions, rotated / 2] tensor on "
                              "the device of the heads")
-    if cos.shape != sin.shape or cos.shape[0] < 1:
+    rows, half = cos.shape
+    if sin.shape != cos.shape or rows < 1:
         raise ValueError("cos and sin must have the same shape with at least one position")
-    if cos.shape[0] >= 2**31:
+    if rows >= 2**31:
         raise ValueError("tables of 2**31 positions or more are not supported")
-    if 2 * cos.shape[1] > x.shape[3]:
+    B, _, T, D = x.shape
+    if 2 * half > D:
         raise ValueError("the tables rotate more lanes than a head has")
-    B, T = x.shape[0], x.shape[2]
     if positions is None:
-        if T > cos.shape[0]:
+        if T > rows:
             raise ValueError("more tokens than positions in the tables")
         return
-    if positions.dtype != torch.int64 or positions.device != x.device:
+    if positions.dtype != torch.int64 or positions.device != device:
         raise ValueError("positions must be int64 on the device of the heads")
-    if tuple(positions.shape) not in ((T,), (B, T)):
+    if positions.shape != (B, T) and positions.shape != (T,):
         raise ValueError("positions must be [tokens] or [batch, tokens]")
 
 
@@ -172,41 +182,45 @@ def _new(x: torch.Tensor) -> torch.Tensor:
                                device=x.device)
 
 
-def _slot(slot: RotaryTensor, x, y, dy, weight) -> None:
-    slot.x, slot.y = x.data_ptr(), y.data_ptr()
-    slot.x_b, slot.x_h, slot.x_t = x.stride()[:3]
-    slot.y_b, slot.y_h, slot.y_t = y.stride()[:3]
-    if dy is not None:
-        slot.dy = dy.data_ptr()
-        slot.dy_b, slot.dy_h, slot.dy_t = dy.stride()[:3]
-    if weight is not None:
-        slot.weight = weight.data_ptr()
-    slot.heads = x.shape[1]
+def _record(x, y, dy, weight) -> bytes:
+    x_b, x_h, x_t, _ = x.stride()
+    y_b, y_h, y_t, _ = y.stride()
+    dy_b, dy_h, dy_t, _ = (0, 0, 0, 0) if dy is None else dy.stride()
+    return _TENSOR.pack(x.data_ptr(), y.data_ptr(), 0 if dy is None else dy.data_ptr(),
+                        0 if weight is None else weight.data_ptr(), x_b, x_h, x_t, y_b, y_h, y_t,
+                        dy_b, dy_h, dy_t, x.shape[1])
 
 
-def _table(cos, sin, positions) -> RotaryTable:
-    table = RotaryTable(cos=cos.data_ptr(), sin=sin.data_ptr(), rows=cos.shape[0],
-                        rotated=2 * cos.shape[1])
+def _table(cos, sin, positions) -> bytes:
+    rows, half = cos.shape
+    at, pos_b, pos_t = 0, 0, 0
     if positions is not None:
-        table.positions = positions.data_ptr()
-        table.pos_t = positions.stride(-1)
-        table.pos_b = positions.stride(0) if positions.ndim == 2 else 0
-    return table
+        at, pos_t = positions.data_ptr(), positions.stride(-1)
+        pos_b = positions.stride(0) if positions.ndim == 2 else 0
+    return _TABLE.pack(cos.data_ptr(), sin.data_ptr(), at, pos_b, pos_t, rows, 2 * half)
 
 
 def _launch(xs, ys, weights, cos, sin, positions, eps, layout, inverse=False) -> None:
-    B, _, T, D = xs[0].shape
+    x = xs[0]
+    B, _, T, D = x.shape
     if B == 0 or T == 0:
         return
-    slots = (RotaryTensor * len(xs))()
-    for slot, x, y, weight in zip(slots, xs, ys, weights):
-        _slot(slot, x, y, None, weight)
-    table = _table(cos, sin, positions)
-    with _lib.on_device(xs[0].device):
-        code = _lib.lib().sfl_rotary(slots, len(xs), byref(table), B, T, D, float(eps),
-                                     int(layout == "half"), int(inverse), _DTYPES[xs[0].dtype],
+    records = b"".join([_record(x, y, None, weight) for x, y, weight in zip(xs, ys, weights)])
+    with _lib.on_device(x.device):
+        code = _lib.lib().sfl_rotary(records, len(xs), _table(cos, sin, positions), B, T, D, eps,
+                                     layout == "half", inverse, _DTYPES[x.dtype],
                                      _lib.stream_ptr())
-    _lib.check(code, "sfl_rotary")
+    if code:
+        _lib.check(code, "sfl_rotary")
+
+
+@lru_cache(maxsize=64)
+def _partial_bytes(device_index: int, dim: int) -> int:
+    """Scratch of the backward grid on a device (current when this is called)."""
+    size = _lib.lib().sfl_rotary_bwd_partial_bytes(1, 1, 1, 1, dim)
+    if size <= 0:
+        raise RuntimeError("sfl_rotary_bwd_partial_bytes refused the head dimension")
+    return size
 
 
 def _rows(grad: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
@@ -264,23 +278,19 @@ def qk_norm_rotary_grad(q, k, q_weight, k_weight, cos, sin, positions, dq_out, d
     B, _, T, D = q.shape
     if B == 0 or T == 0:
         return (*dxs, torch.zeros_like(q_weight), torch.zeros_like(k_weight))
-    dws = torch.empty(2, D, dtype=torch.float32, device=q.device)
-    slots = (RotaryTensor * 2)()
-    for slot, x, dx, dy, weight in zip(slots, xs, dxs, gs, (q_weight, k_weight)):
-        _slot(slot, x, dx, dy, weight)
-    table = _table(cos, sin, positions)
-    handle = _lib.lib()
-    with _lib.on_device(q.device):
-        size = handle.sfl_rotary_bwd_partial_bytes(q.shape[1], k.shape[1], B, T, D)
-        if size <= 0:
-            raise RuntimeError("sfl_rotary_bwd_partial_bytes refused the shape")
-        partial = torch.empty(size, dtype=torch.uint8, device=q.device)
-        code = handle.sfl_rotary_bwd(slots, 2, byref(table), B, T, D, float(eps),
-                                     int(layout == "half"), _DTYPES[q.dtype], partial.data_ptr(),
-                                     size, dws[0].data_ptr(), dws[1].data_ptr(),
-                                     _lib.stream_ptr())
-    _lib.check(code, "sfl_rotary_bwd")
-    return (*dxs, dws[0], dws[1])
+    device = q.device
+    dqw, dkw = torch.empty(2, D, dtype=torch.float32, device=device).unbind(0)
+    records = b"".join([_record(x, dx, dy, weight) for x, dx, dy, weight
+                        in zip(xs, dxs, gs, (q_weight, k_weight))])
+    with _lib.on_device(device):
+        size = _partial_bytes(device.index, D)
+        partial = torch.empty(size, dtype=torch.uint8, device=device)
+        code = _lib.lib().sfl_rotary_bwd(records, 2, _table(cos, sin, positions), B, T, D, eps,
+                                         layout == "half", _DTYPES[q.dtype], partial.data_ptr(),
+                                         size, dqw.data_ptr(), dkw.data_ptr(), _lib.stream_ptr())
+    if code:
+        _lib.check(code, "sfl_rotary_bwd")
+    return (*dxs, dqw, dkw)
 
 
 def qk_norm_rotary_into(q, k, q_weight, k_weight, cos, sin, positions=None, *, eps: float,

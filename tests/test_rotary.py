@@ -122,3 +122,28 @@ def test_entry_points_refuse_before_launching():
     bwd = lambda: handle.sfl_rotary_bwd(slots, 1, ctypes.byref(table), 1, 1, 64, 0.0, 0, 0, 256, 0,
                                         256, 256, None)
     assert bwd() == -2                        # nothing to differentiate without a norm
+
+
+def test_packed_records_have_the_layout_of_the_structures():
+    import ctypes
+
+    from systems_for_llms_b200.ops import rotary as R
+    assert R._TENSOR.size == ctypes.sizeof(R.RotaryTensor)
+    assert R._TABLE.size == ctypes.sizeof(R.RotaryTable)
+    x, y, dy = (torch.zeros(2, 3, 4, 8)[:, :, :, :n] for n in (8, 7, 6))
+    w = torch.ones(8)
+    record = R.RotaryTensor.from_buffer_copy(R._record(x, y, dy, w))
+    assert (record.x, record.y, record.dy, record.weight) == (x.data_ptr(), y.data_ptr(),
+                                                              dy.data_ptr(), w.data_ptr())
+    assert (record.x_b, record.x_h, record.x_t) == x.stride()[:3] and record.heads == 3
+    assert (record.y_b, record.y_h, record.y_t) == y.stride()[:3]
+    assert (record.dy_b, record.dy_h, record.dy_t) == dy.stride()[:3]
+    cos, sin = rotary_tables(8, 16)
+    positions = torch.zeros(2, 6).long()[:, ::2]
+    table = R.RotaryTable.from_buffer_copy(R._table(cos, sin, positions))
+    assert (table.cos, table.sin, table.positions) == (cos.data_ptr(), sin.data_ptr(),
+                                                       positions.data_ptr())
+    assert (table.pos_b, table.pos_t, table.rows, table.rotated) == (6, 2, 16, 8)
+    shared = R.RotaryTable.from_buffer_copy(R._table(cos, sin, positions[0]))
+    assert (shared.pos_b, shared.pos_t) == (0, 2)
+    assert R.RotaryTable.from_buffer_copy(R._table(cos, sin, None)).positions is None
