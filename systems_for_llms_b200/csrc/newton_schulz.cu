@@ -237,6 +237,16 @@ dim3 rows_grid(int rows, long len) {
 }
 
 // ------------------------------------------------- symmetric products: G, b G + c G G ----
+// Two staging tiles take turns: chunk 0 may be written once everything has left them (the tile
+// before may have had no chunk 1), chunk 1 once all but chunk 0's store has.
+__device__ __forceinline__ void reuse(const EpiContext& c, int chunk) {
+  if (c.lane == 0) {
+    if (chunk == 0) tma_store_wait_read<0>();
+    else tma_store_wait_read<1>();
+  }
+  __syncwarp();
+}
+
 // Of a symmetric matrix the 256 x 256 tiles on and above the diagonal are stored.  As an operand
 // with rows of tile i, the steps before turn(i) lie below the diagonal and are read transposed.
 __device__ __forceinline__ int turn(int i) { return i * (pair::kTileN / pair::kBK); }
@@ -310,10 +320,7 @@ struct SymOp : pair::NoMaps, pair::RoundRobin {
         if (p.gram) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] *= p.beta;
-          if (h == 0) {  // this tile's store is the one before the last
-            if (c.lane == 0) tma_store_wait_read<1>();
-            __syncwarp();
-          }
+          if (h == 0) reuse(c, ch);
         } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -346,6 +353,106 @@ struct SymOp : pair::NoMaps, pair::RoundRobin {
 };
 
 // ------------------------------------------------------------ X <- a X + P X ----
+// What the epilogue of the product needs to know.
+struct ApplyView {
+  const CUtensorMap *hi, *lo;       // X as it was: 64-column lines of 32 rows; lo is rewritten in place
+  const CUtensorMap *hi_out, *out;  // the next hi, or the bf16 result
+  int m, n;
+  int folded;                       // 1: P holds a X as well; hi + lo of X are not read
+  int keep_lo;                      // 1: write lo of the next X
+  int last;                         // 0: next X, 1: result through TMA, 2: result element by element
+  float alpha, beta;
+  __nv_bfloat16* result;            // [batch, m, n]
+};
+
+__device__ __forceinline__ void apply_load(const ApplyView& p, const Tile& t, EpiContext& c,
+                                           int begin) {
+  if (c.lane == 0) {
+    tma_store_wait_read<0>();
+    mbar_expect_tx(c.aux_bar, 2 * pair::kEpiTileBytes);
+    tma_load_3d(c.smem, p.hi, c.aux_bar, begin, c.row0, t.z);
+    tma_load_3d(c.smem + pair::kEpiTileBytes, p.lo, c.aux_bar, begin, c.row0, t.z);
+  }
+}
+__device__ __forceinline__ void apply_begin(const ApplyView& p, const Tile& t, EpiContext& c) {
+  const int col0 = t.n0 + c.part * 128;
+  if (!p.folded && c.row0 < p.m && col0 < p.n) apply_load(p, t, c, col0);
+}
+__device__ __forceinline__ void apply_epilogue(const ApplyView& p, const Tile& t, EpiContext& c) {
+  const int col0 = t.n0 + c.part * 128;
+  if (c.row0 >= p.m) return;  // warp-uniform
+  const int row = c.row0 + c.lane;
+#pragma unroll 1
+  for (int ch = 0; ch < 2; ++ch) {
+    const int begin = col0 + ch * 64;
+    if (begin >= p.n) break;  // warp-uniform
+    // hi and lo of a chunk take both staging tiles; without them the chunks alternate
+    uint8_t* tile = p.folded ? c.smem + ch * pair::kEpiTileBytes : c.smem;
+    uint8_t* low = c.smem + pair::kEpiTileBytes;
+    if (p.folded) {
+      reuse(c, ch);
+    } else {
+      pair::wait_aux(c);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float v[32];
+      pair::load_acc(c.acc + c.part * 128 + ch * 64 + h * 32, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // each lane rewrites exactly the bytes it read
+        uint4* qh = reinterpret_cast<uint4*>(pair::tile_chunk(tile, c.lane, 4 * h + j));
+        uint4* ql = reinterpret_cast<uint4*>(pair::tile_chunk(low, c.lane, 4 * h + j));
+        uint4 a = make_uint4(0, 0, 0, 0), b = a;
+        if (!p.folded) {
+          a = *qh;
+          b = *ql;
+        }
+        __half2* eh = reinterpret_cast<__half2*>(&a);
+        __half2* el = reinterpret_cast<__half2*>(&b);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 fh = __half22float2(eh[k]), fl = __half22float2(el[k]);
+          const float x = fmaf(v[8 * j + 2 * k], p.beta, p.alpha * (fh.x + fl.x));
+          const float y = fmaf(v[8 * j + 2 * k + 1], p.beta, p.alpha * (fh.y + fl.y));
+          if (p.last == 0) {
+            eh[k] = __floats2half2_rn(x, y);
+            if (p.keep_lo) {
+              const float2 r = __half22float2(eh[k]);
+              el[k] = __floats2half2_rn(x - r.x, y - r.y);
+            }
+          } else {
+            const uint32_t packed = pack_bf16(x, y);
+            eh[k] = *reinterpret_cast<const __half2*>(&packed);
+          }
+        }
+        *qh = a;
+        if (p.keep_lo) *ql = b;
+        if (p.last == 2 && row < p.m) {
+          const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&a);
+          const int col = begin + h * 32 + 8 * j;
+          __nv_bfloat16* dst = p.result + (static_cast<long>(t.z) * p.m + row) * p.n + col;
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (col + k < p.n) dst[k] = e[k];
+        }
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (c.lane == 0 && p.last != 2) {
+      if (p.last == 0) {
+        pair::store_3d(p.hi_out, tile, begin, c.row0, t.z);
+        if (p.keep_lo) pair::store_3d(p.lo, low, begin, c.row0, t.z);
+      } else {
+        pair::store_3d(p.out, tile, begin, c.row0, t.z);
+      }
+      tma_store_commit();
+    }
+    if (!p.folded && ch == 0 && begin + 64 < p.n) apply_load(p, t, c, begin + 64);
+  }
+}
+
 struct ApplyOp : pair::NoMaps, pair::RoundRobin {
   static constexpr int kEpiTiles = 2;
   struct Params {
@@ -392,95 +499,702 @@ struct ApplyOp : pair::NoMaps, pair::RoundRobin {
   static __device__ __forceinline__ const CUtensorMap* map_b_mn(const Params& p, const Tile& t) {
     return t.kind != 0 ? &p.x : &p.p_mn;
   }
-  static __device__ __forceinline__ void load_aux(const Params& p, const Tile& t, EpiContext& c,
-                                                  int begin) {
-    if (c.lane == 0) {
-      tma_store_wait_read<0>();
-      mbar_expect_tx(c.aux_bar, 2 * pair::kEpiTileBytes);
-      tma_load_3d(c.smem, &p.hi, c.aux_bar, begin, c.row0, t.z);
-      tma_load_3d(c.smem + pair::kEpiTileBytes, &p.lo, c.aux_bar, begin, c.row0, t.z);
-    }
+  static __device__ __forceinline__ ApplyView view(const Params& p) {
+    return ApplyView{&p.hi, &p.lo, &p.hi_out, &p.out, p.m, p.n, p.folded, p.keep_lo, p.last, p.alpha,
+                     p.beta, p.result};
   }
   static __device__ __forceinline__ void begin(const Params& p, const Tile& t, EpiContext& c) {
-    const int col0 = t.n0 + c.part * 128;
-    if (!p.folded && c.row0 < p.m && col0 < p.n) load_aux(p, t, c, col0);
+    apply_begin(view(p), t, c);
   }
   static __device__ __forceinline__ void epilogue(const Params& p, const Tile& t, EpiContext& c) {
-    const int col0 = t.n0 + c.part * 128;
-    if (c.row0 >= p.m) return;  // warp-uniform
-    const int row = c.row0 + c.lane;
-#pragma unroll 1
-    for (int ch = 0; ch < 2; ++ch) {
-      const int begin = col0 + ch * 64;
-      if (begin >= p.n) break;  // warp-uniform
-      // hi and lo of a chunk take both staging tiles; without them the chunks alternate
-      uint8_t* tile = p.folded ? c.smem + ch * pair::kEpiTileBytes : c.smem;
-      uint8_t* low = c.smem + pair::kEpiTileBytes;
-      if (p.folded) {
-        if (c.lane == 0) tma_store_wait_read<1>();
-        __syncwarp();
-      } else {
-        pair::wait_aux(c);
+    apply_epilogue(view(p), t, c);
+  }
+};
+
+// 32 of the 64 fp16 numbers of a row in an operand block (see pair::stage_16).
+__device__ __forceinline__ void kept(uint8_t* block, int row, int half, float (&v)[32]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint4 q = *reinterpret_cast<const uint4*>(pair::tile_chunk(block, row, 4 * half + j));
+    const __half2* e = reinterpret_cast<const __half2*>(&q);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = __half22float2(e[k]);
+      v[8 * j + 2 * k] = f.x;
+      v[8 * j + 2 * k + 1] = f.y;
+    }
+  }
+}
+
+// ------------------------------------ all steps of a matrix with a short side in one kernel ----
+// A matrix whose shorter side is at most 256 has one Gram tile: a cluster computes it, keeps G and
+// then P in the shared memory of its two CTAs as operands of the next product, and walks the tiles
+// of X, step after step, with X alone going through global memory.  Fifteen launches that each wait
+// for the one before (6.7 to 10 us apiece, most of it start and drain) become one.
+//
+// Roles as in pair_kernel.  Ring stages hold 128 rows x 64 (16 KB per CTA): the Gram product reads
+// the same rows as both operands, the others read P from the G / P buffer, four 64-column blocks of
+// 128 rows per CTA - a CTA's rows as A, both CTAs' as the 256 rows of B.  Barriers beyond
+// pair_kernel's: op_ready (leader: all sixteen epilogue warps have written G, or P) and x_ready
+// (both CTAs: all of the step's stores are complete, the next step may load).
+constexpr int kChainStages = 5;
+constexpr int kChainStageBytes = pair::kABytes;
+constexpr int kChainOpBytes = 4 * pair::kABytes;
+constexpr int kChainWarpBytes = 2 * pair::kEpiTileBytes;
+constexpr int kChainSmem = 1024 + kChainStages * kChainStageBytes + kChainOpBytes +
+                           pair::kEpiWarps * kChainWarpBytes + 512;
+static_assert(kChainSmem <= 232448, "more than a CTA's shared memory");
+
+struct ChainParams {
+  CUtensorMap gram[2];      // X as the Gram product's operand (ping, pong)
+  CUtensorMap apply[2];     // X as the other product's operand
+  CUtensorMap hi[2], lo;    // 64-column lines of 32 rows
+  CUtensorMap out;
+  int batch, m, n, wide, steps;
+  int side_kb, long_kb;     // 64-deep steps of the shorter and the longer side
+  int tiles;                // 256-wide tiles along the longer side
+  int last;                 // 1: result through TMA, 2: element by element
+  float a, b, c;
+  __nv_bfloat16* result;
+  int* status;
+};
+
+struct __align__(8) ChainBarriers {
+  uint64_t full[kChainStages];
+  uint64_t empty[kChainStages];
+  uint64_t acc_full[2];
+  uint64_t acc_empty[2];
+  uint64_t op_ready;
+  uint64_t x_ready;
+  uint64_t aux_full[pair::kEpiWarps];
+  uint32_t tmem_base;
+  int abort;
+};
+
+// Orders this thread's later asynchronous (TMA) accesses after what others did before, and others'
+// after what it did: between generic-proxy synchronisation and the async proxy.
+__device__ __forceinline__ void fence_proxy_async_all() {
+  asm volatile("fence.proxy.async;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_release(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
+               : "memory");
+}
+__device__ __forceinline__ void acquire_cluster() {
+  asm volatile("fence.acq_rel.cluster;" ::: "memory");
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
+ns_chain_kernel(const __grid_constant__ ChainParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  uint8_t* op = smem + kChainStages * kChainStageBytes;  // G, then P
+  uint8_t* epi_smem = op + kChainOpBytes;
+  ChainBarriers* bars =
+      reinterpret_cast<ChainBarriers*>(epi_smem + pair::kEpiWarps * kChainWarpBytes);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = pair::cluster_rank();
+  const int clusters = gridDim.x >> 1;
+  const int cluster = blockIdx.x >> 1;
+  volatile int* abort = &bars->abort;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kChainStages; ++s) {
+      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars->acc_full[s], 1);
+      mbar_init(&bars->acc_empty[s], 2 * pair::kEpiWarps);
+    }
+    mbar_init(&bars->op_ready, 2 * pair::kEpiWarps);
+    mbar_init(&bars->x_ready, 2 * pair::kEpiWarps);
+    for (int s = 0; s < pair::kEpiWarps; ++s) mbar_init(&bars->aux_full[s], 1);
+    bars->abort = 0;
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&bars->tmem_base)),
+                 "r"(pair::kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  pair::cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = bars->tmem_base;
+  pdl_launch_dependents();
+  pdl_wait();
+
+  auto give_up = [&](int code) {
+    if (lane == 0) report_status(p.status, code);
+    *abort = 1;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------ TMA producer ----
+    int stage = 0;
+    uint32_t phase = 0, x_phase = 0;
+    bool ok = true;
+    const uint32_t full0 = pair::in_leader(smem_u32(&bars->full[0]));
+    // one stage: a box of 128 rows x 64 (K-major) or two of 64 x 64 (MN-major)
+    auto bring = [&](const CUtensorMap* map, bool mn, int rows0, int k0, int z) {
+      if (!pair::wait_or_leave(&bars->empty[stage], phase ^ 1, abort)) {
+        give_up(kStatusTimeoutEmpty);
+        return false;
       }
+      uint8_t* at = smem + stage * kChainStageBytes;
+      const uint32_t bar = full0 + stage * static_cast<uint32_t>(sizeof(uint64_t));
+      if (elect_one()) {
+        if (rank == 0) mbar_expect_tx(&bars->full[stage], 2 * kChainStageBytes);
+        if (mn) {
+          pair::load_3d(at, map, bar, rows0, k0, z);
+          pair::load_3d(at + pair::kBK * 128, map, bar, rows0 + 64, k0, z);
+        } else {
+          pair::load_3d(at, map, bar, k0, rows0, z);
+        }
+      }
+      __syncwarp();
+      if (++stage == kChainStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+      return true;
+    };
+    const int mine = rank * pair::kCtaM;
+    for (int z = cluster; z < p.batch && ok; z += clusters) {
+      for (int step = 0; step < p.steps && ok; ++step) {
+        const int now = step & 1;
+        if (step > 0) {
+          if (!pair::wait_or_leave(&bars->x_ready, x_phase, abort)) {
+            give_up(kStatusTimeoutEmpty);
+            ok = false;
+            break;
+          }
+          acquire_cluster();
+          fence_proxy_async_all();
+          x_phase ^= 1;
+        }
+        for (int kb = 0; kb < p.long_kb && ok; ++kb)
+          ok = bring(&p.gram[now], !p.wide, mine, kb * pair::kBK, z);
+        for (int t = 0; t < p.tiles && ok; ++t)
+          for (int kb = 0; kb < p.side_kb && ok; ++kb)
+            ok = bring(&p.apply[now], p.wide, t * pair::kTileN + mine, kb * pair::kBK, z);
+      }
+    }
+    for (int s = 0; s < kChainStages; ++s) {  // as in pair_kernel
+      if (!mbar_wait(&bars->empty[stage], phase ^ 1)) break;
+      if (++stage == kChainStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+  } else if (warp == 1) {
+    // -------------------------------------------------------- MMA issuer ----
+    if (rank == 0) {
+      const uint32_t base = smem_u32(smem);
+      const uint64_t k0 = umma_smem_desc(base, 16, 1024);
+      const uint64_t mn0 = umma_smem_desc(base, pair::kBK * 128, 1024);
+      const uint64_t op0 = umma_smem_desc(smem_u32(op), 16, 1024);
+      int stage = 0;
+      uint32_t phase = 0, op_phase = 0;
+      uint32_t uses[2] = {0, 0};  // of each accumulator by the tiles of X
+      bool ok = true;
+      // A stage of the ring times itself (kRing = 2), or as A (0) / B (1) with a block of P
+      auto step_of = [&](auto a_mn, auto b_mn, auto ring, uint32_t d, uint64_t op_block, bool more,
+                         uint64_t* done) {
+        constexpr bool kA = decltype(a_mn)::value, kB = decltype(b_mn)::value;
+        constexpr int kRing = decltype(ring)::value;
+        if (!pair::wait_or_leave(&bars->full[stage], phase, abort)) {
+          give_up(kStatusTimeoutFull);
+          return false;
+        }
+        tc_fence_after();
+        const uint64_t mine = umma_desc_advance((kRing == 1 ? kB : kA) ? mn0 : k0,
+                                                stage * kChainStageBytes);
+        const uint64_t a = kRing == 1 ? op_block : mine;
+        const uint64_t b = kRing == 0 ? op_block : mine;
+        const uint32_t idesc = pair::instruction_descriptor(true, kA, kB);
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < pair::kBK / 16; ++k)
+            pair::mma_pair(d, umma_desc_advance(a, k * (kA ? 2048 : 32)),
+                           umma_desc_advance(b, k * (kB ? 2048 : 32)), idesc, more || k != 0);
+          pair::commit_pair(&bars->empty[stage]);
+          if (done != nullptr) pair::commit_pair(done);
+        }
+        __syncwarp();
+        if (++stage == kChainStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+        return true;
+      };
+      auto wait_op = [&] {
+        if (!pair::wait_or_leave(&bars->op_ready, op_phase, abort)) {
+          give_up(kStatusTimeoutTmemEmpty);
+          return false;
+        }
+        acquire_cluster();
+        tc_fence_after();
+        op_phase ^= 1;
+        return true;
+      };
+      auto wait_acc = [&](int acc) {
+        if (uses[acc] == 0) return true;
+        if (!pair::wait_or_leave(&bars->acc_empty[acc], (uses[acc] - 1) & 1, abort)) {
+          give_up(kStatusTimeoutTmemEmpty);
+          return false;
+        }
+        tc_fence_after();
+        return true;
+      };
+      const std::true_type mn;
+      const std::false_type km;
+      const std::integral_constant<int, 0> as_a;
+      const std::integral_constant<int, 1> as_b;
+      const std::integral_constant<int, 2> itself;
+      for (int z = cluster; z < p.batch && ok; z += clusters) {
+        for (int step = 0; step < p.steps && ok; ++step) {
+          ok = wait_acc(0);
+          for (int kb = 0; kb < p.long_kb && ok; ++kb) {
+            uint64_t* done = kb + 1 == p.long_kb ? &bars->acc_full[0] : nullptr;
+            ok = p.wide ? step_of(km, km, itself, tmem_base, 0, kb != 0, done)
+                        : step_of(mn, mn, itself, tmem_base, 0, kb != 0, done);
+          }
+          ok = ok && wait_op();
+          if (!ok) break;
+          if (elect_one()) {  // G G from shared memory
+            const uint32_t idesc = pair::instruction_descriptor(true, false, false);
+            for (int kb = 0; kb < p.side_kb; ++kb) {
+              const uint64_t g = umma_desc_advance(op0, kb * pair::kABytes);
+#pragma unroll
+              for (int k = 0; k < pair::kBK / 16; ++k)
+                pair::mma_pair(tmem_base + pair::kTileN, umma_desc_advance(g, k * 32),
+                               umma_desc_advance(g, k * 32), idesc, (kb | k) != 0);
+            }
+            pair::commit_pair(&bars->acc_full[1]);
+          }
+          __syncwarp();
+          ok = wait_op();
+          for (int t = 0; t < p.tiles && ok; ++t) {
+            const int acc = t & 1;
+            ok = wait_acc(acc);
+            ++uses[acc];
+            for (int kb = 0; kb < p.side_kb && ok; ++kb) {
+              uint64_t* done = kb + 1 == p.side_kb ? &bars->acc_full[acc] : nullptr;
+              const uint32_t d = tmem_base + acc * pair::kTileN;
+              const uint64_t block = umma_desc_advance(op0, kb * pair::kABytes);
+              ok = p.wide ? step_of(km, mn, as_b, d, block, kb != 0, done)
+                          : step_of(km, km, as_a, d, block, kb != 0, done);
+            }
+          }
+        }
+      }
+    }
+  } else {
+    // ---------------------------------------------------------- epilogue ----
+    const int quarter = warp & 3;
+    EpiContext c;
+    c.part = (warp - 2) >> 2;
+    c.lane = lane;
+    c.smem = epi_smem + (warp - 2) * kChainWarpBytes;
+    c.aux_bar = &bars->aux_full[warp - 2];
+    c.aux_phase = 0;
+    c.abort = abort;
+    c.status = p.status;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t op_ready = pair::in_leader(smem_u32(&bars->op_ready));
+    const int row = quarter * 32 + lane;            // of this CTA's 128 rows of G and P
+    const int diagonal = rank * pair::kCtaM + row;  // their column on the diagonal
+    uint32_t full_phase[2] = {0, 0};
+    bool ok = true;
+    auto wait_full = [&](int acc) {
+      if (!pair::wait_or_leave(&bars->acc_full[acc], full_phase[acc], abort)) {
+        give_up(kStatusTimeoutTmemFull);
+        return false;
+      }
+      full_phase[acc] ^= 1;
+      tc_fence_after();
+      return true;
+    };
+    auto keep = [&](int col, const float (&v)[32]) {  // into the G / P buffer
+      pair::stage_16(op + (col >> 6) * pair::kABytes, row, (col >> 5) & 1, v, true);
+    };
+    auto op_written = [&] {
+      fence_proxy_async_all();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_release(op_ready);
+    };
+    const int cols = p.side_kb * pair::kBK;  // columns of G and P that the products read
+    for (int z = cluster; z < p.batch && ok; z += clusters) {
+      for (int step = 0; step < p.steps && ok; ++step) {
+        const bool folded = step + 2 >= p.steps, last = step + 1 == p.steps;
+        ok = wait_full(0);
+        if (!ok) break;
+#pragma unroll 1
+        for (int ch = 0; ch < 4; ++ch) {
+          const int col = c.part * 128 + ch * 32;
+          if (col >= cols) break;  // warp-uniform
+          float v[32];
+          pair::load_acc(tmem_base + lanes + col, v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] *= 1.0f / kScale;
+          keep(col, v);
+        }
+        op_written();
+        ok = wait_full(1);
+        if (!ok) break;
+#pragma unroll 1
+        for (int ch = 0; ch < 4; ++ch) {
+          const int col = c.part * 128 + ch * 32;
+          if (col >= cols) break;  // warp-uniform
+          float v[32];
+          {
+            // the rounded G that was multiplied: b and c must see the same matrix, or its rounding
+            // enters with the slope of c G G alone
+            float g[32];
+            kept(op + (col >> 6) * pair::kABytes, row, (col >> 5) & 1, g);
+            pair::load_acc(tmem_base + pair::kTileN + lanes + col, v);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = fmaf(v[j], p.c / kScale, g[j] * p.b);
+          }
+          if (folded) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (col + j == diagonal) v[j] += p.a * kScale;
+          }
+          keep(col, v);
+        }
+        op_written();
+        const float unscale = last ? 1.0f / kScale : 1.0f;
+        const ApplyView view{&p.hi[step & 1], &p.lo, &p.hi[(step + 1) & 1], &p.out, p.m, p.n, folded,
+                             step + 3 < p.steps, last ? p.last : 0, folded ? 0.f : p.a * unscale,
+                             unscale / kScale, p.result};
+        for (int t = 0; t < p.tiles && ok; ++t) {
+          const int acc = t & 1;
+          const Tile tile{p.wide ? 0 : t * pair::kTileM, p.wide ? t * pair::kTileN : 0, z, 0, 0, 0,
+                          0, 0, false};
+          c.acc = tmem_base + lanes + acc * pair::kTileN;
+          c.row0 = tile.m0 + rank * pair::kCtaM + quarter * 32;
+          apply_begin(view, tile, c);
+          ok = wait_full(acc);
+          if (!ok) break;
+          apply_epilogue(view, tile, c);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) pair::arrive_leader(&bars->acc_empty[acc]);
+        }
+        if (!last) {
+          if (lane == 0) {
+            tma_store_wait<0>();  // the stores are complete, not only read
+            fence_proxy_async_all();
+            const uint32_t ready = smem_u32(&bars->x_ready);
+            arrive_release(in_cta(ready, 0));
+            arrive_release(in_cta(ready, 1));
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (lane == 0) tma_store_wait<0>();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  pair::cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
+                 "r"(pair::kTmemCols)
+                 : "memory");
+  }
+}
+
+// --------------------------------------------------- a small matrix in one block ----
+// A matrix of at most 128 x 384 (either way round) fits on one SM and stays there from its norm to
+// its result: X as fp16 operand in shared memory, (a - k) X as fp32 in tensor memory, where the
+// product P X is added to it.  Nothing is rounded but the operands.  The block of 128 rows x 64
+// columns of X is at once the K-major operand of X X^T (rows are rows) and the MN-major operand of
+// P X (rows are steps of the reduction): the swizzled layouts are the same bytes.  Tall matrices
+// are taken transposed, X = U^T.  In the last two steps k = -(b + c), which makes P + k I vanish
+// where singular values are 1.
+//
+// One launch instead of seventeen; its time is the latency of three products and three passes
+// through registers per step (128 x 384, five steps: see the table at the entry point).
+constexpr int kBlockRows = 128;
+constexpr int kBlockCols = 384;          // 512 columns of tensor memory less 128 of G
+constexpr int kBlockEpiWarps = 8;
+constexpr int kBlockThreads = 32 * (kBlockEpiWarps + 1);
+constexpr int kBlockBytes = kBlockRows * 128;  // 128 rows x 64 fp16
+
+struct BlockParams {
+  Stack u;
+  int m, n, wide, steps;
+  float a, b, c, eps;
+  int vec_in, vec_out;      // rows may be read / written 16 bytes at a time (wide)
+  __nv_bfloat16* out;
+  int* status;
+};
+
+// 32 columns of a row of the result, back in the orientation of the matrix.
+__device__ __forceinline__ void block_store(const BlockParams& p, float (&v)[32], int row, int col0,
+                                            int longer) {
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] *= 1.0f / (kScale * kScale);
+  __nv_bfloat16* out = p.out + static_cast<long>(blockIdx.x) * p.m * p.n;
+  if (!p.wide) {  // a warp's lanes are neighbours in memory
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (col0 + j < longer)
+        out[static_cast<long>(col0 + j) * p.n + row] = __float2bfloat16_rn(v[j]);
+    return;
+  }
+  __nv_bfloat16* dst = out + static_cast<long>(row) * p.n + col0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (p.vec_out && col0 + 8 * j + 8 <= longer) {
+      *reinterpret_cast<uint4*>(dst + 8 * j) =
+          make_uint4(pack_bf16(v[8 * j], v[8 * j + 1]), pack_bf16(v[8 * j + 2], v[8 * j + 3]),
+                     pack_bf16(v[8 * j + 4], v[8 * j + 5]), pack_bf16(v[8 * j + 6], v[8 * j + 7]));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (col0 + 8 * j + e < longer) dst[8 * j + e] = __float2bfloat16_rn(v[8 * j + e]);
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kBlockThreads, 1)
+ns_block_kernel(const __grid_constant__ BlockParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t done_bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  __shared__ double sums[kBlockEpiWarps];
+  const uint32_t raw = smem_u32(smem_raw);
+  uint8_t* op = smem_raw + (((raw + 1023u) & ~1023u) - raw);  // G, then P: two blocks
+  uint8_t* xs = op + 2 * kBlockBytes;                         // X: up to six blocks
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int quarter = warp & 3, part = warp >> 2;
+  const int row = quarter * 32 + lane;
+  const int side = p.wide ? p.m : p.n, longer = p.wide ? p.n : p.m;
+  const int blocks = (longer + 63) >> 6;     // of X
+  const int chunks = 2 * blocks;             // of 32 columns; a warp takes every other one
+  const uint32_t columns = blocks <= 2 ? 256 : 512;  // of tensor memory: 128 of G, 64 per block
+  const int side_blocks = (side + 63) >> 6;  // of G and P
+  volatile int* abort = &abort_flag;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&done_bar, 1);
+    abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == kBlockEpiWarps) {
+    tmem_alloc(&tmem_slot, columns);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t mine = tmem + (static_cast<uint32_t>(quarter * 32) << 16);
+  const uint32_t x_acc = 128;  // columns of X in tensor memory
+  pdl_launch_dependents();
+  pdl_wait();
+
+  uint32_t phase = 0;
+  // Everyone waits for the products that the last warp has just issued.  A wait that runs out is
+  // reported once; the block then runs to its end without waiting again.
+  auto products_done = [&] {
+    if (!*abort && !mbar_wait(&done_bar, phase)) {
+      if (lane == 0) report_status(p.status, kStatusTimeoutTmemFull);
+      *abort = 1;
+    }
+    phase ^= 1;
+    tc_fence_after();
+  };
+  auto operands_written = [&] {
+    fence_proxy_async_smem();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+  };
+  auto to_tmem = [&](uint32_t at, const float (&v)[32]) {
+    uint32_t q[16];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) q[j] = __float_as_uint(v[16 * h + j]);
+      tmem_st_32x16(at + 16 * h, q);
+    }
+  };
+  auto held = [&](int step) { return step + 2 >= p.steps && p.b + p.c < 0.f ? -(p.b + p.c) : 0.f; };
+
+  // ---- the matrix into tensor memory, its norm, then both forms of X
+  const T* u = matrix<T>(p.u, blockIdx.x);
+  double sum = 0.0;
+  if (warp < kBlockEpiWarps) {
+    for (int ch = part; ch < chunks; ch += 2) {
+      float v[32];
+      if (p.wide) {
+        const T* src = u + static_cast<long>(row < side ? row : 0) * p.u.row + ch * 32;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          float q[4];
+          load4(src, 4 * j, row < side ? longer - ch * 32 : 0, p.vec_in, q);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[4 * j + k] = q[k];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const int l = ch * 32 + j;
+          v[j] = row < side && l < longer ? wide(u[static_cast<long>(l) * p.u.row + row]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 32; ++j) sum = fma(static_cast<double>(v[j]), static_cast<double>(v[j]), sum);
+      to_tmem(mine + x_acc + ch * 32, v);
+    }
+    tmem_st_wait();
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) sums[warp] = sum;
+  }
+  __syncthreads();
+  if (warp < kBlockEpiWarps) {
+    sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < kBlockEpiWarps; ++k) sum += sums[k];
+    const float inv = static_cast<float>(kScale / (sqrt(sum) + static_cast<double>(p.eps)));
+    const float ahead = (p.a - held(0)) * kScale;
+    for (int ch = part; ch < chunks; ch += 2) {
+      float v[32];
+      pair::load_acc(mine + x_acc + ch * 32, v);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] *= inv;
+      pair::stage_16(xs + (ch >> 1) * kBlockBytes, row, ch & 1, v, true);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) v[j] *= ahead;
+      to_tmem(mine + x_acc + ch * 32, v);
+    }
+    tmem_st_wait();
+  }
+  operands_written();
+
+  const uint64_t op_k = umma_smem_desc(smem_u32(op), 16, 1024);
+  const uint64_t x_k = umma_smem_desc(smem_u32(xs), 16, 1024);
+  const uint64_t x_mn = umma_smem_desc(smem_u32(xs), kBlockBytes, 1024);
+  auto idesc = [](int cols, bool b_mn) {
+    return umma_idesc_bf16(kBlockRows, cols, false, b_mn) & ~((1u << 7) | (1u << 10));  // fp16
+  };
+  auto square = [&](uint64_t operand, int count) {  // G = X X^T or G G, into columns 0 .. 127
+    if (warp != kBlockEpiWarps) return;
+    if (elect_one()) {
+      for (int kb = 0; kb < count; ++kb) {
+        const uint64_t at = umma_desc_advance(operand, kb * kBlockBytes);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_bf16_ss(tmem, umma_desc_advance(at, k * 32), umma_desc_advance(at, k * 32),
+                       idesc(kBlockRows, false), (kb | k) != 0);
+      }
+      umma_commit(&done_bar);
+    }
+    __syncwarp();
+  };
+
+  for (int step = 0; step < p.steps; ++step) {
+    const bool last = step + 1 == p.steps;
+    const float k = held(step);
+    square(x_k, blocks);
+    products_done();
+    if (warp < kBlockEpiWarps && part < side_blocks) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float v[32];
-        pair::load_acc(c.acc + c.part * 128 + ch * 64 + h * 32, v);
+        pair::load_acc(mine + part * 64 + h * 32, v);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          // each lane rewrites exactly the bytes it read
-          uint4* qh = reinterpret_cast<uint4*>(pair::tile_chunk(tile, c.lane, 4 * h + j));
-          uint4* ql = reinterpret_cast<uint4*>(pair::tile_chunk(low, c.lane, 4 * h + j));
-          uint4 a = make_uint4(0, 0, 0, 0), b = a;
-          if (!p.folded) {
-            a = *qh;
-            b = *ql;
-          }
-          __half2* eh = reinterpret_cast<__half2*>(&a);
-          __half2* el = reinterpret_cast<__half2*>(&b);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 fh = __half22float2(eh[k]), fl = __half22float2(el[k]);
-            const float x = fmaf(v[8 * j + 2 * k], p.beta, p.alpha * (fh.x + fl.x));
-            const float y = fmaf(v[8 * j + 2 * k + 1], p.beta, p.alpha * (fh.y + fl.y));
-            if (p.last == 0) {
-              eh[k] = __floats2half2_rn(x, y);
-              if (p.keep_lo) {
-                const float2 r = __half22float2(eh[k]);
-                el[k] = __floats2half2_rn(x - r.x, y - r.y);
-              }
-            } else {
-              const uint32_t packed = pack_bf16(x, y);
-              eh[k] = *reinterpret_cast<const __half2*>(&packed);
-            }
-          }
-          *qh = a;
-          if (p.keep_lo) *ql = b;
-          if (p.last == 2 && row < p.m) {
-            const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&a);
-            const int col = begin + h * 32 + 8 * j;
-            __nv_bfloat16* dst = p.result + (static_cast<long>(t.z) * p.m + row) * p.n + col;
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (col + k < p.n) dst[k] = e[k];
-          }
-        }
+        for (int j = 0; j < 32; ++j) v[j] *= 1.0f / kScale;
+        pair::stage_16(op + part * kBlockBytes, row, h, v, true);
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (c.lane == 0 && p.last != 2) {
-        if (p.last == 0) {
-          pair::store_3d(&p.hi_out, tile, begin, c.row0, t.z);
-          if (p.keep_lo) pair::store_3d(&p.lo, low, begin, c.row0, t.z);
-        } else {
-          pair::store_3d(&p.out, tile, begin, c.row0, t.z);
-        }
-        tma_store_commit();
-      }
-      if (!p.folded && ch == 0 && begin + 64 < p.n) load_aux(p, t, c, begin + 64);
     }
+    operands_written();
+    square(op_k, side_blocks);
+    products_done();
+    if (warp < kBlockEpiWarps && part < side_blocks) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[32], g[32];
+        kept(op + part * kBlockBytes, row, h, g);
+        pair::load_acc(mine + part * 64 + h * 32, v);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          v[j] = fmaf(v[j], p.c / kScale, g[j] * p.b);
+          if (part * 64 + h * 32 + j == row) v[j] += k * kScale;
+        }
+        pair::stage_16(op + part * kBlockBytes, row, h, v, true);
+      }
+    }
+    operands_written();
+    if (warp == kBlockEpiWarps) {
+      if (elect_one()) {  // (a - k) X + P X, 256 columns at a time
+        for (int n0 = 0; n0 < blocks * 64; n0 += 256) {
+          const int cols = blocks * 64 - n0 < 256 ? blocks * 64 - n0 : 256;
+          const uint64_t b0 = umma_desc_advance(x_mn, (n0 >> 6) * kBlockBytes);
+          for (int kk = 0; kk < side_blocks * 4; ++kk)
+            umma_bf16_ss(tmem + x_acc + n0,
+                         umma_desc_advance(op_k, (kk >> 2) * kBlockBytes + (kk & 3) * 32),
+                         umma_desc_advance(b0, kk * 2048), idesc(cols, true), 1);
+        }
+        umma_commit(&done_bar);
+      }
+      __syncwarp();
+    }
+    products_done();
+    if (warp < kBlockEpiWarps) {
+      const float ahead = last ? 0.f : p.a - held(step + 1);
+      for (int ch = part; ch < chunks; ch += 2) {
+        float v[32];
+        pair::load_acc(mine + x_acc + ch * 32, v);
+        if (!last) {
+          float h[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            h[j] = v[j] * (1.0f / kScale);
+            v[j] *= ahead;
+          }
+          pair::stage_16(xs + (ch >> 1) * kBlockBytes, row, ch & 1, h, true);
+          to_tmem(mine + x_acc + ch * 32, v);
+        } else if (row < side) {
+          block_store(p, v, row, ch * 32, longer);
+        }
+        __syncwarp();  // tensor memory is read by whole warps
+      }
+      if (!last) tmem_st_wait();
+    }
+    if (!last) operands_written();
   }
-};
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kBlockEpiWarps) {
+    tc_fence_after();
+    tmem_dealloc(tmem, columns);
+  }
+}
 
 // ------------------------------------------------------------------- host ----
 long round_up(long v, long to) { return (v + to - 1) / to * to; }
@@ -503,13 +1217,18 @@ Sizes sizes_of(int batch, int m, int n) {
   return s;
 }
 
+// Every row starts where four elements can be read at once.
+template <typename T>
+int rows_of_four(const Stack& s) {
+  const long bytes = 4 * sizeof(T);
+  return (reinterpret_cast<uintptr_t>(s.base) % bytes) == 0 && s.row % 4 == 0 && s.stride0 % 4 == 0 &&
+         s.stride1 % 4 == 0;
+}
+
 template <typename T>
 int normalise(const Stack& s, int batch, int m, int n, int ld, float eps, double* partial,
               __half* hi, __half* lo, cudaStream_t stream) {
-  const int size = sizeof(T);
-  const int bytes = 4 * size;  // four elements at a time
-  const int vec = (reinterpret_cast<uintptr_t>(s.base) % bytes) == 0 && (s.row * size) % bytes == 0 &&
-                  (s.stride0 * size) % bytes == 0 && (s.stride1 * size) % bytes == 0;
+  const int vec = rows_of_four<T>(s);
   const long quads = static_cast<long>(m) * (ld / 4);
   const long want = (quads + 4L * kNormThreads - 1) / (4L * kNormThreads);
   const int chunks = static_cast<int>(want < 1 ? 1 : (want > kChunks ? kChunks : want));
@@ -518,6 +1237,98 @@ int normalise(const Stack& s, int batch, int m, int n, int ld, float eps, double
   if (rc != 0) return rc;
   return launch_pdl(ns_split_kernel<T>, dim3(chunks, batch), dim3(kNormThreads), 0, stream, s, m, n,
                     ld, vec, static_cast<const double*>(partial), eps, hi, lo);
+}
+
+bool fits_block(int m, int n) {
+  const int side = m < n ? m : n, longer = m < n ? n : m;
+  return side <= kBlockRows && longer <= kBlockCols;
+}
+
+template <typename T>
+int launch_block(const SflNewtonSchulz& a, const Stack& s, cudaStream_t stream) {
+  BlockParams p{};
+  p.u = s;
+  p.m = a.m;
+  p.n = a.n;
+  p.wide = a.m <= a.n;
+  p.steps = a.steps;
+  p.a = a.a;
+  p.b = a.b;
+  p.c = a.c;
+  p.eps = a.eps;
+  p.vec_in = rows_of_four<T>(s);
+  p.vec_out = a.n % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+  p.out = static_cast<__nv_bfloat16*>(a.out);
+  p.status = a.status;
+  const int longer = a.m < a.n ? a.n : a.m;
+  const int smem = 1024 + (2 + tiles_of(longer, 64)) * kBlockBytes;
+  const cudaError_t e = cudaFuncSetAttribute(
+      ns_block_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      1024 + (2 + kBlockCols / 64) * kBlockBytes);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  return launch_pdl(ns_block_kernel<T>, dim3(a.batch), dim3(kBlockThreads), smem, stream, p);
+}
+
+// Whether the chain is the faster way for matrices with a short side: it needs one Gram tile, and
+// its clusters walk the tiles of X one after the other where separate launches spread them over all
+// pairs.  In microseconds per step, fitted on B200 (see the measurements in chain_pays' caller):
+// launches cost 20 plus their waves, the chain 5 plus its serial tiles, per round of matrices.
+bool chain_pays(int batch, int side, int longer, int pairs) {
+  if (side > pair::kTileN || pairs < 1) return false;
+  const double tiles = tiles_of(longer, pair::kTileN), kb = tiles_of(longer, pair::kBK);
+  const double rounds = (batch + pairs - 1) / pairs;
+  const double waves = static_cast<double>(static_cast<long>(batch * tiles + pairs - 1) / pairs);
+  const double launches = 20.0 + rounds * 0.3 * kb + 3.0 * waves;
+  const double chain = rounds * (5.0 + 0.3 * kb + 3.0 * tiles);
+  return chain < launches;
+}
+
+int launch_chain(const SflNewtonSchulz& a, const Sizes& z, __half* const (&hi)[2], __half* lo,
+                 cudaStream_t stream) {
+  const int batch = a.batch, m = a.m, n = a.n;
+  const int side = m < n ? m : n, longer = m < n ? n : m;
+  const bool wide = m <= n;
+  const uint64_t x_stride = static_cast<uint64_t>(m) * z.ld;
+  ChainParams p{};
+  int rc = 0;
+  for (int i = 0; i < 2 && rc == 0; ++i) {
+    rc = pair::map_operand(&p.gram[i], hi[i], !wide, side, longer, z.ld, batch, x_stride);
+    if (rc == 0)
+      rc = pair::map_operand(&p.apply[i], hi[i], wide, longer, side, z.ld, batch, x_stride);
+    if (rc == 0) rc = pair::map_3d(&p.hi[i], hi[i], 2, n, m, z.ld, batch, x_stride, 64, 32);
+  }
+  if (rc == 0) rc = pair::map_3d(&p.lo, lo, 2, n, m, z.ld, batch, x_stride, 64, 32);
+  const bool out_tma = (static_cast<long>(n) * 2) % 16 == 0 &&
+                       (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
+  if (rc == 0 && out_tma)
+    rc = pair::map_3d(&p.out, a.out, 2, n, m, n, batch, static_cast<uint64_t>(m) * n, 64, 32);
+  if (rc != 0) return 1000 + rc;
+  p.batch = batch;
+  p.m = m;
+  p.n = n;
+  p.wide = wide;
+  p.steps = a.steps;
+  p.side_kb = tiles_of(side, pair::kBK);
+  p.long_kb = tiles_of(longer, pair::kBK);
+  p.tiles = tiles_of(longer, pair::kTileN);
+  p.last = out_tma ? 1 : 2;
+  p.a = a.a;
+  p.b = a.b;
+  p.c = a.c;
+  p.result = static_cast<__nv_bfloat16*>(a.out);
+  p.status = a.status;
+  int device = 0;
+  const int pairs = pair::sm_count_here(&device) / 2;
+  if (pairs < 1) return -1;
+  static bool configured[64] = {};
+  if (device >= 64 || !configured[device]) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        ns_chain_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kChainSmem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    if (device < 64) configured[device] = true;
+  }
+  const int clusters = batch < pairs ? batch : pairs;
+  return launch_pdl(ns_chain_kernel, dim3(2 * clusters), dim3(pair::kThreads), kChainSmem, stream, p);
 }
 
 }  // namespace
@@ -570,6 +1381,13 @@ extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {
   if (static_cast<long>(batch) * mt * nt > 0x7fffffffL) return -2;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
 
+  const Stack s{a->update, a->stride0, a->stride1, a->row, a->inner};
+  if (fits_block(m, n)) {
+    if (a->dtype == 0) return launch_block<__nv_bfloat16>(*a, s, stream);
+    if (a->dtype == 1) return launch_block<__half>(*a, s, stream);
+    return launch_block<float>(*a, s, stream);
+  }
+
   uint8_t* at = static_cast<uint8_t*>(a->work);
   __half* hi[2] = {reinterpret_cast<__half*>(at), reinterpret_cast<__half*>(at + z.x_bytes)};
   __half* lo = reinterpret_cast<__half*>(at + 2 * z.x_bytes);
@@ -577,7 +1395,6 @@ extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {
   __half* poly = reinterpret_cast<__half*>(at + 3 * z.x_bytes + z.gram_bytes);
   double* norms = reinterpret_cast<double*>(at + 3 * z.x_bytes + 2 * z.gram_bytes);
 
-  const Stack s{a->update, a->stride0, a->stride1, a->row, a->inner};
   int rc;
   const int ld = static_cast<int>(z.ld);
   __half* first_lo = a->steps > 2 ? lo : nullptr;  // folded steps read hi alone
@@ -589,6 +1406,9 @@ extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {
   const uint64_t x_stride = static_cast<uint64_t>(m) * z.ld;
   const uint64_t g_stride = static_cast<uint64_t>(side) * z.gram_ld;
   const int gt = tiles_of(side, pair::kTileN);
+
+  if (chain_pays(batch, side, longer, pair::pairs_here()))
+    return launch_chain(*a, z, hi, lo, stream);
 
   SymOp::Params q{};
   q.fp16 = true;
