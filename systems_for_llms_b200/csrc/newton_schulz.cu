@@ -526,78 +526,48 @@ __device__ __forceinline__ void kept(uint8_t* block, int row, int half, float (&
   }
 }
 
-// ------------------------------------ all steps of a matrix with a short side in one kernel ----
-// A matrix whose shorter side is at most 256 has one Gram tile: a cluster computes it, keeps G and
-// then P in the shared memory of its two CTAs as operands of the next product, and walks the tiles
-// of X, step after step, with X alone going through global memory.  Fifteen launches that each wait
-// for the one before (6.7 to 10 us apiece, most of it start and drain) become one.
+// ------------------------------------------- G and P of a short side in one kernel ----
+// Where the shorter side is at most 256 the Gram matrix is one tile: a cluster keeps it in the
+// shared memory of its two CTAs, squares it there and stores P alone.  Two dependent launches per
+// step instead of three (256 x 512: 123 -> 105 us for five steps), and G never leaves the SM.
 //
-// Roles as in pair_kernel.  Ring stages hold 128 rows x 64 (16 KB per CTA): the Gram product reads
-// the same rows as both operands, the others read P from the G / P buffer, four 64-column blocks of
-// 128 rows per CTA - a CTA's rows as A, both CTAs' as the 256 rows of B.  Barriers beyond
-// pair_kernel's: op_ready (leader: all sixteen epilogue warps have written G, or P) and x_ready
-// (both CTAs: all of the step's stores are complete, the next step may load).
-constexpr int kChainStages = 5;
-constexpr int kChainStageBytes = pair::kABytes;
-constexpr int kChainOpBytes = 4 * pair::kABytes;
-constexpr int kChainWarpBytes = 2 * pair::kEpiTileBytes;
-constexpr int kChainSmem = 1024 + kChainStages * kChainStageBytes + kChainOpBytes +
-                           pair::kEpiWarps * kChainWarpBytes + 512;
-static_assert(kChainSmem <= 232448, "more than a CTA's shared memory");
+// Roles as in pair_kernel.  A ring stage holds 128 rows x 64 of X, both operands of the Gram
+// product.  G lies as four 64-column blocks of 128 rows per CTA - a CTA's rows as A, both CTAs' as
+// the 256 rows of B.  op_ready (leader's): all sixteen epilogue warps have written G.
+constexpr int kPolyStages = 6;
+constexpr int kPolyStageBytes = pair::kABytes;
+constexpr int kPolyWarpBytes = 2 * pair::kEpiTileBytes;
+constexpr int kPolySmem = 1024 + kPolyStages * kPolyStageBytes + 4 * pair::kABytes +
+                          pair::kEpiWarps * kPolyWarpBytes + 512;
+static_assert(kPolySmem <= 232448, "more than a CTA's shared memory");
 
-struct ChainParams {
-  CUtensorMap gram[2];      // X as the Gram product's operand (ping, pong)
-  CUtensorMap apply[2];     // X as the other product's operand
-  CUtensorMap hi[2], lo;    // 64-column lines of 32 rows
-  CUtensorMap out;
-  int batch, m, n, wide, steps;
+struct PolyParams {
+  CUtensorMap x;            // X as the Gram product's operand
+  CUtensorMap out;          // P in 64-column lines of 32 rows
+  int batch, size, wide;
   int side_kb, long_kb;     // 64-deep steps of the shorter and the longer side
-  int tiles;                // 256-wide tiles along the longer side
-  int last;                 // 1: result through TMA, 2: element by element
-  float a, b, c;
-  __nv_bfloat16* result;
+  float b, c, shift;
   int* status;
 };
 
-struct __align__(8) ChainBarriers {
-  uint64_t full[kChainStages];
-  uint64_t empty[kChainStages];
-  uint64_t acc_full[2];
-  uint64_t acc_empty[2];
+struct __align__(8) PolyBarriers {
+  uint64_t full[kPolyStages];
+  uint64_t empty[kPolyStages];
+  uint64_t acc_full[2];     // G, G G
+  uint64_t acc_empty;       // both have been read
   uint64_t op_ready;
-  uint64_t x_ready;
-  uint64_t aux_full[pair::kEpiWarps];
   uint32_t tmem_base;
   int abort;
 };
 
-// Orders this thread's later asynchronous (TMA) accesses after what others did before, and others'
-// after what it did: between generic-proxy synchronisation and the async proxy.
-__device__ __forceinline__ void fence_proxy_async_all() {
-  asm volatile("fence.proxy.async;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-__device__ __forceinline__ void arrive_release(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
-               : "memory");
-}
-__device__ __forceinline__ void acquire_cluster() {
-  asm volatile("fence.acq_rel.cluster;" ::: "memory");
-}
-
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(pair::kThreads, 1)
-ns_chain_kernel(const __grid_constant__ ChainParams p) {
+ns_poly_kernel(const __grid_constant__ PolyParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
-  uint8_t* op = smem + kChainStages * kChainStageBytes;  // G, then P
-  uint8_t* epi_smem = op + kChainOpBytes;
-  ChainBarriers* bars =
-      reinterpret_cast<ChainBarriers*>(epi_smem + pair::kEpiWarps * kChainWarpBytes);
+  uint8_t* op = smem + kPolyStages * kPolyStageBytes;  // G
+  uint8_t* epi_smem = op + 4 * pair::kABytes;
+  PolyBarriers* bars = reinterpret_cast<PolyBarriers*>(epi_smem + pair::kEpiWarps * kPolyWarpBytes);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = pair::cluster_rank();
@@ -606,17 +576,14 @@ ns_chain_kernel(const __grid_constant__ ChainParams p) {
   volatile int* abort = &bars->abort;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kChainStages; ++s) {
+    for (int s = 0; s < kPolyStages; ++s) {
       mbar_init(&bars->full[s], 1);
       mbar_init(&bars->empty[s], 1);
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars->acc_full[s], 1);
-      mbar_init(&bars->acc_empty[s], 2 * pair::kEpiWarps);
-    }
+    mbar_init(&bars->acc_full[0], 1);
+    mbar_init(&bars->acc_full[1], 1);
+    mbar_init(&bars->acc_empty, 2 * pair::kEpiWarps);
     mbar_init(&bars->op_ready, 2 * pair::kEpiWarps);
-    mbar_init(&bars->x_ready, 2 * pair::kEpiWarps);
-    for (int s = 0; s < pair::kEpiWarps; ++s) mbar_init(&bars->aux_full[s], 1);
     bars->abort = 0;
     mbar_fence_init();
   }
@@ -635,65 +602,45 @@ ns_chain_kernel(const __grid_constant__ ChainParams p) {
   pdl_launch_dependents();
   pdl_wait();
 
-  auto give_up = [&](int code) {
+  auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+    if (pair::wait_or_leave(bar, parity, abort)) return true;
     if (lane == 0) report_status(p.status, code);
     *abort = 1;
+    return false;
   };
 
   if (warp == 0) {
     // ------------------------------------------------------ TMA producer ----
     int stage = 0;
-    uint32_t phase = 0, x_phase = 0;
+    uint32_t phase = 0;
     bool ok = true;
     const uint32_t full0 = pair::in_leader(smem_u32(&bars->full[0]));
-    // one stage: a box of 128 rows x 64 (K-major) or two of 64 x 64 (MN-major)
-    auto bring = [&](const CUtensorMap* map, bool mn, int rows0, int k0, int z) {
-      if (!pair::wait_or_leave(&bars->empty[stage], phase ^ 1, abort)) {
-        give_up(kStatusTimeoutEmpty);
-        return false;
-      }
-      uint8_t* at = smem + stage * kChainStageBytes;
-      const uint32_t bar = full0 + stage * static_cast<uint32_t>(sizeof(uint64_t));
-      if (elect_one()) {
-        if (rank == 0) mbar_expect_tx(&bars->full[stage], 2 * kChainStageBytes);
-        if (mn) {
-          pair::load_3d(at, map, bar, rows0, k0, z);
-          pair::load_3d(at + pair::kBK * 128, map, bar, rows0 + 64, k0, z);
-        } else {
-          pair::load_3d(at, map, bar, k0, rows0, z);
-        }
-      }
-      __syncwarp();
-      if (++stage == kChainStages) {
-        stage = 0;
-        phase ^= 1;
-      }
-      return true;
-    };
-    const int mine = rank * pair::kCtaM;
+    const int rows0 = rank * pair::kCtaM;
     for (int z = cluster; z < p.batch && ok; z += clusters) {
-      for (int step = 0; step < p.steps && ok; ++step) {
-        const int now = step & 1;
-        if (step > 0) {
-          if (!pair::wait_or_leave(&bars->x_ready, x_phase, abort)) {
-            give_up(kStatusTimeoutEmpty);
-            ok = false;
-            break;
+      for (int kb = 0; kb < p.long_kb; ++kb) {
+        ok = wait(&bars->empty[stage], phase ^ 1, kStatusTimeoutEmpty);
+        if (!ok) break;
+        uint8_t* at = smem + stage * kPolyStageBytes;
+        const uint32_t bar = full0 + stage * static_cast<uint32_t>(sizeof(uint64_t));
+        if (elect_one()) {
+          if (rank == 0) mbar_expect_tx(&bars->full[stage], 2 * kPolyStageBytes);
+          if (p.wide) {
+            pair::load_3d(at, &p.x, bar, kb * pair::kBK, rows0, z);
+          } else {
+            pair::load_3d(at, &p.x, bar, rows0, kb * pair::kBK, z);
+            pair::load_3d(at + pair::kBK * 128, &p.x, bar, rows0 + 64, kb * pair::kBK, z);
           }
-          acquire_cluster();
-          fence_proxy_async_all();
-          x_phase ^= 1;
         }
-        for (int kb = 0; kb < p.long_kb && ok; ++kb)
-          ok = bring(&p.gram[now], !p.wide, mine, kb * pair::kBK, z);
-        for (int t = 0; t < p.tiles && ok; ++t)
-          for (int kb = 0; kb < p.side_kb && ok; ++kb)
-            ok = bring(&p.apply[now], p.wide, t * pair::kTileN + mine, kb * pair::kBK, z);
+        __syncwarp();
+        if (++stage == kPolyStages) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
     }
-    for (int s = 0; s < kChainStages; ++s) {  // as in pair_kernel
+    for (int s = 0; s < kPolyStages; ++s) {  // as in pair_kernel
       if (!mbar_wait(&bars->empty[stage], phase ^ 1)) break;
-      if (++stage == kChainStages) {
+      if (++stage == kPolyStages) {
         stage = 0;
         phase ^= 1;
       }
@@ -701,211 +648,125 @@ ns_chain_kernel(const __grid_constant__ ChainParams p) {
   } else if (warp == 1) {
     // -------------------------------------------------------- MMA issuer ----
     if (rank == 0) {
-      const uint32_t base = smem_u32(smem);
-      const uint64_t k0 = umma_smem_desc(base, 16, 1024);
-      const uint64_t mn0 = umma_smem_desc(base, pair::kBK * 128, 1024);
+      const uint64_t k0 = umma_smem_desc(smem_u32(smem), 16, 1024);
+      const uint64_t mn0 = umma_smem_desc(smem_u32(smem), pair::kBK * 128, 1024);
       const uint64_t op0 = umma_smem_desc(smem_u32(op), 16, 1024);
       int stage = 0;
-      uint32_t phase = 0, op_phase = 0;
-      uint32_t uses[2] = {0, 0};  // of each accumulator by the tiles of X
+      uint32_t phase = 0, round = 0;
       bool ok = true;
-      // A stage of the ring times itself (kRing = 2), or as A (0) / B (1) with a block of P
-      auto step_of = [&](auto a_mn, auto b_mn, auto ring, uint32_t d, uint64_t op_block, bool more,
-                         uint64_t* done) {
-        constexpr bool kA = decltype(a_mn)::value, kB = decltype(b_mn)::value;
-        constexpr int kRing = decltype(ring)::value;
-        if (!pair::wait_or_leave(&bars->full[stage], phase, abort)) {
-          give_up(kStatusTimeoutFull);
-          return false;
-        }
-        tc_fence_after();
-        const uint64_t mine = umma_desc_advance((kRing == 1 ? kB : kA) ? mn0 : k0,
-                                                stage * kChainStageBytes);
-        const uint64_t a = kRing == 1 ? op_block : mine;
-        const uint64_t b = kRing == 0 ? op_block : mine;
-        const uint32_t idesc = pair::instruction_descriptor(true, kA, kB);
-        if (elect_one()) {
+      auto square = [&](auto mn, uint64_t at, uint32_t d, bool more) {
+        constexpr bool kMn = decltype(mn)::value;
+        const uint32_t idesc = pair::instruction_descriptor(true, kMn, kMn);
 #pragma unroll
-          for (int k = 0; k < pair::kBK / 16; ++k)
-            pair::mma_pair(d, umma_desc_advance(a, k * (kA ? 2048 : 32)),
-                           umma_desc_advance(b, k * (kB ? 2048 : 32)), idesc, more || k != 0);
-          pair::commit_pair(&bars->empty[stage]);
-          if (done != nullptr) pair::commit_pair(done);
+        for (int k = 0; k < pair::kBK / 16; ++k) {
+          const uint64_t both = umma_desc_advance(at, k * (kMn ? 2048 : 32));
+          pair::mma_pair(d, both, both, idesc, more || k != 0);
         }
-        __syncwarp();
-        if (++stage == kChainStages) {
-          stage = 0;
-          phase ^= 1;
-        }
-        return true;
       };
-      auto wait_op = [&] {
-        if (!pair::wait_or_leave(&bars->op_ready, op_phase, abort)) {
-          give_up(kStatusTimeoutTmemEmpty);
-          return false;
+      for (int z = cluster; z < p.batch && ok; z += clusters, ++round) {
+        if (round > 0) {
+          ok = wait(&bars->acc_empty, (round - 1) & 1, kStatusTimeoutTmemEmpty);
+          tc_fence_after();
         }
-        acquire_cluster();
-        tc_fence_after();
-        op_phase ^= 1;
-        return true;
-      };
-      auto wait_acc = [&](int acc) {
-        if (uses[acc] == 0) return true;
-        if (!pair::wait_or_leave(&bars->acc_empty[acc], (uses[acc] - 1) & 1, abort)) {
-          give_up(kStatusTimeoutTmemEmpty);
-          return false;
-        }
-        tc_fence_after();
-        return true;
-      };
-      const std::true_type mn;
-      const std::false_type km;
-      const std::integral_constant<int, 0> as_a;
-      const std::integral_constant<int, 1> as_b;
-      const std::integral_constant<int, 2> itself;
-      for (int z = cluster; z < p.batch && ok; z += clusters) {
-        for (int step = 0; step < p.steps && ok; ++step) {
-          ok = wait_acc(0);
-          for (int kb = 0; kb < p.long_kb && ok; ++kb) {
-            uint64_t* done = kb + 1 == p.long_kb ? &bars->acc_full[0] : nullptr;
-            ok = p.wide ? step_of(km, km, itself, tmem_base, 0, kb != 0, done)
-                        : step_of(mn, mn, itself, tmem_base, 0, kb != 0, done);
-          }
-          ok = ok && wait_op();
+        for (int kb = 0; kb < p.long_kb && ok; ++kb) {
+          ok = wait(&bars->full[stage], phase, kStatusTimeoutFull);
           if (!ok) break;
-          if (elect_one()) {  // G G from shared memory
-            const uint32_t idesc = pair::instruction_descriptor(true, false, false);
-            for (int kb = 0; kb < p.side_kb; ++kb) {
-              const uint64_t g = umma_desc_advance(op0, kb * pair::kABytes);
-#pragma unroll
-              for (int k = 0; k < pair::kBK / 16; ++k)
-                pair::mma_pair(tmem_base + pair::kTileN, umma_desc_advance(g, k * 32),
-                               umma_desc_advance(g, k * 32), idesc, (kb | k) != 0);
-            }
-            pair::commit_pair(&bars->acc_full[1]);
+          tc_fence_after();
+          const uint64_t at = umma_desc_advance(p.wide ? k0 : mn0, stage * kPolyStageBytes);
+          if (elect_one()) {
+            if (p.wide) square(std::false_type(), at, tmem_base, kb != 0);
+            else square(std::true_type(), at, tmem_base, kb != 0);
+            pair::commit_pair(&bars->empty[stage]);
+            if (kb + 1 == p.long_kb) pair::commit_pair(&bars->acc_full[0]);
           }
           __syncwarp();
-          ok = wait_op();
-          for (int t = 0; t < p.tiles && ok; ++t) {
-            const int acc = t & 1;
-            ok = wait_acc(acc);
-            ++uses[acc];
-            for (int kb = 0; kb < p.side_kb && ok; ++kb) {
-              uint64_t* done = kb + 1 == p.side_kb ? &bars->acc_full[acc] : nullptr;
-              const uint32_t d = tmem_base + acc * pair::kTileN;
-              const uint64_t block = umma_desc_advance(op0, kb * pair::kABytes);
-              ok = p.wide ? step_of(km, mn, as_b, d, block, kb != 0, done)
-                          : step_of(km, km, as_a, d, block, kb != 0, done);
-            }
+          if (++stage == kPolyStages) {
+            stage = 0;
+            phase ^= 1;
           }
         }
+        ok = ok && wait(&bars->op_ready, round & 1, kStatusTimeoutTmemEmpty);
+        if (!ok) break;
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
+        tc_fence_after();
+        if (elect_one()) {
+          for (int kb = 0; kb < p.side_kb; ++kb)
+            square(std::false_type(), umma_desc_advance(op0, kb * pair::kABytes),
+                   tmem_base + pair::kTileN, kb != 0);
+          pair::commit_pair(&bars->acc_full[1]);
+        }
+        __syncwarp();
       }
     }
   } else {
     // ---------------------------------------------------------- epilogue ----
-    const int quarter = warp & 3;
-    EpiContext c;
-    c.part = (warp - 2) >> 2;
-    c.lane = lane;
-    c.smem = epi_smem + (warp - 2) * kChainWarpBytes;
-    c.aux_bar = &bars->aux_full[warp - 2];
-    c.aux_phase = 0;
-    c.abort = abort;
-    c.status = p.status;
+    const int quarter = warp & 3, part = (warp - 2) >> 2;
+    uint8_t* staging = epi_smem + (warp - 2) * kPolyWarpBytes;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t op_ready = pair::in_leader(smem_u32(&bars->op_ready));
-    const int row = quarter * 32 + lane;            // of this CTA's 128 rows of G and P
-    const int diagonal = rank * pair::kCtaM + row;  // their column on the diagonal
-    uint32_t full_phase[2] = {0, 0};
-    bool ok = true;
-    auto wait_full = [&](int acc) {
-      if (!pair::wait_or_leave(&bars->acc_full[acc], full_phase[acc], abort)) {
-        give_up(kStatusTimeoutTmemFull);
-        return false;
-      }
-      full_phase[acc] ^= 1;
+    const int row = quarter * 32 + lane;            // of this CTA's 128 rows
+    const int row0 = rank * pair::kCtaM + quarter * 32;
+    const int cols = p.side_kb * pair::kBK;         // columns of G that are multiplied
+    uint32_t phase = 0;
+    for (int z = cluster; z < p.batch; z += clusters, phase ^= 1) {
+      if (!wait(&bars->acc_full[0], phase, kStatusTimeoutTmemFull)) break;
       tc_fence_after();
-      return true;
-    };
-    auto keep = [&](int col, const float (&v)[32]) {  // into the G / P buffer
-      pair::stage_16(op + (col >> 6) * pair::kABytes, row, (col >> 5) & 1, v, true);
-    };
-    auto op_written = [&] {
-      fence_proxy_async_all();
+#pragma unroll 1
+      for (int ch = 0; ch < 4; ++ch) {
+        const int col = part * 128 + ch * 32;
+        if (col >= cols) break;  // warp-uniform
+        float v[32];
+        pair::load_acc(tmem_base + lanes + col, v);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] *= 1.0f / kScale;
+        pair::stage_16(op + (col >> 6) * pair::kABytes, row, (col >> 5) & 1, v, true);
+      }
+      // both CTAs' shared memory is read by the products that the leader issues
+      asm volatile("fence.proxy.async;" ::: "memory");
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_release(op_ready);
-    };
-    const int cols = p.side_kb * pair::kBK;  // columns of G and P that the products read
-    for (int z = cluster; z < p.batch && ok; z += clusters) {
-      for (int step = 0; step < p.steps && ok; ++step) {
-        const bool folded = step + 2 >= p.steps, last = step + 1 == p.steps;
-        ok = wait_full(0);
-        if (!ok) break;
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(op_ready)
+                     : "memory");
+      if (!wait(&bars->acc_full[1], phase, kStatusTimeoutTmemFull)) break;
+      tc_fence_after();
 #pragma unroll 1
-        for (int ch = 0; ch < 4; ++ch) {
-          const int col = c.part * 128 + ch * 32;
-          if (col >= cols) break;  // warp-uniform
-          float v[32];
-          pair::load_acc(tmem_base + lanes + col, v);
+      for (int ch = 0; ch < 2; ++ch) {
+        const int begin = part * 128 + ch * 64;
+        if (begin >= p.size || row0 >= p.size) break;  // warp-uniform
+        uint8_t* tile = staging + ch * pair::kEpiTileBytes;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] *= 1.0f / kScale;
-          keep(col, v);
-        }
-        op_written();
-        ok = wait_full(1);
-        if (!ok) break;
-#pragma unroll 1
-        for (int ch = 0; ch < 4; ++ch) {
-          const int col = c.part * 128 + ch * 32;
-          if (col >= cols) break;  // warp-uniform
-          float v[32];
-          {
-            // the rounded G that was multiplied: b and c must see the same matrix, or its rounding
-            // enters with the slope of c G G alone
-            float g[32];
-            kept(op + (col >> 6) * pair::kABytes, row, (col >> 5) & 1, g);
-            pair::load_acc(tmem_base + pair::kTileN + lanes + col, v);
+        for (int h = 0; h < 2; ++h) {
+          const int col = begin + h * 32;
+          float v[32], g[32];
+          // the rounded G that was multiplied: b and c must see the same matrix, or its rounding
+          // enters with the slope of c G G alone
+          kept(op + (col >> 6) * pair::kABytes, row, h, g);
+          pair::load_acc(tmem_base + pair::kTileN + lanes + col, v);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = fmaf(v[j], p.c / kScale, g[j] * p.b);
+          for (int j = 0; j < 32; ++j) {
+            v[j] = fmaf(v[j], p.c / kScale, g[j] * p.b);
+            if (col + j == row0 + lane) v[j] += p.shift;
           }
-          if (folded) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (col + j == diagonal) v[j] += p.a * kScale;
+          if (h == 0) {
+            if (lane == 0) {
+              if (ch == 0) tma_store_wait_read<0>();
+              else tma_store_wait_read<1>();
+            }
+            __syncwarp();
           }
-          keep(col, v);
+          pair::stage_16(tile, lane, h, v, true);
         }
-        op_written();
-        const float unscale = last ? 1.0f / kScale : 1.0f;
-        const ApplyView view{&p.hi[step & 1], &p.lo, &p.hi[(step + 1) & 1], &p.out, p.m, p.n, folded,
-                             step + 3 < p.steps, last ? p.last : 0, folded ? 0.f : p.a * unscale,
-                             unscale / kScale, p.result};
-        for (int t = 0; t < p.tiles && ok; ++t) {
-          const int acc = t & 1;
-          const Tile tile{p.wide ? 0 : t * pair::kTileM, p.wide ? t * pair::kTileN : 0, z, 0, 0, 0,
-                          0, 0, false};
-          c.acc = tmem_base + lanes + acc * pair::kTileN;
-          c.row0 = tile.m0 + rank * pair::kCtaM + quarter * 32;
-          apply_begin(view, tile, c);
-          ok = wait_full(acc);
-          if (!ok) break;
-          apply_epilogue(view, tile, c);
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) pair::arrive_leader(&bars->acc_empty[acc]);
-        }
-        if (!last) {
-          if (lane == 0) {
-            tma_store_wait<0>();  // the stores are complete, not only read
-            fence_proxy_async_all();
-            const uint32_t ready = smem_u32(&bars->x_ready);
-            arrive_release(in_cta(ready, 0));
-            arrive_release(in_cta(ready, 1));
-          }
-          __syncwarp();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          pair::store_3d(&p.out, tile, begin, row0, z);
+          tma_store_commit();
         }
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) pair::arrive_leader(&bars->acc_empty);
     }
     if (lane == 0) tma_store_wait<0>();
   }
@@ -1269,66 +1130,19 @@ int launch_block(const SflNewtonSchulz& a, const Stack& s, cudaStream_t stream) 
   return launch_pdl(ns_block_kernel<T>, dim3(a.batch), dim3(kBlockThreads), smem, stream, p);
 }
 
-// Whether the chain is the faster way for matrices with a short side: it needs one Gram tile, and
-// its clusters walk the tiles of X one after the other where separate launches spread them over all
-// pairs.  In microseconds per step, fitted on B200 (see the measurements in chain_pays' caller):
-// launches cost 20 plus their waves, the chain 5 plus its serial tiles, per round of matrices.
-bool chain_pays(int batch, int side, int longer, int pairs) {
-  if (side > pair::kTileN || pairs < 1) return false;
-  const double tiles = tiles_of(longer, pair::kTileN), kb = tiles_of(longer, pair::kBK);
-  const double rounds = (batch + pairs - 1) / pairs;
-  const double waves = static_cast<double>(static_cast<long>(batch * tiles + pairs - 1) / pairs);
-  const double launches = 20.0 + rounds * 0.3 * kb + 3.0 * waves;
-  const double chain = rounds * (5.0 + 0.3 * kb + 3.0 * tiles);
-  return chain < launches;
-}
-
-int launch_chain(const SflNewtonSchulz& a, const Sizes& z, __half* const (&hi)[2], __half* lo,
-                 cudaStream_t stream) {
-  const int batch = a.batch, m = a.m, n = a.n;
-  const int side = m < n ? m : n, longer = m < n ? n : m;
-  const bool wide = m <= n;
-  const uint64_t x_stride = static_cast<uint64_t>(m) * z.ld;
-  ChainParams p{};
-  int rc = 0;
-  for (int i = 0; i < 2 && rc == 0; ++i) {
-    rc = pair::map_operand(&p.gram[i], hi[i], !wide, side, longer, z.ld, batch, x_stride);
-    if (rc == 0)
-      rc = pair::map_operand(&p.apply[i], hi[i], wide, longer, side, z.ld, batch, x_stride);
-    if (rc == 0) rc = pair::map_3d(&p.hi[i], hi[i], 2, n, m, z.ld, batch, x_stride, 64, 32);
-  }
-  if (rc == 0) rc = pair::map_3d(&p.lo, lo, 2, n, m, z.ld, batch, x_stride, 64, 32);
-  const bool out_tma = (static_cast<long>(n) * 2) % 16 == 0 &&
-                       (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
-  if (rc == 0 && out_tma)
-    rc = pair::map_3d(&p.out, a.out, 2, n, m, n, batch, static_cast<uint64_t>(m) * n, 64, 32);
-  if (rc != 0) return 1000 + rc;
-  p.batch = batch;
-  p.m = m;
-  p.n = n;
-  p.wide = wide;
-  p.steps = a.steps;
-  p.side_kb = tiles_of(side, pair::kBK);
-  p.long_kb = tiles_of(longer, pair::kBK);
-  p.tiles = tiles_of(longer, pair::kTileN);
-  p.last = out_tma ? 1 : 2;
-  p.a = a.a;
-  p.b = a.b;
-  p.c = a.c;
-  p.result = static_cast<__nv_bfloat16*>(a.out);
-  p.status = a.status;
+int launch_poly(const PolyParams& p, cudaStream_t stream) {
   int device = 0;
   const int pairs = pair::sm_count_here(&device) / 2;
   if (pairs < 1) return -1;
   static bool configured[64] = {};
   if (device >= 64 || !configured[device]) {
     const cudaError_t e = cudaFuncSetAttribute(
-        ns_chain_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kChainSmem);
+        ns_poly_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPolySmem);
     if (e != cudaSuccess) return static_cast<int>(e);
     if (device < 64) configured[device] = true;
   }
-  const int clusters = batch < pairs ? batch : pairs;
-  return launch_pdl(ns_chain_kernel, dim3(2 * clusters), dim3(pair::kThreads), kChainSmem, stream, p);
+  const int clusters = p.batch < pairs ? p.batch : pairs;
+  return launch_pdl(ns_poly_kernel, dim3(2 * clusters), dim3(pair::kThreads), kPolySmem, stream, p);
 }
 
 }  // namespace
@@ -1407,9 +1221,6 @@ extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {
   const uint64_t g_stride = static_cast<uint64_t>(side) * z.gram_ld;
   const int gt = tiles_of(side, pair::kTileN);
 
-  if (chain_pays(batch, side, longer, pair::pairs_here()))
-    return launch_chain(*a, z, hi, lo, stream);
-
   SymOp::Params q{};
   q.fp16 = true;
   q.status = a->status;
@@ -1449,33 +1260,51 @@ extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {
   for (int step = 0; step < a->steps; ++step) {
     __half* now = hi[step & 1];
     __half* next = hi[(step + 1) & 1];
-    // G = X X^T (wide: X is K-major) or X^T X (tall: X read MN-major)
-    q.gram = 1;
-    q.mn = !wide;
-    q.num_kb = tiles_of(longer, pair::kBK);
-    q.alpha = 0.f;
-    q.beta = 1.0f / kScale;
-    q.shift = 0.f;
-    rc = pair::map_operand(wide ? &q.k_major : &q.mn_major, now, !wide, side, longer, z.ld, batch,
-                           x_stride);
-    if (rc == 0) rc = gram_map(&q.out, gram);
-    if (rc != 0) return 1000 + rc;
-    rc = pair::launch_pair<SymOp>(q, stream);
-    if (rc != 0) return rc;
-    // P = b G + c G G (+ a I)
     const bool folded = step + 2 >= a->steps;
     const float k = folded ? a->a : 0.f;
-    q.gram = 0;
-    q.num_kb = tiles_of(side, pair::kBK);
-    q.alpha = a->b;
-    q.beta = a->c / kScale;
-    q.shift = k * kScale;
-    q.aux = q.out;
-    rc = symmetric(&q.k_major, &q.mn_major, gram);
-    if (rc == 0) rc = gram_map(&q.out, poly);
-    if (rc != 0) return 1000 + rc;
-    rc = pair::launch_pair<SymOp>(q, stream);
-    if (rc != 0) return rc;
+    if (side <= pair::kTileN) {
+      PolyParams g{};
+      rc = pair::map_operand(&g.x, now, !wide, side, longer, z.ld, batch, x_stride);
+      if (rc == 0) rc = gram_map(&g.out, poly);
+      if (rc != 0) return 1000 + rc;
+      g.batch = batch;
+      g.size = side;
+      g.wide = wide;
+      g.side_kb = tiles_of(side, pair::kBK);
+      g.long_kb = tiles_of(longer, pair::kBK);
+      g.b = a->b;
+      g.c = a->c;
+      g.shift = k * kScale;
+      g.status = a->status;
+      rc = launch_poly(g, stream);
+      if (rc != 0) return rc;
+    } else {
+      // G = X X^T (wide: X is K-major) or X^T X (tall: X read MN-major)
+      q.gram = 1;
+      q.mn = !wide;
+      q.num_kb = tiles_of(longer, pair::kBK);
+      q.alpha = 0.f;
+      q.beta = 1.0f / kScale;
+      q.shift = 0.f;
+      rc = pair::map_operand(wide ? &q.k_major : &q.mn_major, now, !wide, side, longer, z.ld, batch,
+                             x_stride);
+      if (rc == 0) rc = gram_map(&q.out, gram);
+      if (rc != 0) return 1000 + rc;
+      rc = pair::launch_pair<SymOp>(q, stream);
+      if (rc != 0) return rc;
+      // P = b G + c G G (+ a I)
+      q.gram = 0;
+      q.num_kb = tiles_of(side, pair::kBK);
+      q.alpha = a->b;
+      q.beta = a->c / kScale;
+      q.shift = k * kScale;
+      q.aux = q.out;
+      rc = symmetric(&q.k_major, &q.mn_major, gram);
+      if (rc == 0) rc = gram_map(&q.out, poly);
+      if (rc != 0) return 1000 + rc;
+      rc = pair::launch_pair<SymOp>(q, stream);
+      if (rc != 0) return rc;
+    }
     // X <- a X + P X (wide) or a X + X P (tall; P is symmetric)
     const bool last = step + 1 == a->steps;
     x.last = !last ? 0 : (out_tma ? 1 : 2);
