@@ -25,6 +25,9 @@
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
+#include <string.h>
+
+#include <type_traits>
 
 #include "launch.cuh"
 #include "ptx.cuh"
@@ -71,10 +74,6 @@ struct RotaryParams {
   float* partial;     // backward with norm: [blocks, D]
 };
 
-template <typename T> __device__ __forceinline__ float to_f32(T v);
-template <> __device__ __forceinline__ float to_f32(float v) { return v; }
-template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ float from_f32(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) {
@@ -92,22 +91,44 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// The eight elements as they lie in memory; converted to fp32 only when they are used, so that
-// loads in flight hold 16 bytes (32 for fp32) of registers per lane.
-template <typename T> struct Raw { T v[kVec]; };
+// The eight elements as they lie in memory, in 32-bit words; converted to fp32 only when they are
+// used, so that loads in flight hold 16 bytes (32 for fp32) of registers per lane.  Conversions
+// work on words: one shift or mask per bf16 number instead of an extraction and a shift.
+template <typename T> struct Raw { uint32_t w[kVec * sizeof(T) / 4]; };
+
+template <typename T>
+__device__ __forceinline__ void unpack(const Raw<T>& r, float (&f)[kVec]) {
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(r.w) / 4); ++i) {
+    if constexpr (sizeof(T) == 4) {
+      f[i] = __uint_as_float(r.w[i]);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
+      f[2 * i] = v.x;
+      f[2 * i + 1] = v.y;
+    } else {
+      f[2 * i] = __uint_as_float(r.w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
+    }
+  }
+}
 
 template <bool VEC, typename T>
 __device__ __forceinline__ void load_raw(Raw<T>& r, const T* row, int e0, int D, bool live) {
+  constexpr int kQuads = static_cast<int>(sizeof(r.w) / 16);
   if constexpr (VEC) {
     const uint4* src = reinterpret_cast<const uint4*>(row + e0);
-    uint4* dst = reinterpret_cast<uint4*>(r.v);
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(Raw<T>) / 16); ++i)
-      dst[i] = live ? src[i] : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < kQuads; ++i) {
+      const uint4 q = live ? src[i] : make_uint4(0, 0, 0, 0);
+      r.w[4 * i] = q.x; r.w[4 * i + 1] = q.y; r.w[4 * i + 2] = q.z; r.w[4 * i + 3] = q.w;
+    }
   } else {
+    T v[kVec];
 #pragma unroll
     for (int i = 0; i < kVec; ++i)
-      r.v[i] = live && e0 + i < D ? row[e0 + i] : from_f32<T>(0.f);
+      v[i] = live && e0 + i < D ? row[e0 + i] : from_f32<T>(0.f);
+    memcpy(r.w, v, sizeof(v));
   }
 }
 
@@ -189,42 +210,43 @@ __device__ __forceinline__ void partners(const RotaryParams& p, const Raw<T>& mi
     const int half = p.rotated >> 1;
     const bool turns = e0 < p.rotated;
     const int src = turns ? (e0 < half ? lane + half / kVec : lane - half / kVec) : lane;
-    constexpr int kWords = static_cast<int>(sizeof(Raw<T>) / 4);
-    const uint32_t* from = reinterpret_cast<const uint32_t*>(mine.v);
-    uint32_t* to = reinterpret_cast<uint32_t*>(other.v);
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) {
-      const uint32_t got = __shfl_sync(0xffffffffu, from[i], src);
-      to[i] = turns ? got : 0u;
+    for (int i = 0; i < static_cast<int>(sizeof(mine.w) / 4); ++i) {
+      const uint32_t got = __shfl_sync(0xffffffffu, mine.w[i], src);
+      other.w[i] = turns ? got : 0u;
     }
   } else if constexpr (PAIR == kHalfShared) {
     const int half = p.rotated >> 1;
     const T* head = strip + (lane * kVec - e0);  // the head's first element
     __syncwarp();
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) strip[lane * kVec + i] = mine.v[i];
+    memcpy(strip + lane * kVec, mine.w, sizeof(mine.w));
     __syncwarp();
+    T v[kVec];
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
       const int e = e0 + i;
-      other.v[i] = e < p.rotated ? head[e < half ? e + half : e - half] : from_f32<T>(0.f);
+      v[i] = e < p.rotated ? head[e < half ? e + half : e - half] : from_f32<T>(0.f);
     }
+    memcpy(other.w, v, sizeof(v));
   }
 }
 
 // f_e = own_e C_e + partner_e S_e
 template <typename T, int PAIR>
-__device__ __forceinline__ void combine(const RotaryParams& p, const Raw<T>& mine,
+__device__ __forceinline__ void combine(const RotaryParams& p, const float (&own)[kVec],
                                         const Raw<T>& other, const float (&C)[kVec],
                                         const float (&S)[kVec], int e0, float (&f)[kVec]) {
+  if constexpr (PAIR == kInterleaved) {
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) {
-    if constexpr (PAIR == kInterleaved) {
-      f[i] = to_f32(mine.v[i]) * C[i];
-      if (e0 + (i & ~1) < p.rotated) f[i] = fmaf(to_f32(mine.v[i ^ 1]), S[i], f[i]);
-    } else {
-      f[i] = fmaf(to_f32(other.v[i]), S[i], to_f32(mine.v[i]) * C[i]);
+    for (int i = 0; i < kVec; ++i) {
+      f[i] = own[i] * C[i];
+      if (e0 + (i & ~1) < p.rotated) f[i] = fmaf(own[i ^ 1], S[i], f[i]);
     }
+  } else {
+    float partner[kVec];
+    unpack(other, partner);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) f[i] = fmaf(partner[i], S[i], own[i] * C[i]);
   }
 }
 
@@ -277,7 +299,7 @@ __device__ __forceinline__ Where where(const RotaryParams& p) {
 template <typename T, int PAIR, bool VEC, bool NORM, int PER>
 __global__ void __launch_bounds__(32 * kWarps, PER == 4 && VEC && sizeof(T) == 2 ? 8 : 4)
 rotary_kernel(const __grid_constant__ RotaryParams p) {
-  __shared__ T strips[PAIR == kHalfShared ? kWarps * 32 * kVec : 1];
+  __shared__ __align__(16) T strips[PAIR == kHalfShared ? kWarps * 32 * kVec : 1];
   // Only the short form lets its successor in early: waiting CTAs would take the slots of this
   // kernel's later ones (measured on the long form: 1150 us against 845 us, run by itself).
   if constexpr (PER == 1) pdl_launch_dependents();
@@ -331,17 +353,19 @@ rotary_kernel(const __grid_constant__ RotaryParams p) {
   for (int round = 0;;) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
+      float own[kVec];
+      unpack(raw[j], own);
       float rstd = 1.f;
       if constexpr (NORM) {
         float sq = 0.f;
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) sq = fmaf(to_f32(raw[j].v[i]), to_f32(raw[j].v[i]), sq);
+        for (int i = 0; i < kVec; ++i) sq = fmaf(own[i], own[i], sq);
         rstd = rsqrtf(fmaf(group_sum(sq, p.group), p.inv_dim, p.eps));
       }
       Raw<T> other;
       partners<T, PAIR>(p, raw[j], other, w.e0, w.lane, strip);
       float f[kVec];
-      combine<T, PAIR>(p, raw[j], other, C, S, w.e0, f);
+      combine<T, PAIR>(p, own, other, C, S, w.e0, f);
       if constexpr (NORM) {
 #pragma unroll
         for (int i = 0; i < kVec; ++i) f[i] *= rstd;
@@ -366,7 +390,7 @@ constexpr int kBwdBlocksPerSm = 5;
 template <typename T, int PAIR, bool VEC, int PER>
 __global__ void __launch_bounds__(32 * kWarps, VEC && sizeof(T) == 2 ? kBwdBlocksPerSm : 4)
 rotary_bwd_kernel(const __grid_constant__ RotaryParams p) {
-  __shared__ T strips[PAIR == kHalfShared ? kWarps * 32 * kVec : 1];
+  __shared__ __align__(16) T strips[PAIR == kHalfShared ? kWarps * 32 * kVec : 1];
   __shared__ float fold[kWarps][kMaxDim];
   __shared__ __align__(16) float weights[kMaxDim];  // eight registers per lane fewer than held there
   pdl_wait();
@@ -412,16 +436,17 @@ rotary_bwd_kernel(const __grid_constant__ RotaryParams p) {
       for (int j = 0; j < PER; ++j) {
         Raw<T> other;
         partners<T, PAIR>(p, rg[j], other, w.e0, w.lane, strip);
-        float v[kVec];
-        combine<T, PAIR>(p, rg[j], other, C, S, w.e0, v);
+        float v[kVec], u[kVec];
+        unpack(rg[j], u);
+        combine<T, PAIR>(p, u, other, C, S, w.e0, v);
+        unpack(rx[j], u);
         const float4 w0 = my_weights[0], w1 = my_weights[1];
         const float weight[kVec] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
         float sq = 0.f, dot = 0.f;
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
-          const float u = to_f32(rx[j].v[i]);
-          sq = fmaf(u, u, sq);
-          dot = fmaf(v[i] * weight[i], u, dot);
+          sq = fmaf(u[i], u[i], sq);
+          dot = fmaf(v[i] * weight[i], u[i], dot);
         }
         sq = group_sum(sq, p.group);
         dot = group_sum(dot, p.group);
@@ -430,9 +455,8 @@ rotary_bwd_kernel(const __grid_constant__ RotaryParams p) {
         if (w.live && h0 + j * heads_per < s.heads) {
 #pragma unroll
           for (int i = 0; i < kVec; ++i) {
-            const float u = to_f32(rx[j].v[i]);
-            acc[i] = fmaf(v[i], u * rstd, acc[i]);
-            v[i] = rstd * fmaf(-u, pull, v[i] * weight[i]);
+            acc[i] = fmaf(v[i], u[i] * rstd, acc[i]);
+            v[i] = rstd * fmaf(-u[i], pull, v[i] * weight[i]);
           }
           store_raw<VEC>(dx + j * heads_per * s.y_h, v, w.e0, p.D);
         }
