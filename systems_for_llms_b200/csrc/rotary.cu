@@ -16,10 +16,14 @@
 // and a warp issues the loads of several head groups of one token before it uses the first.
 // The table row of the token is read once for all of them and multiplied by the weights, so that
 // a head costs two products per element; partners of the half layout travel between lanes as the
-// 16-bit pairs they were loaded as.  (A first form with a product per weight, fp32 exchanges,
-// IEEE division and 64-bit index arithmetic issued 255 instructions per head group and was bound
-// by them: 1.4 ms where this takes a fifth.)  The backward pass recomputes the statistics from x,
-// which it has to read anyway, instead of storing them.
+// 16-bit pairs they were loaded as, and arithmetic is done on two fp32 numbers per instruction.
+// (A first form with a product per weight, fp32 exchanges, IEEE division and 64-bit index
+// arithmetic issued 255 instructions per head group and was bound by them.)  The backward pass
+// recomputes the statistics from x, which it has to read anyway, instead of storing them.
+//
+// Measured at 2 x 32768 tokens of 32 + 8 heads of 128, bf16: forward 247 us for 1.34 GB (5.4 TB/s),
+// backward 475 us for 2.0 GB (4.2 TB/s; 40 registers of operands in flight per lane leave it five
+// blocks per SM, and a ring of asynchronous copies through shared memory took 598 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -81,6 +85,39 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) {
 }
 template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
 
+// Two fp32 numbers in one register pair, and the instructions that work on both: these kernels
+// are bound by instruction issue as much as by memory.
+struct Two { unsigned long long v; };
+__device__ __forceinline__ Two two(float lo, float hi) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void split(Two a, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v));
+}
+__device__ __forceinline__ Two mul(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float sum(Two a) {
+  float lo, hi;
+  split(a, lo, hi);
+  return lo + hi;
+}
+__device__ __forceinline__ Two swapped(Two a) {
+  float lo, hi;
+  split(a, lo, hi);
+  return two(hi, lo);
+}
+constexpr int kTwos = kVec / 2;
+
 // Two values in one conversion instruction.
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
@@ -97,18 +134,16 @@ template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi
 template <typename T> struct Raw { uint32_t w[kVec * sizeof(T) / 4]; };
 
 template <typename T>
-__device__ __forceinline__ void unpack(const Raw<T>& r, float (&f)[kVec]) {
+__device__ __forceinline__ void unpack(const Raw<T>& r, Two (&f)[kTwos]) {
 #pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(r.w) / 4); ++i) {
+  for (int i = 0; i < kTwos; ++i) {
     if constexpr (sizeof(T) == 4) {
-      f[i] = __uint_as_float(r.w[i]);
+      f[i] = two(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
     } else if constexpr (std::is_same<T, __half>::value) {
       const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&r.w[i]));
-      f[2 * i] = v.x;
-      f[2 * i + 1] = v.y;
+      f[i] = two(v.x, v.y);
     } else {
-      f[2 * i] = __uint_as_float(r.w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(r.w[i] & 0xffff0000u);
+      f[i] = two(__uint_as_float(r.w[i] << 16), __uint_as_float(r.w[i] & 0xffff0000u));
     }
   }
 }
@@ -133,7 +168,10 @@ __device__ __forceinline__ void load_raw(Raw<T>& r, const T* row, int e0, int D,
 }
 
 template <bool VEC, typename T>
-__device__ __forceinline__ void store_raw(T* row, const float (&f)[kVec], int e0, int D) {
+__device__ __forceinline__ void store_raw(T* row, const Two (&g)[kTwos], int e0, int D) {
+  float f[kVec];
+#pragma unroll
+  for (int i = 0; i < kTwos; ++i) split(g[i], f[2 * i], f[2 * i + 1]);
   if constexpr (VEC && sizeof(T) == 4) {
     float4* dst = reinterpret_cast<float4*>(row + e0);
     dst[0] = make_float4(f[0], f[1], f[2], f[3]);
@@ -231,22 +269,27 @@ __device__ __forceinline__ void partners(const RotaryParams& p, const Raw<T>& mi
   }
 }
 
+__device__ __forceinline__ void pair_up(const float (&f)[kVec], Two (&g)[kTwos]) {
+#pragma unroll
+  for (int i = 0; i < kTwos; ++i) g[i] = two(f[2 * i], f[2 * i + 1]);
+}
+
 // f_e = own_e C_e + partner_e S_e
 template <typename T, int PAIR>
-__device__ __forceinline__ void combine(const RotaryParams& p, const float (&own)[kVec],
-                                        const Raw<T>& other, const float (&C)[kVec],
-                                        const float (&S)[kVec], int e0, float (&f)[kVec]) {
+__device__ __forceinline__ void combine(const RotaryParams& p, const Two (&own)[kTwos],
+                                        const Raw<T>& other, const Two (&C)[kTwos],
+                                        const Two (&S)[kTwos], int e0, Two (&f)[kTwos]) {
   if constexpr (PAIR == kInterleaved) {
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      f[i] = own[i] * C[i];
-      if (e0 + (i & ~1) < p.rotated) f[i] = fmaf(own[i ^ 1], S[i], f[i]);
+    for (int i = 0; i < kTwos; ++i) {
+      f[i] = mul(own[i], C[i]);
+      if (e0 + 2 * i < p.rotated) f[i] = fma(swapped(own[i]), S[i], f[i]);
     }
   } else {
-    float partner[kVec];
+    Two partner[kTwos];
     unpack(other, partner);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) f[i] = fmaf(partner[i], S[i], own[i] * C[i]);
+    for (int i = 0; i < kTwos; ++i) f[i] = fma(partner[i], S[i], mul(own[i], C[i]));
   }
 }
 
@@ -295,7 +338,8 @@ __device__ __forceinline__ Where where(const RotaryParams& p) {
 
 // One warp takes PER head groups of one token.  PER = 4 keeps 2 KB of loads in flight per warp;
 // PER = 1 is for calls with few tokens, which are over sooner when every head group has a warp
-// of its own (16 tokens x 40 heads x 128: 3.0 us against 3.9 us).
+// of its own.  Kernel time at 40 heads of 128, PER 1 against 4: one token 2.1 and 2.7 us, 16
+// tokens 2.2 and 2.8; at 512 tokens of 32 heads of 64, 256 blocks of PER 4, 3.3 and 3.0.
 template <typename T, int PAIR, bool VEC, bool NORM, int PER>
 __global__ void __launch_bounds__(32 * kWarps, PER == 4 && VEC && sizeof(T) == 2 ? 8 : 4)
 rotary_kernel(const __grid_constant__ RotaryParams p) {
@@ -350,25 +394,28 @@ rotary_kernel(const __grid_constant__ RotaryParams p) {
         S[i] *= w.e0 + i < p.D ? s.weight[partner_of(p, w.e0 + i)] : 0.f;
     }
   }
+  Two C2[kTwos], S2[kTwos];
+  pair_up(C, C2);
+  pair_up(S, S2);
   for (int round = 0;;) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-      float own[kVec];
+      Two own[kTwos], f[kTwos];
       unpack(raw[j], own);
-      float rstd = 1.f;
+      Two scale;
       if constexpr (NORM) {
-        float sq = 0.f;
+        Two sq = mul(own[0], own[0]);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) sq = fmaf(own[i], own[i], sq);
-        rstd = rsqrtf(fmaf(group_sum(sq, p.group), p.inv_dim, p.eps));
+        for (int i = 1; i < kTwos; ++i) sq = fma(own[i], own[i], sq);
+        const float rstd = rsqrtf(fmaf(group_sum(sum(sq), p.group), p.inv_dim, p.eps));
+        scale = two(rstd, rstd);
       }
       Raw<T> other;
       partners<T, PAIR>(p, raw[j], other, w.e0, w.lane, strip);
-      float f[kVec];
-      combine<T, PAIR>(p, own, other, C, S, w.e0, f);
+      combine<T, PAIR>(p, own, other, C2, S2, w.e0, f);
       if constexpr (NORM) {
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) f[i] *= rstd;
+        for (int i = 0; i < kTwos; ++i) f[i] = mul(f[i], scale);
       }
       if (w.live && h0 + j * heads_per < s.heads)
         store_raw<VEC>(y + j * y_step, f, w.e0, p.D);
@@ -384,7 +431,9 @@ rotary_kernel(const __grid_constant__ RotaryParams p) {
 
 // Backward with the norm.  A persistent grid: every warp keeps the weight gradient of its
 // eight elements in registers over all its tokens; the block folds its warps in a fixed order
-// and leaves one row of partial sums (deterministic, no atomics).
+// and leaves one row of partial sums (deterministic, no atomics).  Two head groups per round and
+// five blocks per SM: 2 x 32768 tokens of 40 heads take 475 us, 16 x 512 tokens of 32 heads of 64
+// 16.6; six blocks 463 and 17.8, seven 541 and 17.6, one group and eight blocks 581 and 24.9.
 constexpr int kBwdBlocksPerSm = 5;
 
 template <typename T, int PAIR, bool VEC, int PER>
@@ -409,9 +458,9 @@ rotary_bwd_kernel(const __grid_constant__ RotaryParams p) {
   for (int e = threadIdx.x; e < kMaxDim; e += blockDim.x) weights[e] = e < p.D ? s.weight[e] : 0.f;
   __syncthreads();
   const float4* my_weights = reinterpret_cast<const float4*>(weights + w.e0);
-  float acc[kVec];
+  Two acc[kTwos];
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) acc[i] = 0.f;
+  for (int i = 0; i < kTwos; ++i) acc[i] = two(0.f, 0.f);
   for (unsigned item = block * kWarps + warp; item < items; item += blocks * kWarps) {
     const unsigned token = item / chunks;
     int h0 = static_cast<int>(item - token * chunks) * rounds * heads_per * PER + w.sub;
@@ -429,34 +478,41 @@ rotary_bwd_kernel(const __grid_constant__ RotaryParams p) {
       }
     };
     load();
-    float C[kVec], S[kVec];
-    load_angles<PAIR>(p, b, t, w.e0, C, S);
+    Two C2[kTwos], S2[kTwos];
+    {
+      float C[kVec], S[kVec];
+      load_angles<PAIR>(p, b, t, w.e0, C, S);
+      pair_up(C, C2);
+      pair_up(S, S2);
+    }
     for (int round = 0;;) {
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
         Raw<T> other;
         partners<T, PAIR>(p, rg[j], other, w.e0, w.lane, strip);
-        float v[kVec], u[kVec];
+        Two v[kTwos], u[kTwos];
         unpack(rg[j], u);
-        combine<T, PAIR>(p, u, other, C, S, w.e0, v);
+        combine<T, PAIR>(p, u, other, C2, S2, w.e0, v);
         unpack(rx[j], u);
         const float4 w0 = my_weights[0], w1 = my_weights[1];
-        const float weight[kVec] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-        float sq = 0.f, dot = 0.f;
+        const Two weight[kTwos] = {two(w0.x, w0.y), two(w0.z, w0.w), two(w1.x, w1.y), two(w1.z, w1.w)};
+        Two sq2 = mul(u[0], u[0]), dot2 = mul(mul(v[0], weight[0]), u[0]);
 #pragma unroll
-        for (int i = 0; i < kVec; ++i) {
-          sq = fmaf(u[i], u[i], sq);
-          dot = fmaf(v[i] * weight[i], u[i], dot);
+        for (int i = 1; i < kTwos; ++i) {
+          sq2 = fma(u[i], u[i], sq2);
+          dot2 = fma(mul(v[i], weight[i]), u[i], dot2);
         }
-        sq = group_sum(sq, p.group);
-        dot = group_sum(dot, p.group);
+        const float sq = group_sum(sum(sq2), p.group);
+        const float dot = group_sum(sum(dot2), p.group);
         const float rstd = rsqrtf(fmaf(sq, p.inv_dim, p.eps));
-        const float pull = dot * p.inv_dim * rstd * rstd;  // mean(v w xhat) / rms
+        const float pull = -dot * p.inv_dim * rstd * rstd * rstd;  // -mean(v w xhat) / mean square
         if (w.live && h0 + j * heads_per < s.heads) {
+          const Two scale = two(rstd, rstd), back = two(pull, pull);
 #pragma unroll
-          for (int i = 0; i < kVec; ++i) {
-            acc[i] = fmaf(v[i], u[i] * rstd, acc[i]);
-            v[i] = rstd * fmaf(-u[i], pull, v[i] * weight[i]);
+          for (int i = 0; i < kTwos; ++i) {
+            const Two vs = mul(v[i], scale);
+            acc[i] = fma(vs, u[i], acc[i]);
+            v[i] = fma(u[i], back, mul(vs, weight[i]));
           }
           store_raw<VEC>(dx + j * heads_per * s.y_h, v, w.e0, p.D);
         }
@@ -472,11 +528,14 @@ rotary_bwd_kernel(const __grid_constant__ RotaryParams p) {
   }
   // heads of the warp, then warps of the block
 #pragma unroll
-  for (int i = 0; i < kVec; ++i)
-    for (int o = p.group; o < 32; o <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-  if (w.sub == 0 && w.live) {
+  for (int i = 0; i < kTwos; ++i) {
+    float each[2];
+    split(acc[i], each[0], each[1]);
 #pragma unroll
-    for (int i = 0; i < kVec; ++i) fold[warp][w.e0 + i] = acc[i];
+    for (int k = 0; k < 2; ++k) {
+      for (int o = p.group; o < 32; o <<= 1) each[k] += __shfl_xor_sync(0xffffffffu, each[k], o);
+      if (w.sub == 0 && w.live) fold[warp][w.e0 + 2 * i + k] = each[k];
+    }
   }
   __syncthreads();
   for (int e = threadIdx.x; e < p.D; e += blockDim.x) {
@@ -576,8 +635,8 @@ int fill(RotaryParams& p, const SflRotaryTensor* tensors, int count, const SflRo
 }
 
 // Warp items per token.  A warp that walks all heads of its token reads the angles and weights
-// once for them (a third of the instructions of a one-round item at 8 heads of 128); with fewer
-// tokens than keep the SMs busy that way, the heads are spread over more warps.
+// once for them (237 -> 172 instructions per head group at 16 heads of 64); with fewer tokens
+// than keep the SMs busy that way, the heads are spread over more warps.
 void set_chunks(RotaryParams& p, int count, int per, long warps_wanted) {
   const int each = 32 / p.group * per;
   const int all0 = (p.side[0].heads + each - 1) / each;
@@ -606,7 +665,7 @@ int launch_forward(RotaryParams p, int count, int sms, cudaStream_t stream) {
     return launch_pdl(kernel, dim3(static_cast<unsigned>(blocks)), dim3(32 * kWarps), 0, stream, p);
   };
   set_chunks(p, count, 4, 64L * sms);  // two rounds of 32 resident warps per SM
-  if (token_blocks * (p.chunks0 + p.chunks1) >= 2L * sms)
+  if (token_blocks * (p.chunks0 + p.chunks1) >= sms)
     return go(rotary_kernel<T, PAIR, VEC, NORM, 4>);
   set_chunks(p, count, 1, 64L * sms);
   return go(rotary_kernel<T, PAIR, VEC, NORM, 1>);
