@@ -23,7 +23,7 @@
 // and P X nearly cancel; there lo is dropped and X <- (P + a I) hi, one product whose factors are
 // smaller than the terms they replace.  Sums are fp32, the norm is accumulated in 64 bits.
 // Measured against 64 bits: 1.8e-3 to 2.3e-3 of the result's norm, of which its rounding to bf16 is
-// 1.7e-3 (hi alone throughout: up to 1e-2; a X apart in every step: up to 2.7e-3).
+// 1.7e-3 (in a simulation, hi alone throughout: up to 2e-2; a X apart in every step: up to 2.7e-3).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -792,7 +792,8 @@ ns_poly_kernel(const __grid_constant__ PolyParams p) {
 // where singular values are 1.
 //
 // One launch instead of seventeen; its time is the latency of three products and three passes
-// through registers per step (128 x 384, five steps: see the table at the entry point).
+// through registers per step (128 x 384, five steps: 38 us a call, where
+// the launch per product took 114).
 constexpr int kBlockRows = 128;
 constexpr int kBlockCols = 384;          // 512 columns of tensor memory less 128 of G
 constexpr int kBlockEpiWarps = 8;
@@ -1178,6 +1179,12 @@ extern "C" long sfl_newton_schulz_bytes(int batch, int m, int n) {
   using namespace sfl;
   if (batch < 1 || m < 1 || n < 1 || batch > 65535) return -1;
   return sizes_of(batch, m, n).total;
+}
+
+extern "C" int sfl_newton_schulz_kernels(int m, int n, int steps) {
+  using namespace sfl;
+  if (fits_block(m, n)) return 1;
+  return 2 + steps * ((m < n ? m : n) <= pair::kTileN ? 2 : 3);
 }
 
 extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {

@@ -157,6 +157,8 @@ typedef struct SflNewtonSchulz {
   int* status;
 } SflNewtonSchulz;
 long sfl_newton_schulz_bytes(int batch, int m, int n);
+/* Kernels that one call launches. */
+int sfl_newton_schulz_kernels(int m, int n, int steps);
 int sfl_newton_schulz(const SflNewtonSchulz* args, void* stream);
 
 /* Muon around it.  The same parameter of `rows` layers: `len` consecutive fp32 elements (a multiple

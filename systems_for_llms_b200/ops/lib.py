@@ -105,8 +105,9 @@ def register_signature(name: str, argtypes: list) -> None:
 # Kernels launched per call of each entry point (default 1, 0 for host-only calls).
 _KERNELS_PER_CALL = {"sfl_attn_bwd": 2, "sfl_rotary_bwd": 2, "sfl_rotary_bwd_partial_bytes": 0,
                      "sfl_linear_ce_part_bytes": 0, "sfl_linear_ce_dh_sum_bytes": 0,
-                     "sfl_linear_ce_fwd": 3, "sfl_linear_ce_bwd": 2,
-                     "sfl_newton_schulz_bytes": 0, "sfl_newton_schulz": 17,
+                     "sfl_linear_ce_fwd": 0, "sfl_linear_ce_bwd": 0,   # their callers count
+                     "sfl_newton_schulz_bytes": 0, "sfl_newton_schulz_kernels": 0,
+                     "sfl_newton_schulz": 0,
                      "sfl_embedding_bwd": 2, "sfl_block_forward": 7, "sfl_block_backward": 11,
                      "sfl_block_saved_bytes": 0, "sfl_block_scratch_bytes": 0, "sfl_rmsnorm_bwd_blocks": 0, "sfl_sqnorm_blocks": 0,
                      "sfl_ipc_alloc": 0, "sfl_ipc_free": 0, "sfl_ipc_get_handle": 0,
@@ -120,6 +121,11 @@ _launches = [0]
 def launch_count() -> int:
     """Number of this library's kernels launched by the current process so far."""
     return _launches[0]
+
+
+def count_kernels(launched: int) -> None:
+    """Adds the kernels of a call whose number depends on its sizes."""
+    _launches[0] += launched
 
 
 class _Library:

@@ -57,7 +57,11 @@ _lib.register_signature("sfl_linear_ce_bwd", [POINTER(LinearCe), POINTER(LinearC
 
 def piece_size(rows: int, vocab: int) -> int:
     """Entries of the vocabulary per piece: as many as keep dl at ``PIECE_BYTES``, at least
-    ``MIN_PIECE`` (smaller pieces leave the products too few tiles for the SMs), at most all."""
+    ``MIN_PIECE`` (smaller pieces leave the products too few tiles for the SMs), at most all.
+
+    Forward and backward of 4096 x 1024 x 32768 take 0.25 ms in one piece, 0.35 ms in pieces of
+    9472 and 0.36 ms in pieces of 4096; 8192 x 2048 x 131072 takes 13.7 to 13.9 ms in pieces of
+    12288, 14.3 to 14.5 of 2048, 14.2 to 14.6 in one (2.1 GB of dl)."""
     fit = PIECE_BYTES // (2 * rows) // PIECE_STEP * PIECE_STEP
     return min(max(fit, MIN_PIECE), -(-vocab // PIECE_STEP) * PIECE_STEP)
 
@@ -119,6 +123,7 @@ def linear_ce_forward(hidden, weight, targets, ignore_index: int, mean: bool | N
                                         int(bool(mean)), _lib.ptr(totals), _lib.ptr(loss),
                                         _lib.stream_ptr())
     _lib.check(code, "sfl_linear_ce_fwd")
+    _lib.count_kernels(3 if reduce else 2)
     return row_loss, lse2, totals, loss
 
 
@@ -150,6 +155,7 @@ def linear_ce_backward(hidden, weight, targets, ignore_index: int, lse2, grad, t
                              dw_kind=kind, piece=piece)
         code = handle.sfl_linear_ce_bwd(byref(args), byref(grads), _lib.stream_ptr())
     _lib.check(code, "sfl_linear_ce_bwd")
+    _lib.count_kernels(2 * -(-vocab // piece) + (dh_sum is not None))
     return dh
 
 

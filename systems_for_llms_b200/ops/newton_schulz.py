@@ -35,8 +35,8 @@ class NewtonSchulz(Structure):
 
 _P = c_void_p
 _lib.register_signature("sfl_newton_schulz_bytes", [c_int, c_int, c_int])
+_lib.register_signature("sfl_newton_schulz_kernels", [c_int, c_int, c_int])
 _lib.register_signature("sfl_newton_schulz", [POINTER(NewtonSchulz), _P])
-
 
 _lib.register_signature("sfl_muon_momentum", [_P, _P, _P, c_int, c_long, c_long, c_float, c_int, _P,
                                               _P, _P])
@@ -113,6 +113,16 @@ def _strided(update: torch.Tensor) -> torch.Tensor:
     return update
 
 
+def _overlap(out: torch.Tensor, update: torch.Tensor) -> bool:
+    """Whether contiguous ``out`` lies within the bytes that ``update`` spans without being it."""
+    begin, size = update.data_ptr(), update.element_size()
+    end = begin + size * (1 + sum((n - 1) * s for n, s in zip(update.shape, update.stride())))
+    at = out.data_ptr()
+    if at >= end or at + 2 * out.numel() <= begin:
+        return False
+    return not (at == begin and update.dtype == out.dtype and update.is_contiguous())
+
+
 def newton_schulz(update: torch.Tensor, *, steps: int = 5, coefficients=QUINTIC,
                   eps: float = 1e-7, out: torch.Tensor | None = None) -> torch.Tensor:
     """Orthogonalises every matrix of ``update [..., m, n]`` (bf16, fp16 or fp32).
@@ -124,7 +134,8 @@ def newton_schulz(update: torch.Tensor, *, steps: int = 5, coefficients=QUINTIC,
     computed with fp16 operands whose rounding does not compound (off by about 0.002 of its norm,
     rounding to bf16 included; the normalised matrix is held to 2^-37 absolutely, which only shows
     where ``eps`` dwarfs the norm and the result is far below 1).  A matrix of zeros gives zeros; one that holds an infinity or NaN
-    gives NaN without touching its neighbours.  ``out`` receives the result.  Coefficients under
+    gives NaN without touching its neighbours.  ``out`` receives the result; it may be a contiguous
+    bf16 ``update`` itself and is otherwise refused when it lies within the bytes the update spans.  Coefficients under
     which singular values starting below 1 exceed 2 are refused: the operands are scaled for
     bounded ones.  The operator is not differentiable.
     """
@@ -154,6 +165,8 @@ def newton_schulz(update: torch.Tensor, *, steps: int = 5, coefficients=QUINTIC,
     elif (out.shape != update.shape or out.dtype != torch.bfloat16 or not out.is_contiguous()
           or out.device != update.device):
         raise ValueError("out must be a contiguous bf16 tensor of the update's shape on its device")
+    elif out.numel() and _overlap(out, update):
+        raise ValueError("out must be update itself (contiguous bf16) or lie apart from it")
     if update.numel() == 0:
         return out
     x = _strided(update)
@@ -177,6 +190,7 @@ def newton_schulz(update: torch.Tensor, *, steps: int = 5, coefficients=QUINTIC,
     with _lib.on_device(x.device):
         code = handle.sfl_newton_schulz(byref(args), _lib.stream_ptr())
     _lib.check(code, "sfl_newton_schulz")
+    _lib.count_kernels(handle.sfl_newton_schulz_kernels(m, n, steps))
     return out
 
 

@@ -314,7 +314,7 @@ def rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
     ``positions`` (int64 ``[T]`` or ``[B, T]``) are rows of the tables; without them token ``t``
     is at position ``t``.  A position outside the tables makes the rotated lanes of its token
     NaN.  ``layout`` pairs lanes (2i, 2i+1) or (i, i + R/2).  The result is rounded once from
-    fp32 to the type of ``x``; ``out`` (inference only) receives it and may be ``x``.
+    fp32 to the type of ``x``; ``out`` (inference only) receives it; it may be ``x`` and must not overlap it in any other way.
     """
     if layout not in LAYOUTS:
         raise ValueError("layout must be one of " + ", ".join(LAYOUTS))
@@ -340,7 +340,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor,
     of its mean square plus ``eps``, multiplied by its fp32 weight ``[D]`` and turned as by
     ``rotary``.  Statistics and rotation are fp32; each result is rounded once.  ``out``
     (inference only) is a pair of tensors that receive the results, for example the rows of a
-    KV cache that the new keys belong to; they may be ``q`` and ``k`` themselves.
+    KV cache that the new keys belong to; they may be ``q`` and ``k`` themselves
+    and must not overlap either in any other way.
     """
     if layout not in LAYOUTS:
         raise ValueError("layout must be one of " + ", ".join(LAYOUTS))

@@ -333,3 +333,29 @@ def test_streams_and_graphs(dev):
     check(dev)
     for got, expected in zip(results, want):
         assert all(torch.equal(a, b) for a, b in zip(got, expected))
+
+
+@pytest.mark.parametrize("rows, dim, vocab, piece", [(300, 64, 700, 256), (300, 64, 700, 768),
+                                                     (1024, 512, 10000, 10240)])
+def test_kernels_are_counted(dev, rows, dim, vocab, piece):
+    from systems_for_llms_b200.ops import lib
+    from systems_for_llms_b200.ops.linear_loss import linear_ce_backward, linear_ce_forward
+    from torch.profiler import ProfilerActivity, profile
+    h = torch.randn(rows, dim, device=dev).bfloat16()
+    w = torch.randn(vocab, dim, device=dev).bfloat16()
+    t = torch.randint(vocab, (rows,), device=dev)
+    dw = torch.empty_like(w)
+
+    def both():
+        _, lse2, totals, _ = linear_ce_forward(h, w, t, -100, True)
+        linear_ce_forward(h, w, t, -100, None)
+        linear_ce_backward(h, w, t, -100, lse2, None, totals, dw, piece=piece)
+    both()
+    torch.cuda.synchronize()
+    before = lib.launch_count()
+    with profile(activities=[ProfilerActivity.CUDA]) as p:
+        both()
+        torch.cuda.synchronize()
+    seen = sum(e.device_type == torch.autograd.DeviceType.CUDA and "sfl::" in e.name
+               for e in p.events())
+    assert lib.launch_count() - before == seen > 0

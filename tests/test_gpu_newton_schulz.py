@@ -288,3 +288,41 @@ def test_streams_and_graphs(dev):
         side.wait_stream(other)
     check(dev)
     assert all(torch.equal(a, b) for a, b in zip(results, want))
+
+
+def test_out_in_place_or_apart(dev):
+    from systems_for_llms_b200.ops.newton_schulz import newton_schulz
+    torch.manual_seed(40)
+    for m, n in [(96, 200), (200, 300), (300, 400)]:     # the three forms
+        u = torch.randn(2, m, n, device=dev).bfloat16()
+        want = newton_schulz(u)
+        same = u.clone()
+        assert newton_schulz(same, out=same) is same
+        assert torch.equal(same, want)
+        store = torch.empty(3, m, n, device=dev, dtype=torch.bfloat16)
+        store[:2] = u
+        with pytest.raises(ValueError):
+            newton_schulz(store[:2], out=store[1:])      # a block would overwrite the next input
+        store = torch.randn(2, m, n, device=dev)
+        with pytest.raises(ValueError):
+            newton_schulz(store, out=store.view(torch.bfloat16).view(-1)[:2 * m * n].view(2, m, n))
+        assert torch.equal(newton_schulz(u, out=store.view(torch.bfloat16).view(-1)[:2 * m * n]
+                                         .view(2, m, n)), want)
+    check(dev)
+
+
+@pytest.mark.parametrize("shape, steps", [((2, 96, 200), 5), ((200, 300), 3), ((300, 280), 2)])
+def test_kernels_are_counted(dev, shape, steps):
+    from systems_for_llms_b200.ops import lib
+    from systems_for_llms_b200.ops.newton_schulz import newton_schulz
+    from torch.profiler import ProfilerActivity, profile
+    u = torch.randn(shape, device=dev)
+    newton_schulz(u, steps=steps)
+    torch.cuda.synchronize()
+    before = lib.launch_count()
+    with profile(activities=[ProfilerActivity.CUDA]) as p:
+        newton_schulz(u, steps=steps)
+        torch.cuda.synchronize()
+    seen = sum(e.device_type == torch.autograd.DeviceType.CUDA and "sfl::" in e.name
+               for e in p.events())
+    assert lib.launch_count() - before == seen > 0
