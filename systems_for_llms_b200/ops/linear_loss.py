@@ -59,8 +59,8 @@ def piece_size(rows: int, vocab: int) -> int:
     """Entries of the vocabulary per piece: as many as keep dl at ``PIECE_BYTES``, at least
     ``MIN_PIECE`` (smaller pieces leave the products too few tiles for the SMs), at most all.
 
-    Forward and backward of 4096 x 1024 x 32768 take 0.25 ms in one piece, 0.35 ms in pieces of
-    9472 and 0.36 ms in pieces of 4096; 8192 x 2048 x 131072 takes 13.7 to 13.9 ms in pieces of
+    Forward and backward of 4096 x 1024 x 10000 take 0.25 ms in one piece, 0.35 ms with 9472
+    entries in the first and 0.36 ms in pieces of 4096; 8192 x 2048 x 131072 takes 13.7 to 13.9 ms in pieces of
     12288, 14.3 to 14.5 of 2048, 14.2 to 14.6 in one (2.1 GB of dl)."""
     fit = PIECE_BYTES // (2 * rows) // PIECE_STEP * PIECE_STEP
     return min(max(fit, MIN_PIECE), -(-vocab // PIECE_STEP) * PIECE_STEP)
