@@ -38,6 +38,9 @@ from . import comm as pm
 
 class FusedShardedTransformer(nn.Module):
     def __init__(self, model, engine, group=None, comm_ctas: int = 48):
+        if model.qk_norm or model.head_loss != "logits":
+            raise ValueError("per-head query/key norms and the head loss by pieces are not "
+                             "supported by the fused sharded model")
         super().__init__()
         self.model = model
         self.engine = engine

@@ -76,6 +76,13 @@ def test_tensor_parallel_surgery_refuses_per_head_norms():
         parallelize_model(TransformerLM(**TINY, qk_norm=True))
 
 
+@pytest.mark.parametrize("option", [dict(qk_norm=True), dict(head_loss="pieces")])
+def test_fused_sharded_model_refuses_what_it_does_not_cover(option):
+    from systems_for_llms_b200.parallel.fsdp_fused import FusedShardedTransformer
+    with pytest.raises(ValueError, match="not supported"):
+        FusedShardedTransformer(TransformerLM(**TINY, **option), None)
+
+
 def test_qk_norm_leaves_the_random_stream_alone_and_adds_two_weights_per_layer():
     torch.manual_seed(3)
     plain = TransformerLM(**TINY)
