@@ -120,10 +120,11 @@ long sfl_linear_ce_part_bytes(int rows, int vocab);
 int sfl_linear_ce_fwd(const SflLinearCe* a, void* part, long part_bytes, float* row_loss, int mean,
                       float* totals, float* loss, void* stream);
 
-/* dh 16-bit [rows, dim] and dw [vocab, dim] (dw_kind 0: 16-bit, 1: fp32, 2: added to fp32), both
- * times the device scalar grad (NULL: 1) and over totals[1] (NULL: not).  The vocabulary is walked
- * in pieces of `piece` entries (a multiple of 256): dlogits is 16-bit [rows, piece] scratch, dh_sum
- * scratch of sfl_linear_ce_dh_sum_bytes (which may be none; asks for the current device). */
+/* dh 16-bit [rows, dim] and dw [vocab, dim] (dw_kind 0: 16-bit, 1: fp32, 2: added to fp32, 3: dw is
+ * NULL and not computed), both times the device scalar grad (NULL: 1) and over totals[1] (NULL:
+ * not).  dh may be NULL as well when dw is not.  The vocabulary is walked in pieces of `piece`
+ * entries (a multiple of 256): dlogits is 16-bit [rows, piece] scratch, dh_sum scratch of
+ * sfl_linear_ce_dh_sum_bytes (which may be none; asks for the current device). */
 typedef struct SflLinearCeGrad {
   const float* grad;
   const float* totals;
@@ -136,7 +137,7 @@ typedef struct SflLinearCeGrad {
   long ld_dw;
   int dw_kind, piece;
 } SflLinearCeGrad;
-long sfl_linear_ce_dh_sum_bytes(int rows, int dim, int vocab, int piece);
+long sfl_linear_ce_dh_sum_bytes(int rows, int dim, int vocab, int piece, int with_dw);
 int sfl_linear_ce_bwd(const SflLinearCe* a, const SflLinearCeGrad* g, void* stream);
 
 /* ------------------------------------------------- orthogonalised updates -- */

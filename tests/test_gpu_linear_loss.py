@@ -120,6 +120,34 @@ def test_loss_and_gradients(dev, shape, dtype):
         assert (dh[~e.valid] == 0).all()
 
 
+@pytest.mark.parametrize("shape, piece", [((129, 136, 257), None), ((300, 200, 1000), 512),
+                                          ((64, 128, 6000), None)])   # the last splits dh's sum
+def test_one_gradient_alone(dev, shape, piece):
+    """What is not asked for is not computed; the sum of dh may be split differently, so each is
+    held to the formula and not to the other."""
+    from systems_for_llms_b200.ops import linear_loss as L
+    h, w, t = make(dev, *shape, torch.bfloat16)
+    e = Exact(h, w, t)
+    scale = 1.0 / e.valid.sum().item()
+    want_h, want_w, bh, bw = e.grads(scale, pieces=16)
+    hidden, weight = h.detach().requires_grad_(), w.detach().requires_grad_()
+    dh, = torch.autograd.grad(L.linear_cross_entropy(hidden, w, t), hidden)
+    dw, = torch.autograd.grad(L.linear_cross_entropy(h, weight, t), weight)
+    within(dh, want_h, bh + 4 * U * want_h.abs())
+    within(dw, want_w, bw + 4 * U * want_w.abs())
+    _, lse2, totals, _ = L.linear_ce_forward(h, w, t, -100, True)
+    one = torch.ones((), device=dev)
+    dh = L.linear_ce_backward(h, w, t, -100, lse2, one, totals, None, piece=piece)
+    out = torch.full_like(w, float("nan"))
+    assert L.linear_ce_backward(h, w, t, -100, lse2, one, totals, out, piece=piece,
+                                need_dh=False) is None
+    check(dev)
+    within(dh, want_h, bh + 4 * U * want_h.abs())
+    within(out, want_w, bw + 4 * U * want_w.abs())
+    with pytest.raises(ValueError):
+        L.linear_ce_backward(h, w, t, -100, lse2, one, totals, None, need_dh=False)
+
+
 @pytest.mark.parametrize("piece", [256, 512, 1024])
 def test_pieces_and_weight_gradient_kinds(dev, piece):
     from systems_for_llms_b200.ops.linear_loss import linear_ce_backward, linear_ce_forward

@@ -73,6 +73,23 @@ def test_entry_points_refuse_before_launching():
                                     ctypes.byref(LinearCeGrad(**spec)), None) == -2
 
 
+def test_a_gradient_left_out_is_said_twice():
+    from systems_for_llms_b200.ops import build as builder
+    from systems_for_llms_b200.ops import lib
+    try:
+        builder.build()
+        handle = lib.lib()
+    except Exception as error:
+        pytest.skip(f"kernel library unavailable: {error}")
+    args = LinearCe(hidden=256, ld_hidden=64, weight=512, ld_weight=64, targets=256, rows=4, dim=64,
+                    vocab=100, lse2=256)
+    spec = dict(dlogits=256, dh=256, ld_dh=64, dw=256, ld_dw=64, dw_kind=0, piece=256)
+    for kw in (dict(dw_kind=3), dict(dw=None, dw_kind=1), dict(dh=None, dw=None, dw_kind=3),
+               dict(dw_kind=4, dw=None)):
+        grads = LinearCeGrad(**{**spec, **kw})
+        assert handle.sfl_linear_ce_bwd(ctypes.byref(args), ctypes.byref(grads), None) == -2, kw
+
+
 def test_records_match_the_compiled_library():
     from systems_for_llms_b200.ops import build as builder
     from systems_for_llms_b200.ops import lib
