@@ -12,6 +12,8 @@ Tolerances, with U = 2^-24 and h, w the operands as given:
   piece), rounded once: (r + K U) (|dl| |.|) + 2 E (p |.|) + r |result|.
 """
 
+import ctypes
+
 import pytest
 import torch
 
@@ -368,7 +370,6 @@ def test_streams_and_graphs(dev):
 def test_kernels_are_counted(dev, rows, dim, vocab, piece):
     from systems_for_llms_b200.ops import lib
     from systems_for_llms_b200.ops.linear_loss import linear_ce_backward, linear_ce_forward
-    from torch.profiler import ProfilerActivity, profile
     h = torch.randn(rows, dim, device=dev).bfloat16()
     w = torch.randn(vocab, dim, device=dev).bfloat16()
     t = torch.randint(vocab, (rows,), device=dev)
@@ -381,9 +382,10 @@ def test_kernels_are_counted(dev, rows, dim, vocab, piece):
     both()
     torch.cuda.synchronize()
     before = lib.launch_count()
-    with profile(activities=[ProfilerActivity.CUDA]) as p:
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
         both()
-        torch.cuda.synchronize()
-    seen = sum(e.device_type == torch.autograd.DeviceType.CUDA and "sfl::" in e.name
-               for e in p.events())
-    assert lib.launch_count() - before == seen > 0
+    nodes = ctypes.c_size_t()          # of the captured graph: kernels alone
+    assert ctypes.CDLL("libcudart.so.12").cudaGraphGetNodes(
+        ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(nodes)) == 0
+    assert lib.launch_count() - before == nodes.value > 0

@@ -15,6 +15,8 @@ since roundings are many and independent.  The result's rounding to bf16 adds 2^
 sqrt(3)) of its norm.
 """
 
+import ctypes
+
 import pytest
 import torch
 
@@ -315,14 +317,14 @@ def test_out_in_place_or_apart(dev):
 def test_kernels_are_counted(dev, shape, steps):
     from systems_for_llms_b200.ops import lib
     from systems_for_llms_b200.ops.newton_schulz import newton_schulz
-    from torch.profiler import ProfilerActivity, profile
     u = torch.randn(shape, device=dev)
     newton_schulz(u, steps=steps)
     torch.cuda.synchronize()
     before = lib.launch_count()
-    with profile(activities=[ProfilerActivity.CUDA]) as p:
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
         newton_schulz(u, steps=steps)
-        torch.cuda.synchronize()
-    seen = sum(e.device_type == torch.autograd.DeviceType.CUDA and "sfl::" in e.name
-               for e in p.events())
-    assert lib.launch_count() - before == seen > 0
+    nodes = ctypes.c_size_t()          # of the captured graph: kernels alone
+    assert ctypes.CDLL("libcudart.so.12").cudaGraphGetNodes(
+        ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(nodes)) == 0
+    assert lib.launch_count() - before == nodes.value > 0
