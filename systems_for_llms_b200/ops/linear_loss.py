@@ -15,7 +15,8 @@ never rounds a logit.  The reference materialises logits and softmax
 
 from __future__ import annotations
 
-from ctypes import POINTER, Structure, byref, c_int, c_int64, c_long, c_void_p
+from ctypes import Structure, c_int, c_int64, c_long, c_void_p
+from struct import Struct
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -48,11 +49,15 @@ class LinearCeGrad(Structure):
                 ("ld_dw", c_long), ("dw_kind", c_int), ("piece", c_int)]
 
 
+# Calls pass the two records as packed bytes (the layouts above), as ops/rotary.py does.
+_CALL = Struct("PlPlPq4i2P")
+_GRAD = Struct("4PlPlPl2i")
+
 _P = c_void_p
 _lib.register_signature("sfl_linear_ce_part_bytes", [c_int, c_int])
-_lib.register_signature("sfl_linear_ce_fwd", [POINTER(LinearCe), _P, c_long, _P, c_int, _P, _P, _P])
+_lib.register_signature("sfl_linear_ce_fwd", [_P, _P, c_long, _P, c_int, _P, _P, _P])
 _lib.register_signature("sfl_linear_ce_dh_sum_bytes", [c_int, c_int, c_int, c_int, c_int])
-_lib.register_signature("sfl_linear_ce_bwd", [POINTER(LinearCe), POINTER(LinearCeGrad), _P])
+_lib.register_signature("sfl_linear_ce_bwd", [_P, _P, _P])
 
 
 def piece_size(rows: int, vocab: int) -> int:
@@ -89,50 +94,47 @@ def _check(hidden, weight, targets) -> None:
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` as a matrix whose rows TMA can address (16-byte aligned, contiguous), copying only
     what does not lie that way already."""
-    t = t.reshape(-1, t.shape[-1])
-    if t.stride(1) != 1 or t.stride(0) % 8 or t.stride(0) < t.shape[1] or t.data_ptr() % 16:
+    if t.ndim != 2:
+        t = t.reshape(-1, t.shape[-1])
+    pitch, step = t.stride()
+    if step != 1 or pitch % 8 or pitch < t.shape[1] or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def _args(hidden, weight, targets, ignore_index, lse2) -> LinearCe:
-    return LinearCe(hidden=hidden.data_ptr(), ld_hidden=hidden.stride(0), weight=weight.data_ptr(),
-                    ld_weight=weight.stride(0), targets=targets.data_ptr(),
-                    ignore_index=ignore_index, rows=hidden.shape[0], dim=hidden.shape[1],
-                    vocab=weight.shape[0], fp16=int(hidden.dtype == torch.float16),
-                    lse2=lse2.data_ptr(), status=captured_status_word(hidden.device).data_ptr())
+def _call(hidden, weight, targets, ignore_index, lse2: int) -> bytes:
+    rows, dim = hidden.shape
+    return _CALL.pack(hidden.data_ptr(), hidden.stride(0), weight.data_ptr(), weight.stride(0),
+                      targets.data_ptr(), ignore_index, rows, dim, weight.shape[0],
+                      hidden.dtype == torch.float16, lse2,
+                      captured_status_word(hidden.device).data_ptr())
 
 
-def linear_ce_forward(hidden, weight, targets, ignore_index: int, mean: bool | None):
-    """Kernels of the forward pass over prepared matrices: ``(row_loss, lse2, totals, loss)``.
-    ``mean`` None leaves out the reduction (totals and loss are None)."""
-    rows, vocab = hidden.shape[0], weight.shape[0]
+def _forward(hidden, weight, targets, ignore_index: int, mean: bool | None, row_loss):
+    """``(kept, loss)``: ``kept`` is lse2 of the rows and behind them the two totals.  Without a
+    tensor for them the rows' losses stay in scratch."""
+    rows = hidden.shape[0]
     dev = hidden.device
     handle = _lib.lib()
-    size = handle.sfl_linear_ce_part_bytes(rows, vocab)
-    part = torch.empty(size, dtype=torch.uint8, device=dev)
-    row_loss, lse2 = torch.empty(2, rows, dtype=torch.float32, device=dev).unbind(0)
-    reduce = mean is not None
-    totals, loss = None, None
-    if reduce:
-        totals = torch.empty(2, dtype=torch.float32, device=dev)
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-    args = _args(hidden, weight, targets, ignore_index, lse2)
+    size = handle.sfl_linear_ce_part_bytes(rows, weight.shape[0])
+    scratch = torch.empty(size + 4 * rows, dtype=torch.uint8, device=dev)
+    part = scratch.data_ptr()
+    kept = torch.empty(rows + 2, dtype=torch.float32, device=dev)
+    lse2 = kept.data_ptr()
+    loss = None if mean is None else torch.empty((), dtype=torch.float32, device=dev)
+    args = _call(hidden, weight, targets, ignore_index, lse2)
     with _lib.on_device(dev):
-        code = handle.sfl_linear_ce_fwd(byref(args), part.data_ptr(), size, row_loss.data_ptr(),
-                                        int(bool(mean)), _lib.ptr(totals), _lib.ptr(loss),
-                                        _lib.stream_ptr())
+        code = handle.sfl_linear_ce_fwd(args, part, size,
+                                        part + size if row_loss is None else row_loss.data_ptr(),
+                                        bool(mean), None if loss is None else lse2 + 4 * rows,
+                                        _lib.ptr(loss), _lib.stream_ptr())
     _lib.check(code, "sfl_linear_ce_fwd")
-    _lib.count_kernels(3 if reduce else 2)
-    return row_loss, lse2, totals, loss
+    _lib.count_kernels(2 if loss is None else 3)
+    return kept, loss
 
 
-def linear_ce_backward(hidden, weight, targets, ignore_index: int, lse2, grad, totals, dw,
-                       accumulate: bool = False, piece: int | None = None,
-                       need_dh: bool = True) -> torch.Tensor | None:
-    """Kernels of the backward pass: writes (or, for fp32 ``dw``, adds to) the weight gradient and
-    returns dh.  ``grad`` is a device scalar; with ``totals`` both are divided by the count.  Without
-    ``dw``, or without ``need_dh``, that product is not computed."""
+def _backward(hidden, weight, targets, ignore_index: int, lse2: int, grad, totals: int | None, dw,
+              accumulate: bool, piece: int | None, need_dh: bool) -> torch.Tensor | None:
     rows, dim = hidden.shape
     vocab = weight.shape[0]
     dev = hidden.device
@@ -148,43 +150,71 @@ def linear_ce_backward(hidden, weight, targets, ignore_index: int, lse2, grad, t
         raise ValueError("dw must be fp32, or of the operands' type when it is overwritten")
     if piece is None:
         piece = piece_size(rows, vocab)
-    dlogits = torch.empty(rows, piece, dtype=hidden.dtype, device=dev)
     dh = torch.empty(rows, dim, dtype=hidden.dtype, device=dev) if need_dh else None
-    args = _args(hidden, weight, targets, ignore_index, lse2)
+    args = _call(hidden, weight, targets, ignore_index, lse2)
     handle = _lib.lib()
     with _lib.on_device(dev):
-        size = (handle.sfl_linear_ce_dh_sum_bytes(rows, dim, vocab, piece, int(dw is not None))
+        size = (handle.sfl_linear_ce_dh_sum_bytes(rows, dim, vocab, piece, dw is not None)
                 if need_dh else 0)
-        dh_sum = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
-        grads = LinearCeGrad(grad=_lib.ptr(grad), totals=_lib.ptr(totals),
-                             dlogits=dlogits.data_ptr(), dh_sum=_lib.ptr(dh_sum), dh_sum_bytes=size,
-                             dh=_lib.ptr(dh), ld_dh=dim, dw=_lib.ptr(dw),
-                             ld_dw=0 if dw is None else dw.stride(0), dw_kind=kind, piece=piece)
-        code = handle.sfl_linear_ce_bwd(byref(args), byref(grads), _lib.stream_ptr())
+        dl_bytes = -(-2 * rows * piece // 256) * 256
+        scratch = torch.empty(dl_bytes + size, dtype=torch.uint8, device=dev)
+        dlogits = scratch.data_ptr()
+        grads = _GRAD.pack(0 if grad is None else grad.data_ptr(), totals or 0, dlogits,
+                           dlogits + dl_bytes if size > 0 else 0, size,
+                           0 if dh is None else dh.data_ptr(), dim,
+                           0 if dw is None else dw.data_ptr(), 0 if dw is None else dw.stride(0),
+                           kind, piece)
+        code = handle.sfl_linear_ce_bwd(args, grads, _lib.stream_ptr())
     _lib.check(code, "sfl_linear_ce_bwd")
-    _lib.count_kernels(2 * -(-vocab // piece) + (dh_sum is not None))
+    _lib.count_kernels(2 * -(-vocab // piece) + (size > 0))
     return dh
+
+
+def linear_ce_forward(hidden, weight, targets, ignore_index: int, mean: bool | None):
+    """Kernels of the forward pass over prepared matrices: ``(row_loss, lse2, totals, loss)``.
+    ``mean`` None leaves out the reduction (totals and loss are None)."""
+    rows = hidden.shape[0]
+    row_loss = torch.empty(rows, dtype=torch.float32, device=hidden.device)
+    kept, loss = _forward(hidden, weight, targets, ignore_index, mean, row_loss)
+    return row_loss, kept[:rows], None if mean is None else kept[rows:], loss
+
+
+def linear_ce_backward(hidden, weight, targets, ignore_index: int, lse2, grad, totals, dw,
+                       accumulate: bool = False, piece: int | None = None,
+                       need_dh: bool = True) -> torch.Tensor | None:
+    """Kernels of the backward pass: writes (or, for fp32 ``dw``, adds to) the weight gradient and
+    returns dh.  ``grad`` is a device scalar; with ``totals`` both are divided by the count.  Without
+    ``dw``, or without ``need_dh``, that product is not computed."""
+    return _backward(hidden, weight, targets, ignore_index, lse2.data_ptr(), grad, _lib.ptr(totals),
+                     dw, accumulate, piece, need_dh)
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, targets, ignore_index, mean):
         h, w = _rows(hidden), _rows(weight)
-        t = targets.reshape(-1).contiguous()
-        _, lse2, totals, loss = linear_ce_forward(h, w, t, ignore_index, mean)
-        ctx.save_for_backward(h, w, t, lse2, totals)
+        t = _flat(targets)
+        kept, loss = _forward(h, w, t, ignore_index, mean, None)
+        ctx.save_for_backward(h, w, t, kept)
         ctx.ignore_index, ctx.mean, ctx.shape = ignore_index, mean, hidden.shape
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        h, w, t, lse2, totals = ctx.saved_tensors
+        h, w, t, kept = ctx.saved_tensors
+        lse2 = kept.data_ptr()
         need_dh, need_dw = ctx.needs_input_grad[:2]      # a frozen head, or frozen hidden states
         dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if need_dw else None
-        dh = linear_ce_backward(h, w, t, ctx.ignore_index, lse2, grad.float(),
-                                totals if ctx.mean else None, dw, need_dh=need_dh)
-        return dh.view(ctx.shape) if need_dh else None, dw, None, None, None
+        dh = _backward(h, w, t, ctx.ignore_index, lse2, grad.float(),
+                       lse2 + 4 * h.shape[0] if ctx.mean else None, dw, False, None, need_dh)
+        if need_dh and dh.shape != ctx.shape:
+            dh = dh.view(ctx.shape)
+        return dh, dw, None, None, None
+
+
+def _flat(targets: torch.Tensor) -> torch.Tensor:
+    return targets if targets.ndim == 1 and targets.is_contiguous() else targets.reshape(-1).contiguous()
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: torch.Tensor, *,
@@ -218,7 +248,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, targets: to
     if needs_grad:
         return _LinearCrossEntropy.apply(hidden, weight, targets, ignore_index, reduction == "mean")
     h, w = _rows(hidden), _rows(weight)
-    t = targets.reshape(-1).contiguous()
-    mean = None if reduction == "none" else reduction == "mean"
-    row_loss, _, _, loss = linear_ce_forward(h, w, t, ignore_index, mean)
-    return row_loss.view(targets.shape) if mean is None else loss
+    t = _flat(targets)
+    if reduction == "none":
+        row_loss = torch.empty(targets.shape, dtype=torch.float32, device=hidden.device)
+        _forward(h, w, t, ignore_index, None, row_loss)
+        return row_loss
+    return _forward(h, w, t, ignore_index, reduction == "mean", None)[1]

@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import math
 from ctypes import POINTER, Structure, byref, c_float, c_int, c_long, c_void_p
+from functools import lru_cache
 
 import torch
 
@@ -103,6 +104,9 @@ def largest_singular_value(coefficients=QUINTIC, steps: int = 5) -> float:
     return worst
 
 
+_largest_singular_value = lru_cache(maxsize=64)(largest_singular_value)
+
+
 def _strided(update: torch.Tensor) -> torch.Tensor:
     """``update`` with rows the kernels can read (last dimension contiguous) and at most two
     leading dimensions; copies only what does not lie that way."""
@@ -155,7 +159,7 @@ def newton_schulz(update: torch.Tensor, *, steps: int = 5, coefficients=QUINTIC,
     a, b, c = (float(v) for v in coefficients)
     if not all(math.isfinite(v) for v in (a, b, c)):
         raise ValueError("coefficients must be finite")
-    if largest_singular_value((a, b, c), steps) > 2.0:
+    if _largest_singular_value((a, b, c), steps) > 2.0:
         raise ValueError("these coefficients let singular values exceed 2")
     m, n = update.shape[-2:]
     if max(m, n) >= 2**31:
