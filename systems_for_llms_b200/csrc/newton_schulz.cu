@@ -381,7 +381,6 @@ __device__ __forceinline__ void apply_begin(const ApplyView& p, const Tile& t, E
 __device__ __forceinline__ void apply_epilogue(const ApplyView& p, const Tile& t, EpiContext& c) {
   const int col0 = t.n0 + c.part * 128;
   if (c.row0 >= p.m) return;  // warp-uniform
-  const int row = c.row0 + c.lane;
 #pragma unroll 1
   for (int ch = 0; ch < 2; ++ch) {
     const int begin = col0 + ch * 64;
@@ -428,19 +427,27 @@ __device__ __forceinline__ void apply_epilogue(const ApplyView& p, const Tile& t
         }
         *qh = a;
         if (p.keep_lo) *ql = b;
-        if (p.last == 2 && row < p.m) {
-          const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&a);
-          const int col = begin + h * 32 + 8 * j;
-          __nv_bfloat16* dst = p.result + (static_cast<long>(t.z) * p.m + row) * p.n + col;
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            if (col + k < p.n) dst[k] = e[k];
-        }
       }
+    }
+    if (p.last == 2) {  // rows that TMA cannot address: written by the whole warp, row after row
+      __syncwarp();
+      const int rows = p.m - c.row0 < 32 ? p.m - c.row0 : 32, col = begin + c.lane;
+      uint16_t* dst = reinterpret_cast<uint16_t*>(p.result) +
+                      (static_cast<long>(t.z) * p.m + c.row0) * p.n + col;
+#pragma unroll 4
+      for (int r = 0; r < rows; ++r, dst += p.n) {
+        const int at = (c.lane & 7) * 2;
+        if (col < p.n)
+          dst[0] = *reinterpret_cast<const uint16_t*>(pair::tile_chunk(tile, r, c.lane >> 3) + at);
+        if (col + 32 < p.n)
+          dst[32] = *reinterpret_cast<const uint16_t*>(pair::tile_chunk(tile, r, 4 + (c.lane >> 3)) + at);
+      }
+      __syncwarp();
+      continue;
     }
     fence_proxy_async_smem();
     __syncwarp();
-    if (c.lane == 0 && p.last != 2) {
+    if (c.lane == 0) {
       if (p.last == 0) {
         pair::store_3d(p.hi_out, tile, begin, c.row0, t.z);
         if (p.keep_lo) pair::store_3d(p.lo, low, begin, c.row0, t.z);
