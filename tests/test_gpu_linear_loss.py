@@ -389,3 +389,24 @@ def test_kernels_are_counted(dev, rows, dim, vocab, piece):
     assert ctypes.CDLL("libcudart.so.12").cudaGraphGetNodes(
         ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(nodes)) == 0
     assert lib.launch_count() - before == nodes.value > 0
+
+
+def test_offsets_beyond_32_bits(dev):
+    from systems_for_llms_b200.ops.linear_loss import linear_ce_backward, linear_ce_forward
+    h, w, t = make(dev, 130, 64, 300, torch.bfloat16)
+    pitch = 2 ** 23                                    # 300 rows of it pass 2**31 elements
+
+    def both(h, w, dw):
+        rows, lse2, totals, loss = linear_ce_forward(h, w, t, -100, True)
+        return rows, loss, linear_ce_backward(h, w, t, -100, lse2, None, totals, dw)
+
+    want_dw = torch.empty(300, 64, device=dev)
+    want = both(h, w, want_dw)
+    store = torch.empty(299 * pitch + 128, dtype=torch.bfloat16, device=dev)
+    fw = store.as_strided((300, 64), (pitch, 1)).copy_(w)
+    fh = store.as_strided((130, 64), (pitch, 1), 64).copy_(h)
+    out = torch.empty(299 * pitch + 64, device=dev)
+    dw = out.as_strided((300, 64), (pitch, 1))
+    got = both(fh, fw, dw)
+    check(dev)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(dw, want_dw)

@@ -328,3 +328,18 @@ def test_kernels_are_counted(dev, shape, steps):
     assert ctypes.CDLL("libcudart.so.12").cudaGraphGetNodes(
         ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(nodes)) == 0
     assert lib.launch_count() - before == nodes.value > 0
+
+
+@pytest.mark.parametrize("m, n", [(96, 200), (200, 96), (200, 300), (300, 280)])
+def test_offsets_beyond_32_bits(dev, m, n):
+    from systems_for_llms_b200.ops.newton_schulz import newton_schulz
+    u = gradient(dev, 2, m, n).bfloat16()
+    want = newton_schulz(u)
+    pitch = -(-2 ** 31 // (m - 1)) + 8                 # a matrix whose last row is past 2**31
+    store = torch.empty((m - 1) * pitch + 2 * n + 8, dtype=torch.bfloat16, device=dev)
+    far = store.as_strided((2, m, n), (n + 4, pitch, 1)).copy_(u)
+    assert torch.equal(newton_schulz(far), want)
+    apart = torch.empty(2 ** 31 + m * n, dtype=torch.bfloat16, device=dev)
+    far = apart.as_strided((2, m, n), (2 ** 31, n, 1)).copy_(u)
+    assert torch.equal(newton_schulz(far), want)
+    check(dev)

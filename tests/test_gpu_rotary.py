@@ -296,3 +296,20 @@ def test_streams_and_graphs(dev):
         assert all(torch.equal(a, b) for a, b in zip(got, expected))
     direct = call(*sets[2])
     assert all(torch.equal(a, b) for a, b in zip(direct, want[2]))
+
+
+def test_offsets_beyond_32_bits(dev):
+    """Heads of one tensor 2**31 elements apart, as in a long cache, read and written in place."""
+    from systems_for_llms_b200.ops.rotary import qk_norm_rotary, qk_norm_rotary_grad
+    q, k, weights, grads = inputs(dev, torch.bfloat16, 1, 2, 2, 5, 64)
+    cos, sin = tables(dev, 64, 64)
+    kw = dict(eps=1e-5, layout="half")
+    want = qk_norm_rotary(q, k, *weights, cos, sin, **kw)
+    want_grads = qk_norm_rotary_grad(q, k, *weights, cos, sin, None, *grads, **kw)
+    store = torch.empty(2 ** 31 + 8192, dtype=torch.bfloat16, device=dev)
+    far = lambda at: store[at:].as_strided((1, 2, 5, 64), (64, 2 ** 31, 64, 1), store[at:].storage_offset())
+    fq, fk, fg, fh = (far(1024 * i).copy_(t) for i, t in enumerate((q, k, *grads)))
+    got = qk_norm_rotary_grad(fq, fk, *weights, cos, sin, None, fg, fh, out=(fg, fh), **kw)
+    assert all(torch.equal(a, b) for a, b in zip(got, want_grads))
+    got = qk_norm_rotary(fq, fk, *weights, cos, sin, out=(fq, fk), **kw)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
