@@ -20,20 +20,36 @@ inline bool pdl_enabled() {
   return on;
 }
 
+// The same in clusters of `cluster` CTAs (0: as the kernel says).
 template <typename Kernel, typename... Args>
-int launch_pdl(Kernel kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-               Args... args) {
+int launch_pdl_clusters(int cluster, Kernel kernel, dim3 grid, dim3 block, size_t smem,
+                        cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t config{};
   config.gridDim = grid;
   config.blockDim = block;
   config.dynamicSmemBytes = smem;
   config.stream = stream;
-  cudaLaunchAttribute attribute{};
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &attribute;
-  config.numAttrs = pdl_enabled() ? 1 : 0;
+  cudaLaunchAttribute attributes[2] = {};
+  int count = 0;
+  if (pdl_enabled()) {
+    attributes[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[count++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 0) {
+    attributes[count].id = cudaLaunchAttributeClusterDimension;
+    attributes[count].val.clusterDim.x = cluster;
+    attributes[count].val.clusterDim.y = 1;
+    attributes[count++].val.clusterDim.z = 1;
+  }
+  config.attrs = attributes;
+  config.numAttrs = count;
   return static_cast<int>(cudaLaunchKernelEx(&config, kernel, args...));
+}
+
+template <typename Kernel, typename... Args>
+int launch_pdl(Kernel kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+               Args... args) {
+  return launch_pdl_clusters(0, kernel, grid, block, smem, stream, args...);
 }
 
 }  // namespace sfl

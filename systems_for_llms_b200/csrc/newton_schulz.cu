@@ -789,7 +789,7 @@ ns_poly_kernel(const __grid_constant__ PolyParams p) {
   }
 }
 
-// --------------------------------------------------- a small matrix in one block ----
+// ------------------------------------------- a short-sided matrix that stays on chip ----
 // A matrix of at most 128 x 384 (either way round) fits on one SM and stays there from its norm to
 // its result: X as fp16 operand in shared memory, (a - k) X as fp32 in tensor memory, where the
 // product P X is added to it.  Nothing is rounded but the operands.  The block of 128 rows x 64
@@ -798,53 +798,96 @@ ns_poly_kernel(const __grid_constant__ PolyParams p) {
 // are taken transposed, X = U^T.  In the last two steps k = -(b + c), which makes P + k I vanish
 // where singular values are 1.
 //
-// One launch instead of seventeen; its time is the latency of three products and three passes
-// through registers per step (128 x 384, five steps: 38 us a call, where
-// the launch per product took 114).
+// Up to eight times longer matrices are shared by a cluster, 384 columns or fewer to each CTA.
+// Only the norm and G need the others: every CTA leaves its share of X X^T in shared memory, adds
+// the shares of some rows in a fixed order and stores the sum into all (96 KB a step and CTA);
+// polynomial and update are its own.
+//
+// One launch instead of twelve or more; its time is the latency of three products and three passes
+// through registers per step and, in a cluster, of two barriers and the exchange.  Five steps of
+// 128 x 384 take 38 us a call, where a launch per product took 114; 128 x 2000 65 us (128 with a
+// launch for G and P and one for X), 96 matrices of 100 x 2000 330 us (491).
 constexpr int kBlockRows = 128;
 constexpr int kBlockCols = 384;          // 512 columns of tensor memory less 128 of G
 constexpr int kBlockEpiWarps = 8;
 constexpr int kBlockThreads = 32 * (kBlockEpiWarps + 1);
 constexpr int kBlockBytes = kBlockRows * 128;  // 128 rows x 64 fp16
+constexpr int kMaxCluster = 8;                 // CTAs that share a matrix
+constexpr int kPartPitch = kBlockRows + 4;     // of a CTA's share of G: rows start four banks apart
+constexpr int kPartBytes = kBlockRows * kPartPitch * static_cast<int>(sizeof(float));
+
+// The same shared-memory offset in another CTA of the cluster, and accesses to it.
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 load_far(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ double load_far_double(uint32_t addr) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void store_far(uint32_t addr, uint32_t a, uint32_t b) {
+  asm volatile("st.shared::cluster.v2.b32 [%0], {%1, %2};" ::"r"(addr), "r"(a), "r"(b) : "memory");
+}
 
 struct BlockParams {
   Stack u;
   int m, n, wide, steps;
+  int cluster, share;       // CTAs per matrix, 64-column blocks of the longer side in each
   float a, b, c, eps;
   int vec_in, vec_out;      // rows may be read / written 16 bytes at a time (wide)
   __nv_bfloat16* out;
   int* status;
 };
 
-// 32 columns of a row of the result, back in the orientation of the matrix.
-__device__ __forceinline__ void block_store(const BlockParams& p, float (&v)[32], int row, int col0,
-                                            int longer) {
+// 32 columns of the warp's rows of the result, back in the orientation of the matrix.  `block` is
+// the operand block that held them, free by now.
+__device__ __forceinline__ void block_store(const BlockParams& p, float (&v)[32], int z, int row0,
+                                            int side, int col0, int longer, uint8_t* block, int half) {
+  const int lane = threadIdx.x & 31, row = row0 + lane;
 #pragma unroll
   for (int j = 0; j < 32; ++j) v[j] *= 1.0f / (kScale * kScale);
-  __nv_bfloat16* out = p.out + static_cast<long>(blockIdx.x) * p.m * p.n;
+  __nv_bfloat16* out = p.out + static_cast<long>(z) * p.m * p.n;
   if (!p.wide) {  // a warp's lanes are neighbours in memory
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      if (col0 + j < longer)
+      if (row < side && col0 + j < longer)
         out[static_cast<long>(col0 + j) * p.n + row] = __float2bfloat16_rn(v[j]);
     return;
   }
-  __nv_bfloat16* dst = out + static_cast<long>(row) * p.n + col0;
+  if (p.vec_out) {  // rows are whole groups of eight
+    __nv_bfloat16* dst = out + static_cast<long>(row) * p.n + col0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (p.vec_out && col0 + 8 * j + 8 <= longer) {
-      *reinterpret_cast<uint4*>(dst + 8 * j) =
-          make_uint4(pack_bf16(v[8 * j], v[8 * j + 1]), pack_bf16(v[8 * j + 2], v[8 * j + 3]),
-                     pack_bf16(v[8 * j + 4], v[8 * j + 5]), pack_bf16(v[8 * j + 6], v[8 * j + 7]));
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (col0 + 8 * j + e < longer) dst[8 * j + e] = __float2bfloat16_rn(v[8 * j + e]);
-    }
+    for (int j = 0; j < 4; ++j)
+      if (row < side && col0 + 8 * j < longer)
+        *reinterpret_cast<uint4*>(dst + 8 * j) =
+            make_uint4(pack_bf16(v[8 * j], v[8 * j + 1]), pack_bf16(v[8 * j + 2], v[8 * j + 3]),
+                       pack_bf16(v[8 * j + 4], v[8 * j + 5]), pack_bf16(v[8 * j + 6], v[8 * j + 7]));
+    return;
   }
+  pair::stage_16(block, row, half, v, false);  // row after row, lanes along the row
+  __syncwarp();
+  uint16_t* dst = reinterpret_cast<uint16_t*>(out) + static_cast<long>(row0) * p.n + col0 + lane;
+  const int rows = side - row0 < 32 ? side - row0 : 32;
+  if (col0 + lane < longer) {
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r, dst += p.n)
+      *dst = *reinterpret_cast<const uint16_t*>(
+          pair::tile_chunk(block, row0 + r, 4 * half + (lane >> 3)) + (lane & 7) * 2);
+  }
+  __syncwarp();
 }
 
-template <typename T>
+template <typename T, bool SHARED>
 __global__ void __launch_bounds__(kBlockThreads, 1)
 ns_block_kernel(const __grid_constant__ BlockParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -852,15 +895,22 @@ ns_block_kernel(const __grid_constant__ BlockParams p) {
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   __shared__ double sums[kBlockEpiWarps];
+  __shared__ double cta_sum;
   const uint32_t raw = smem_u32(smem_raw);
   uint8_t* op = smem_raw + (((raw + 1023u) & ~1023u) - raw);  // G, then P: two blocks
   uint8_t* xs = op + 2 * kBlockBytes;                         // X: up to six blocks
+  float* parts = reinterpret_cast<float*>(xs + p.share * kBlockBytes);  // this CTA's share of G
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int quarter = warp & 3, part = warp >> 2;
   const int row = quarter * 32 + lane;
   const int side = p.wide ? p.m : p.n, longer = p.wide ? p.n : p.m;
-  const int blocks = (longer + 63) >> 6;     // of X
+  const int cluster = SHARED ? p.cluster : 1;
+  const int rank = SHARED ? static_cast<int>(pair::cluster_rank()) : 0;
+  const int z = SHARED ? blockIdx.x / cluster : blockIdx.x;
+  const int first = rank * p.share * 64;     // column of the longer side
+  const int left = longer - first;
+  const int blocks = left >= p.share * 64 ? p.share : (left + 63) >> 6;  // of X
   const int chunks = 2 * blocks;             // of 32 columns; a warp takes every other one
   const uint32_t columns = blocks <= 2 ? 256 : 512;  // of tensor memory: 128 of G, 64 per block
   const int side_blocks = (side + 63) >> 6;  // of G and P
@@ -913,24 +963,24 @@ ns_block_kernel(const __grid_constant__ BlockParams p) {
   auto held = [&](int step) { return step + 2 >= p.steps && p.b + p.c < 0.f ? -(p.b + p.c) : 0.f; };
 
   // ---- the matrix into tensor memory, its norm, then both forms of X
-  const T* u = matrix<T>(p.u, blockIdx.x);
+  const T* u = matrix<T>(p.u, z);
   double sum = 0.0;
   if (warp < kBlockEpiWarps) {
     for (int ch = part; ch < chunks; ch += 2) {
       float v[32];
       if (p.wide) {
-        const T* src = u + static_cast<long>(row < side ? row : 0) * p.u.row + ch * 32;
+        const T* src = u + static_cast<long>(row < side ? row : 0) * p.u.row + first + ch * 32;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           float q[4];
-          load4(src, 4 * j, row < side ? longer - ch * 32 : 0, p.vec_in, q);
+          load4(src, 4 * j, row < side ? left - ch * 32 : 0, p.vec_in, q);
 #pragma unroll
           for (int k = 0; k < 4; ++k) v[4 * j + k] = q[k];
         }
       } else {
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
-          const int l = ch * 32 + j;
+          const int l = first + ch * 32 + j;
           v[j] = row < side && l < longer ? wide(u[static_cast<long>(l) * p.u.row + row]) : 0.f;
         }
       }
@@ -944,10 +994,24 @@ ns_block_kernel(const __grid_constant__ BlockParams p) {
     if (lane == 0) sums[warp] = sum;
   }
   __syncthreads();
+  if constexpr (SHARED) {
+    if (threadIdx.x == 0) {
+      sum = 0.0;
+#pragma unroll
+      for (int k = 0; k < kBlockEpiWarps; ++k) sum += sums[k];
+      cta_sum = sum;
+    }
+    __syncwarp();
+    pair::cluster_sync();
+  }
   if (warp < kBlockEpiWarps) {
     sum = 0.0;
+    if constexpr (SHARED) {
+      for (int k = 0; k < cluster; ++k) sum += load_far_double(in_cta(smem_u32(&cta_sum), k));
+    } else {
 #pragma unroll
-    for (int k = 0; k < kBlockEpiWarps; ++k) sum += sums[k];
+      for (int k = 0; k < kBlockEpiWarps; ++k) sum += sums[k];
+    }
     const float inv = static_cast<float>(kScale / (sqrt(sum) + static_cast<double>(p.eps)));
     const float ahead = (p.a - held(0)) * kScale;
     for (int ch = part; ch < chunks; ch += 2) {
@@ -997,8 +1061,41 @@ ns_block_kernel(const __grid_constant__ BlockParams p) {
         pair::load_acc(mine + part * 64 + h * 32, v);
 #pragma unroll
         for (int j = 0; j < 32; ++j) v[j] *= 1.0f / kScale;
-        pair::stage_16(op + part * kBlockBytes, row, h, v, true);
+        if constexpr (SHARED) {
+          float4* dst = reinterpret_cast<float4*>(parts + row * kPartPitch + part * 64 + h * 32);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            dst[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        } else {
+          pair::stage_16(op + part * kBlockBytes, row, h, v, true);
+        }
       }
+    }
+    if constexpr (SHARED) {
+      // Every CTA adds the shares of its rows of G, in order, and leaves the sum with all.  The
+      // others' products read G only after the second barrier, and nobody rewrites a share before it.
+      pair::cluster_sync();
+      const int col = 4 * lane;
+      if (warp < kBlockEpiWarps && col < side_blocks * 64) {
+        const uint32_t from = smem_u32(parts + col);
+#pragma unroll 2
+        for (int r = rank + cluster * warp; r < kBlockRows; r += cluster * kBlockEpiWarps) {
+          float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int k = 0; k < kMaxCluster; ++k) {
+            if (k >= cluster) break;
+            const float4 q = load_far(in_cta(from + r * kPartPitch * static_cast<int>(sizeof(float)), k));
+            g = make_float4(g.x + q.x, g.y + q.y, g.z + q.z, g.w + q.w);
+          }
+          const uint32_t lo = pair::pack_16(true, g.x, g.y), hi = pair::pack_16(true, g.z, g.w);
+          const uint32_t to = smem_u32(pair::tile_chunk(op + (col >> 6) * kBlockBytes, r, (col & 63) >> 3)) +
+                              (col & 7) * 2;
+          for (int k = 0; k < cluster; ++k) store_far(in_cta(to, k), lo, hi);
+        }
+        fence_proxy_async();
+      }
+      __syncwarp();
+      pair::cluster_sync();
     }
     operands_written();
     square(op_k, side_blocks);
@@ -1047,8 +1144,9 @@ ns_block_kernel(const __grid_constant__ BlockParams p) {
           }
           pair::stage_16(xs + (ch >> 1) * kBlockBytes, row, ch & 1, h, true);
           to_tmem(mine + x_acc + ch * 32, v);
-        } else if (row < side) {
-          block_store(p, v, row, ch * 32, longer);
+        } else {
+          block_store(p, v, z, quarter * 32, side, first + ch * 32, longer,
+                      xs + (ch >> 1) * kBlockBytes, ch & 1);
         }
         __syncwarp();  // tensor memory is read by whole warps
       }
@@ -1108,13 +1206,19 @@ int normalise(const Stack& s, int batch, int m, int n, int ld, float eps, double
                     ld, vec, static_cast<const double*>(partial), eps, hi, lo);
 }
 
-bool fits_block(int m, int n) {
+// A matrix stays on chip up to 128 x 384 for each of at most eight CTAs.  It takes as few as hold
+// it, whatever the stack: the order of G's sum, and with it the last bits of the result, then do not
+// depend on its neighbours.  (More CTAs are sooner done with one matrix and later with many: 128 x
+// 1000 in three takes 60 us and 32 of them 63, in eight 48 and 144.)
+bool fits_blocks(int m, int n) {
   const int side = m < n ? m : n, longer = m < n ? n : m;
-  return side <= kBlockRows && longer <= kBlockCols;
+  return side <= kBlockRows && longer <= kMaxCluster * kBlockCols;
 }
 
 template <typename T>
 int launch_block(const SflNewtonSchulz& a, const Stack& s, cudaStream_t stream) {
+  const int blocks = tiles_of(a.m < a.n ? a.n : a.m, 64);
+  const int cluster = tiles_of(blocks, kBlockCols / 64);
   BlockParams p{};
   p.u = s;
   p.m = a.m;
@@ -1129,13 +1233,17 @@ int launch_block(const SflNewtonSchulz& a, const Stack& s, cudaStream_t stream) 
   p.vec_out = a.n % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
   p.out = static_cast<__nv_bfloat16*>(a.out);
   p.status = a.status;
-  const int longer = a.m < a.n ? a.n : a.m;
-  const int smem = 1024 + (2 + tiles_of(longer, 64)) * kBlockBytes;
-  const cudaError_t e = cudaFuncSetAttribute(
-      ns_block_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-      1024 + (2 + kBlockCols / 64) * kBlockBytes);
-  if (e != cudaSuccess) return static_cast<int>(e);
-  return launch_pdl(ns_block_kernel<T>, dim3(a.batch), dim3(kBlockThreads), smem, stream, p);
+  p.cluster = cluster;  // every CTA has a block: share (cluster - 1) < blocks
+  p.share = tiles_of(blocks, cluster);
+  auto go = [&](auto kernel, int extra) -> int {
+    const cudaError_t e =
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             1024 + (2 + kBlockCols / 64) * kBlockBytes + extra);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    return launch_pdl_clusters(extra > 0 ? cluster : 0, kernel, dim3(a.batch * cluster), dim3(kBlockThreads),
+                               1024 + (2 + p.share) * kBlockBytes + extra, stream, p);
+  };
+  return cluster == 1 ? go(ns_block_kernel<T, false>, 0) : go(ns_block_kernel<T, true>, kPartBytes);
 }
 
 int launch_poly(const PolyParams& p, cudaStream_t stream) {
@@ -1190,7 +1298,7 @@ extern "C" long sfl_newton_schulz_bytes(int batch, int m, int n) {
 
 extern "C" int sfl_newton_schulz_kernels(int m, int n, int steps) {
   using namespace sfl;
-  if (fits_block(m, n)) return 1;
+  if (fits_blocks(m, n)) return 1;
   return 2 + steps * ((m < n ? m : n) <= pair::kTileN ? 2 : 3);
 }
 
@@ -1210,7 +1318,7 @@ extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
 
   const Stack s{a->update, a->stride0, a->stride1, a->row, a->inner};
-  if (fits_block(m, n)) {
+  if (fits_blocks(m, n)) {
     if (a->dtype == 0) return launch_block<__nv_bfloat16>(*a, s, stream);
     if (a->dtype == 1) return launch_block<__half>(*a, s, stream);
     return launch_block<float>(*a, s, stream);

@@ -343,3 +343,35 @@ def test_offsets_beyond_32_bits(dev, m, n):
     far = apart.as_strided((2, m, n), (2 ** 31, n, 1)).copy_(u)
     assert torch.equal(newton_schulz(far), want)
     check(dev)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(128, 385), (96, 1000), (1000, 96), (50, 2000), (2, 2500), (1, 700),
+                                   (1601, 128), (65, 769), (2049, 33)])
+def test_matrices_shared_by_several_blocks(dev, shape, dtype):
+    from systems_for_llms_b200.ops.newton_schulz import newton_schulz
+    u = gradient(dev, *shape, dtype=dtype, seed=5)
+    compare(newton_schulz(u), u)
+    check(dev)
+
+
+def test_stacks_of_shared_matrices(dev):
+    from systems_for_llms_b200.ops.newton_schulz import newton_schulz
+    for m, n in ((70, 900), (900, 70)):
+        u = gradient(dev, 3, 7, m, n, seed=6)
+        u[1, 2] = 0
+        u[2, 3, 4, 5] = float("nan")
+        got = newton_schulz(u)
+        check(dev)
+        assert (got[1, 2] == 0).all() and got[2, 3].isnan().all()
+        for i, j in ((0, 0), (1, 1), (1, 3), (2, 2), (2, 4), (2, 6)):
+            assert torch.equal(newton_schulz(u[i, j]), got[i, j])
+            compare(got[i, j], u[i, j])
+        flat = torch.zeros(3, 9, m + 2, n + 4, device=dev)
+        view = flat[:, 1:8, 1:m + 1, 3:n + 3].copy_(u)
+        again = newton_schulz(view)
+        assert torch.equal(again.nan_to_num(7.0), got.nan_to_num(7.0))
+    many = gradient(dev, 200, 40, 500, seed=7)
+    got = newton_schulz(many)
+    assert torch.equal(got[173], newton_schulz(many[173]))
+    check(dev)
