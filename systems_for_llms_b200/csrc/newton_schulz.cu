@@ -472,8 +472,6 @@ struct ApplyOp : pair::NoMaps, pair::RoundRobin {
     int* status;
     int mt, per;
     int m, n;
-    int band;                  // row tiles that are walked before the next column tile
-    int nt;
     int wide;                  // A = P and B = X (MN-major), else A = X and B = P
     int folded;                // 1: P holds a X as well; hi + lo of X are not read
     int keep_lo;               // 1: write lo of the next X
@@ -483,12 +481,8 @@ struct ApplyOp : pair::NoMaps, pair::RoundRobin {
   };
   static __device__ __forceinline__ Tile tile(const Params& p, int w) {
     const int z = w / p.per;
-    int in = w - z * p.per;
-    const int b = in / (p.band * p.nt);
-    in -= b * p.band * p.nt;
-    const int width = p.mt - b * p.band < p.band ? p.mt - b * p.band : p.band;
-    const int n = in / width;
-    const int m = b * p.band + in - n * width;
+    const int in = w - z * p.per;
+    const int n = in / p.mt, m = in - n * p.mt;
     return Tile{m * pair::kTileM, n * pair::kTileN, z, p.num_kb, 0, p.wide,
                 p.wide ? turn(m) : 0, p.wide ? p.num_kb : turn(n), false};
   }
@@ -1357,8 +1351,6 @@ extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {
   x.per = mt * nt;
   x.total = batch * x.per;
   x.num_kb = tiles_of(side, pair::kBK);
-  x.nt = nt;
-  x.band = mt < 8 ? mt : 8;
   x.m = m;
   x.n = n;
   x.wide = wide;
