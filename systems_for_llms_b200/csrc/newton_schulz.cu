@@ -77,6 +77,14 @@ __device__ __forceinline__ void load4(const T* row, int c, int n, bool vec, floa
   }
 }
 
+// kScale / (norm + eps) as a power of two and the rest, neither of which leaves the fp32 range: the
+// norm of fp32 entries spans 2^-149 to 2^140.
+__device__ __forceinline__ float2 inverse_norm(double square_sum, float eps) {
+  const double inv = kScale / (sqrt(square_sum) + static_cast<double>(eps));
+  const double power = inv > 1e30 ? 0x1p100 : (inv < 1e-30 ? 0x1p-40 : 1.0);
+  return make_float2(static_cast<float>(power), static_cast<float>(inv / power));
+}
+
 // A block's share of a matrix: its threads lie side by side along a row (or along several short
 // rows), and each visits kDepth rows at a time so that as many loads are in flight.
 constexpr int kDepth = 4;
@@ -136,7 +144,7 @@ template <typename T>
 __global__ void __launch_bounds__(kNormThreads)
 ns_split_kernel(Stack s, int m, int n, int ld, int vec, const double* __restrict__ partial,
                 float eps, __half* __restrict__ hi, __half* __restrict__ lo /* may be NULL */) {
-  __shared__ float inv_sh;
+  __shared__ float2 inv_sh;
   pdl_launch_dependents();
   pdl_wait();
   const int z = blockIdx.y;
@@ -147,10 +155,10 @@ ns_split_kernel(Stack s, int m, int n, int ld, int vec, const double* __restrict
     if (threadIdx.x + 32 < gridDim.x) sum += mine[threadIdx.x + 32];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (threadIdx.x == 0) inv_sh = static_cast<float>(kScale / (sqrt(sum) + static_cast<double>(eps)));
+    if (threadIdx.x == 0) inv_sh = inverse_norm(sum, eps);
   }
   __syncthreads();
-  const float inv = inv_sh;
+  const float2 inv = inv_sh;
   const T* src = matrix<T>(s, z);
   const long out0 = static_cast<long>(z) * m * ld;
   const int quads = ld >> 2;
@@ -168,7 +176,7 @@ ns_split_kernel(Stack s, int m, int n, int ld, int vec, const double* __restrict
       __half h[4], l[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float x = v[d][j] * inv;
+        const float x = v[d][j] * inv.x * inv.y;
         h[j] = __float2half_rn(x);
         l[j] = __float2half_rn(x - __half2float(h[j]));
       }
@@ -1006,13 +1014,13 @@ ns_block_kernel(const __grid_constant__ BlockParams p) {
 #pragma unroll
       for (int k = 0; k < kBlockEpiWarps; ++k) sum += sums[k];
     }
-    const float inv = static_cast<float>(kScale / (sqrt(sum) + static_cast<double>(p.eps)));
+    const float2 inv = inverse_norm(sum, p.eps);
     const float ahead = (p.a - held(0)) * kScale;
     for (int ch = part; ch < chunks; ch += 2) {
       float v[32];
       pair::load_acc(mine + x_acc + ch * 32, v);
 #pragma unroll
-      for (int j = 0; j < 32; ++j) v[j] *= inv;
+      for (int j = 0; j < 32; ++j) v[j] = v[j] * inv.x * inv.y;
       pair::stage_16(xs + (ch >> 1) * kBlockBytes, row, ch & 1, v, true);
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] *= ahead;

@@ -137,7 +137,8 @@ def newton_schulz(update: torch.Tensor, *, steps: int = 5, coefficients=QUINTIC,
     parameter of all layers inside a flat buffer is one call).  The result is bf16, contiguous,
     computed with fp16 operands whose rounding does not compound (off by about 0.002 of its norm,
     rounding to bf16 included; the normalised matrix is held to 2^-37 absolutely, which only shows
-    where ``eps`` dwarfs the norm and the result is far below 1).  A matrix of zeros gives zeros; one that holds an infinity or NaN
+    where ``eps`` dwarfs the norm and the result is far below 1).  A matrix of zeros gives zeros
+    (NaN, as 0 / 0 is, where ``eps`` is 0); one that holds an infinity or NaN
     gives NaN without touching its neighbours.  ``out`` receives the result; it may be a contiguous
     bf16 ``update`` itself and is otherwise refused when it lies within the bytes the update spans.  Coefficients under
     which singular values starting below 1 exceed 2 are refused: the operands are scaled for

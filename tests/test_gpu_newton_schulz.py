@@ -375,3 +375,17 @@ def test_stacks_of_shared_matrices(dev):
     got = newton_schulz(many)
     assert torch.equal(got[173], newton_schulz(many[173]))
     check(dev)
+
+
+@pytest.mark.parametrize("shape", [(40, 72), (64, 500), (200, 300), (300, 280)])
+def test_norms_at_the_ends_of_the_range(dev, shape):
+    """Entries that are subnormal, or so large that their norm is not an fp32 number.  Scaling by
+    powers of two is exact, so the bound is the ordinary one."""
+    from systems_for_llms_b200.ops.newton_schulz import newton_schulz
+    u = torch.randn(shape, device=dev).clamp(-3, 3)
+    for scale in (2.0 ** -140, 2.0 ** -120, 2.0 ** 126):
+        scaled = (u.double() * scale).float()
+        assert scaled.isfinite().all() and (scaled != 0).any()
+        compare(newton_schulz(scaled, eps=0.0), scaled, eps=0.0)
+    assert newton_schulz(torch.zeros(shape, device=dev), eps=0.0).isnan().all()
+    check(dev)
