@@ -1379,16 +1379,40 @@ extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {
     return pair::map_3d(map, v, 2, n, m, z.ld, batch, x_stride, 64, 32);
   };
 
+  // Encoding a map takes the host as long as a product takes a small matrix: each is made once.
+  struct {
+    CUtensorMap gram_x[2], apply_x[2], x[2], lo, gram, gram_k, gram_mn, poly, poly_k, poly_mn, out;
+  } maps;
+  const bool fused_poly = side <= pair::kTileN;
+  rc = 0;
+  for (int i = 0; i < 2 && rc == 0; ++i) {
+    rc = pair::map_operand(&maps.gram_x[i], hi[i], !wide, side, longer, z.ld, batch, x_stride);
+    if (rc == 0)
+      rc = wide ? pair::map_operand(&maps.apply_x[i], hi[i], true, n, m, z.ld, batch, x_stride)
+                : pair::map_operand(&maps.apply_x[i], hi[i], false, m, n, z.ld, batch, x_stride);
+    if (rc == 0) rc = x_map(&maps.x[i], hi[i]);
+  }
+  if (rc == 0) rc = x_map(&maps.lo, lo);
+  if (rc == 0 && !fused_poly) rc = gram_map(&maps.gram, gram);
+  if (rc == 0 && !fused_poly) rc = symmetric(&maps.gram_k, &maps.gram_mn, gram);
+  if (rc == 0) rc = gram_map(&maps.poly, poly);
+  if (rc == 0) rc = symmetric(&maps.poly_k, &maps.poly_mn, poly);
+  if (rc == 0 && out_tma)
+    rc = pair::map_3d(&maps.out, a->out, 2, n, m, n, batch, static_cast<uint64_t>(m) * n, 64, 32);
+  if (rc != 0) return 1000 + rc;
+  x.lo = maps.lo;
+  x.p_k = maps.poly_k;
+  x.p_mn = maps.poly_mn;
+  if (out_tma) x.out = maps.out;
+
   for (int step = 0; step < a->steps; ++step) {
-    __half* now = hi[step & 1];
-    __half* next = hi[(step + 1) & 1];
+    const int now = step & 1;
     const bool folded = step + 2 >= a->steps;
     const float k = folded ? a->a : 0.f;
-    if (side <= pair::kTileN) {
+    if (fused_poly) {
       PolyParams g{};
-      rc = pair::map_operand(&g.x, now, !wide, side, longer, z.ld, batch, x_stride);
-      if (rc == 0) rc = gram_map(&g.out, poly);
-      if (rc != 0) return 1000 + rc;
+      g.x = maps.gram_x[now];
+      g.out = maps.poly;
       g.batch = batch;
       g.size = side;
       g.wide = wide;
@@ -1408,10 +1432,8 @@ extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {
       q.alpha = 0.f;
       q.beta = 1.0f / kScale;
       q.shift = 0.f;
-      rc = pair::map_operand(wide ? &q.k_major : &q.mn_major, now, !wide, side, longer, z.ld, batch,
-                             x_stride);
-      if (rc == 0) rc = gram_map(&q.out, gram);
-      if (rc != 0) return 1000 + rc;
+      (wide ? q.k_major : q.mn_major) = maps.gram_x[now];
+      q.out = maps.gram;
       rc = pair::launch_pair<SymOp>(q, stream);
       if (rc != 0) return rc;
       // P = b G + c G G (+ a I)
@@ -1420,10 +1442,10 @@ extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {
       q.alpha = a->b;
       q.beta = a->c / kScale;
       q.shift = k * kScale;
-      q.aux = q.out;
-      rc = symmetric(&q.k_major, &q.mn_major, gram);
-      if (rc == 0) rc = gram_map(&q.out, poly);
-      if (rc != 0) return 1000 + rc;
+      q.k_major = maps.gram_k;
+      q.mn_major = maps.gram_mn;
+      q.aux = maps.gram;
+      q.out = maps.poly;
       rc = pair::launch_pair<SymOp>(q, stream);
       if (rc != 0) return rc;
     }
@@ -1435,16 +1457,9 @@ extern "C" int sfl_newton_schulz(const SflNewtonSchulz* a, void* stream_) {
     x.keep_lo = step + 3 < a->steps;  // the next step is not folded either
     x.alpha = (a->a - k) * unscale;
     x.beta = unscale / kScale;
-    rc = symmetric(&x.p_k, &x.p_mn, poly);
-    if (rc == 0)
-      rc = wide ? pair::map_operand(&x.x, now, true, n, m, z.ld, batch, x_stride)
-                : pair::map_operand(&x.x, now, false, m, n, z.ld, batch, x_stride);
-    if (rc == 0) rc = x_map(&x.hi, now);
-    if (rc == 0) rc = x_map(&x.lo, lo);
-    if (rc == 0) rc = x_map(&x.hi_out, next);
-    if (rc == 0 && x.last == 1)
-      rc = pair::map_3d(&x.out, a->out, 2, n, m, n, batch, static_cast<uint64_t>(m) * n, 64, 32);
-    if (rc != 0) return 1000 + rc;
+    x.x = maps.apply_x[now];
+    x.hi = maps.x[now];
+    x.hi_out = maps.x[now ^ 1];
     rc = pair::launch_pair<ApplyOp>(x, stream);
     if (rc != 0) return rc;
   }
