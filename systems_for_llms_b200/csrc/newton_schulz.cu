@@ -731,7 +731,7 @@ ns_poly_kernel(const __grid_constant__ PolyParams p) {
         pair::stage_16(op + (col >> 6) * pair::kABytes, row, (col >> 5) & 1, v, true);
       }
       // both CTAs' shared memory is read by the products that the leader issues
-      asm volatile("fence.proxy.async;" ::: "memory");
+      fence_proxy_async();
       tc_fence_before();
       __syncwarp();
       if (lane == 0)

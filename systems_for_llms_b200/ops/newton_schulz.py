@@ -140,9 +140,9 @@ def newton_schulz(update: torch.Tensor, *, steps: int = 5, coefficients=QUINTIC,
     where ``eps`` dwarfs the norm and the result is far below 1).  A matrix of zeros gives zeros
     (NaN, as 0 / 0 is, where ``eps`` is 0); one that holds an infinity or NaN
     gives NaN without touching its neighbours.  ``out`` receives the result; it may be a contiguous
-    bf16 ``update`` itself and is otherwise refused when it lies within the bytes the update spans.  Coefficients under
-    which singular values starting below 1 exceed 2 are refused: the operands are scaled for
-    bounded ones.  The operator is not differentiable.
+    bf16 ``update`` itself and is otherwise refused when it lies within the bytes the update spans.
+    Coefficients under which singular values starting below 1 exceed 2 are refused: the operands are
+    scaled for bounded ones.  The operator is not differentiable.
     """
     if not isinstance(update, torch.Tensor) or not update.is_cuda:
         raise ValueError("update must be a CUDA tensor")
@@ -160,7 +160,9 @@ def newton_schulz(update: torch.Tensor, *, steps: int = 5, coefficients=QUINTIC,
     a, b, c = (float(v) for v in coefficients)
     if not all(math.isfinite(v) for v in (a, b, c)):
         raise ValueError("coefficients must be finite")
-    if _largest_singular_value((a, b, c), steps) > 2.0:
+    # Bounded by 2 on [0, 1], |a| is at most 10 and |b s^2 + c s^4| at most 14 (twice Chebyshev's
+    # polynomial of degree five is the extreme), which fp16 holds times 2^12.
+    if _largest_singular_value((a, b, c), steps) > 2.0 * (1 + 1e-12):      # a rounding above is 2
         raise ValueError("these coefficients let singular values exceed 2")
     m, n = update.shape[-2:]
     if max(m, n) >= 2**31:

@@ -389,3 +389,19 @@ def test_norms_at_the_ends_of_the_range(dev, shape):
         compare(newton_schulz(scaled, eps=0.0), scaled, eps=0.0)
     assert newton_schulz(torch.zeros(shape, device=dev), eps=0.0).isnan().all()
     check(dev)
+
+
+@pytest.mark.parametrize("shape", [(40, 72), (64, 500), (200, 300), (300, 280)])
+def test_the_largest_coefficients(dev, shape):
+    """Twice Chebyshev's polynomial of degree five reaches 2 and has the largest coefficients that
+    are accepted; with singular values spread over [0, 1] the operands come to their extremes."""
+    from systems_for_llms_b200.ops.newton_schulz import newton_schulz
+    u = gradient(dev, *shape)
+    left, values, right = torch.linalg.svd(u.double(), full_matrices=False)
+    spread = torch.linspace(0, 1, values.numel(), device=dev, dtype=torch.float64)
+    for few in (spread[-1:], spread):      # one singular value of the whole norm, or all of them
+        sv = torch.cat([few, few.new_zeros(values.numel() - few.numel())])
+        x = (left * sv @ right).float()
+        got = newton_schulz(x, steps=1, coefficients=(10.0, -40.0, 32.0), eps=0.0)
+        check(dev)
+        compare(got, x, steps=1, coefficients=(10.0, -40.0, 32.0), eps=0.0)
